@@ -3,7 +3,8 @@
 Three hand-written sm_100a kernels (W8A8 s8 GEMM, FP8 e4m3 GEMM, int8 decode
 GEMV) exported as flat C symbols (include/baracuda_kernels_q.h) and wrapped by
 typed plans that mirror the reference's `select / can_implement /
-workspace_size / run / sku` contract.
+workspace_size / run / sku` contract, and the attention step between a layer's
+quantized projections: norms and rotation, a paged 4-bit cache, attention over it.
 """
 from .vocab import (  # noqa: F401
     ArchSku,
@@ -49,4 +50,19 @@ from .plans import (  # noqa: F401
     W8A8GemmPlan,
     device_status,
     set_tuning,
+)
+from .kv4 import (  # noqa: F401
+    Kv4AppendArgs,
+    Kv4AppendDescriptor,
+    Kv4AppendPlan,
+    Kv4AttentionArgs,
+    Kv4AttentionDescriptor,
+    Kv4AttentionPlan,
+    Kv4CacheDescriptor,
+    Kv4ReadArgs,
+    Kv4ReadDescriptor,
+    Kv4ReadPlan,
+    QkNormRopeArgs,
+    QkNormRopeDescriptor,
+    QkNormRopePlan,
 )

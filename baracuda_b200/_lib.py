@@ -21,6 +21,10 @@ _GEMV_HEAD = [_i32, _i32, _i32, _i32, _i32, _f32, _f32, _vp, _i64, _i64, _vp, _i
 _GEMV_CAN = (_i32, [_i32] * 5 + [_i64] * 6)
 _GEMV_WS = (_sz, [_i32] * 5)
 
+_QK_IN = [_i32] * 4 + [_vp, _i64, _vp, _i64]  # tokens, heads, head_dim, q, k
+_QK_TURN = [_vp, _vp, _f32, _vp, _i32, _i32, _i32, _vp, _i64, _i32, _vp]  # weights, angles, positions
+_KV4_CACHE = [_vp, _i64, _i32, _i32]  # cache, page_stride, num_pages, page_size
+
 # symbol -> (restype, argtypes); every symbol the header declares is listed here
 SIGNATURES: dict[str, tuple] = {
     "baracuda_kernels_gemm_w8a8_s8_rcr_bf16_sm100a_run": (_i32, _GEMM_PREFIX + [_vp, _vp, _f32, _f32] + _TAIL),
@@ -135,6 +139,24 @@ SIGNATURES: dict[str, tuple] = {
     "baracuda_kernels_gemm_fp8_e4m3_rcr_bf16_sm100a_swiglu_can_implement": (
         _i32, [_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64]),
     "baracuda_kernels_q_interleave_gate_up_run": (_i32, [_i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "baracuda_kernels_kv4_page_bytes": (_sz, [_i32] * 3),
+    "baracuda_kernels_qk_norm_rope_bf16_sm100a_run": (_i32, _QK_IN + _QK_TURN + [_vp, _i64, _vp, _i64] + _TAIL),
+    "baracuda_kernels_qk_norm_rope_bf16_sm100a_can_implement": (_i32, [_i32] * 6),
+    "baracuda_kernels_qk_norm_rope_bf16_sm100a_workspace_size": (_sz, [_i32] * 4),
+    "baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_run": (
+        _i32, _QK_IN + [_vp, _i64] + _QK_TURN + [_vp, _i64] + _KV4_CACHE + [_vp] + _TAIL),
+    "baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_can_implement": (_i32, [_i32] * 7),
+    "baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_workspace_size": (_sz, [_i32] * 4),
+    "baracuda_kernels_kv4_append_bf16_sm100a_run": (_i32, [_i32] * 3 + [_vp, _i64, _vp, _i64] + _KV4_CACHE + [_vp] + _TAIL),
+    "baracuda_kernels_kv4_append_bf16_sm100a_can_implement": (_i32, [_i32] * 4),
+    "baracuda_kernels_kv4_append_bf16_sm100a_workspace_size": (_sz, [_i32] * 3),
+    "baracuda_kernels_kv4_read_bf16_sm100a_run": (_i32, [_i32] * 3 + _KV4_CACHE + [_vp] + [_vp, _i64, _vp, _i64] + _TAIL),
+    "baracuda_kernels_kv4_read_bf16_sm100a_can_implement": (_i32, [_i32] * 4),
+    "baracuda_kernels_kv4_read_bf16_sm100a_workspace_size": (_sz, [_i32] * 3),
+    "baracuda_kernels_attention_kv4_bf16_sm100a_run": (
+        _i32, [_i32] * 7 + [_vp, _i64, _vp] + _KV4_CACHE + [_vp, _i64, _vp, _f32, _i32, _i32, _vp, _i64, _vp] + _TAIL),
+    "baracuda_kernels_attention_kv4_bf16_sm100a_can_implement": (_i32, [_i32] * 7),
+    "baracuda_kernels_attention_kv4_bf16_sm100a_workspace_size": (_sz, [_i32] * 6),
     "baracuda_q_nccl_version": (_i32, []),
     "baracuda_q_nccl_unique_id": (_i32, [_vp]),
     "baracuda_q_nccl_comm_init_rank": (_i32, [C.POINTER(_vp), _i32, _vp, _i32]),

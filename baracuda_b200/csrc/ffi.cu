@@ -4,6 +4,7 @@
 // launch.  No allocation, no host synchronisation, no library state.
 
 #include "../../include/baracuda_kernels_q.h"
+#include "kv4_format.cuh"
 #include "launch.h"
 
 namespace {
@@ -883,6 +884,10 @@ int32_t baracuda_kernels_q_device_status(void) {
     int32_t gemv = bq::read_and_clear_gemv_device_status();
     const int32_t barrier = bq::read_and_clear_peer_barrier_device_status();
     if (gemv == 0) gemv = barrier;
+    const int32_t append = bq::read_and_clear_kv4_append_device_status();
+    if (gemv == 0) gemv = append;
+    const int32_t attention = bq::read_and_clear_kv4_attention_device_status();
+    if (gemv == 0) gemv = attention;
     return gemm != 0 ? gemm : gemv;
 }
 

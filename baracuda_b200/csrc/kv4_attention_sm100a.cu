@@ -1,0 +1,691 @@
+// Attention of a few query rows per sequence over the 4-bit cache (kv4_format.cuh).
+//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j]) v[j],  j over the keys that row i sees; lse = log sum_j exp(...)
+//
+// Bound: the cache's bytes (144 per token and kv head at D = 128), which every other term hides behind as long as a token
+// costs few instructions.  So codes are never turned into numbers: both products run on mma.m16n8k16 with the codes as the A
+// operand in the form in which they lie in memory (f16 subnormals, one AND per pair; one shift per word), 16 tokens x 8 query
+// rows at a time, and scales and minima enter outside:
+//   q . k[t]  = sum_g s[t, g] * (q_g . c[t, g]) + m[t, g] * sum(q_g)           (S^T = C Q^T per group of 64 channels)
+//   sum_t p[t] v[t] = sum_t (p[t] s[t, g]) c[t, g] + sum_t p[t] m[t, g]         (O^T = C^T W, W = p * s in f16)
+// The query rows are brought to f16 by a power of two of their own (bf16 has 8 bits of precision, f16 11: exact unless 2^-38
+// of the row's largest), products and sums are f32.  W is rounded to f16 once, 2^-11 relative, after a power of two that keeps
+// it in range whatever the scales (vscale below).  The softmax is the one-pass form with a running reference: a warp rescales
+// only when a score exceeds the reference by more than 2^SLACK, so the common step has one vote instead of a reduction.
+//
+// Work: a CTA of 4 warps takes one (sequence, kv head, block of 8 or 16 query rows, slice of the keys); each warp streams its
+// own 32-token steps through a ring of three shared-memory stages filled by bulk copies (one lane per 16-token tile looks the
+// page up and issues the copy), so the main loop has no CTA-wide synchronisation.  Warps are joined in shared memory, slices
+// through the workspace by a second kernel (in slice order: the result does not depend on timing).
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/baracuda_kernels_q.h"
+#include "kv4_format.cuh"
+#include "ptx_sm100a.cuh"
+
+namespace bq {
+
+namespace {
+
+__device__ int g_kv4_attention_device_status = 0;
+
+constexpr int AT_WARPS = 4;
+constexpr int AT_STAGES = 3;
+constexpr int AT_STEP = 32;  // tokens of a warp's step
+constexpr float SLACK = 4.0f;
+constexpr float NO_REF = -1.0e30f;
+constexpr long long AT_WAIT_LIMIT = 2000000000LL;  // cycles: about a second
+
+struct AttnParams {
+    const __nv_bfloat16* q;
+    int64_t ldq;
+    const int32_t* cu_q;
+    Kv4Cache cache;
+    const int32_t* table;
+    int64_t ld_table;
+    const int32_t* kv_lens;
+    __nv_bfloat16* out;
+    int64_t ldo;
+    float* lse;
+    float scale_log2;  // scale * log2(e)
+    int32_t causal, window;
+    int32_t batch, total_q, max_q, max_kv, heads_q, group;
+    int32_t row_tiles, splits;
+    float* part_o;   // [tile][split][rows][D]
+    float2* part_ml; // [tile][split][rows]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A sequence as this launch sees it: query rows [row0, row0 + n), len keys.  Lengths beyond what the caller announced are cut
+// (and reported), so that no read or write leaves the buffers.
+struct Sequence {
+    int row0, n, len;
+};
+__device__ __forceinline__ Sequence sequence_of(const AttnParams& p, int b) {
+    Sequence s;
+    int end = p.cu_q[b + 1];
+    s.row0 = p.cu_q[b];
+    s.len = p.kv_lens[b];
+    if (s.row0 < 0 || end > p.total_q || end - s.row0 > p.max_q || s.len > p.max_kv) atomicCAS(&g_kv4_attention_device_status, 0, 403);
+    s.row0 = max(s.row0, 0);
+    end = min(end, p.total_q);
+    s.n = max(0, min(end - s.row0, p.max_q));
+    s.len = max(0, min(s.len, p.max_kv));
+    return s;
+}
+
+template <int D, int NT>
+struct AttnSmem {
+    static constexpr int STAGE = (AT_STEP / KV4_TILE) * kv4_tile_bytes(D);
+    static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
+    static constexpr int JOIN = AT_WARPS * 8 * NT * (D + 2) * 4;
+    static constexpr int BODY = RING > JOIN ? RING : JOIN;
+    static constexpr int BARS = BODY;
+    static constexpr int VALID = BARS + AT_WARPS * AT_STAGES * 8;
+    static constexpr int TOTAL = VALID + AT_WARPS * AT_STAGES * 4;
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __grid_constant__ AttnParams p) {
+    using L = AttnSmem<D, NT>;
+    constexpr int G = D / KV4_GROUP;
+    constexpr int W = D >= 128 ? 2 : 1;       // groups of a 16-byte chunk of keys
+    constexpr int TILE = kv4_tile_bytes(D);
+    constexpr int ROWS = 8 * NT;
+    constexpr int MT = D / 16;                // 16-channel blocks of the output
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+
+    int id = blockIdx.x;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int tile_id = id;
+    const int rt = id % p.row_tiles;
+    id /= p.row_tiles;
+    const int hk = id % p.cache.heads_kv, b = id / p.cache.heads_kv;
+    const Sequence sq = sequence_of(p, b);
+    const int rows = min(ROWS, sq.n * p.group - rt * ROWS);  // row = query index * group + head in group
+    if (rows <= 0) return;
+
+    // keys that any row of this block sees, and this CTA's slice of them, in steps
+    const int i_first = rt * ROWS / p.group, i_last = (rt * ROWS + rows - 1) / p.group;
+    const int past = sq.len - sq.n;  // the last key that query row i sees is past + i when causal
+    int hi_all = p.causal ? min(sq.len, past + i_last + 1) : sq.len;
+    int lo_all = p.window > 0 ? max(0, past + i_first - p.window + 1) : 0;
+    hi_all = max(hi_all, 0);
+    const int step0 = lo_all / AT_STEP, steps = max(0, (hi_all + AT_STEP - 1) / AT_STEP - step0);
+    const int per = (steps + p.splits - 1) / p.splits;
+    const int my_begin = min(split * per, steps), my_end = min(my_begin + per, steps);
+
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS) + warp * AT_STAGES;
+    volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::VALID) + warp * AT_STAGES;
+    uint8_t* ring = smem + warp * AT_STAGES * L::STAGE;
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < AT_STAGES; ++s) mbar_init(&bars[s], 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+
+    // the lanes that fetch: lane t takes tile t of a step
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
+    const int tiles_per_page = p.cache.page_size / KV4_TILE;
+    const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
+    auto tile_of = [&](int step) { return (step0 + step) * (AT_STEP / KV4_TILE) + lane; };
+    auto page_of = [&](int step) {  // -1 where there is nothing to fetch
+        const int t = tile_of(step);
+        if (lane >= AT_STEP / KV4_TILE || step >= my_end || t * KV4_TILE >= hi_all) return -1;
+        const int page = table[t / tiles_per_page];
+        if (page < 0 || page >= p.cache.num_pages) {
+            atomicCAS(&g_kv4_attention_device_status, 0, 404);
+            return -1;
+        }
+        return page;
+    };
+    auto fetch = [&](int step, int page, int stage) {
+        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) {
+            valid[stage] = have;
+            mbar_arrive_expect_tx(&bars[stage], __popc(have) * TILE);
+        }
+        __syncwarp();
+        if (page >= 0) {
+            bulk_load_1d(ring + stage * L::STAGE + lane * TILE,
+                         head_base + static_cast<int64_t>(page) * p.cache.page_stride + (tile_of(step) % tiles_per_page) * TILE, TILE,
+                         &bars[stage]);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < AT_STAGES; ++s) {
+        const int step = my_begin + warp + s * AT_WARPS;
+        if (step < my_end) fetch(step, page_of(step), s);
+    }
+
+    // the query rows as B fragments: lane (r, c) holds, of row r of each 8-row block, channels 64 g + 16 c .. + 15
+    uint32_t qf[NT][G][8];
+    float qscale[NT][2], qsum[NT][2][G];  // of this lane's score columns 2 c, 2 c + 1
+    int row_hi[NT][2], row_lo[NT][2];     // keys [lo, hi) that those rows see
+    int hi_min = 0x7fffffff, lo_max = 0;  // over the rows that exist: steps inside need no mask
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = rt * ROWS + nt * 8 + r;
+        const bool there = nt * 8 + r < rows;
+        float x[G][16];
+        float top = 0.0f, sums[G];
+        const __nv_bfloat16* src = p.q + static_cast<int64_t>(sq.row0 + (there ? row / p.group : 0)) * p.ldq +
+                                   static_cast<int64_t>(hk * p.group + (there ? row % p.group : 0)) * D + 16 * c;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+            if (there) {
+                raw[0] = *reinterpret_cast<const uint4*>(src + 64 * g);
+                raw[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 8);
+            }
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(raw);
+            sums[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[g][2 * e] = __low2float(h[e]);
+                x[g][2 * e + 1] = __high2float(h[e]);
+                top = fmaxf(top, fmaxf(fabsf(x[g][2 * e]), fabsf(x[g][2 * e + 1])));
+                sums[g] += x[g][2 * e] + x[g][2 * e + 1];
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;  // 2^-ex brings the largest into [2^14, 2^15)
+        ex = max(-100, min(100, ex));
+        if (top == 0.0f || top > 3.0e38f) ex = 0;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // nibbles n and n + 4 of a word are a pair; odd nibbles come as 16 times the code
+                const float* w = &x[g][8 * u];
+                const float odd = down * 0.0625f;
+                qf[nt][g][4 * u] = pack_half2(w[0] * down, w[4] * down);
+                qf[nt][g][4 * u + 1] = pack_half2(w[1] * odd, w[5] * odd);
+                qf[nt][g][4 * u + 2] = pack_half2(w[2] * down, w[6] * down);
+                qf[nt][g][4 * u + 3] = pack_half2(w[3] * odd, w[7] * odd);
+            }
+        }
+        const int i = row / p.group;
+        const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
+        const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
+        if (there) hi_min = min(hi_min, hi), lo_max = max(lo_max, lo);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int from = (2 * c + e) * 4;  // a lane that holds row 2 c + e
+            qscale[nt][e] = __shfl_sync(0xffffffffu, up, from) * (16777216.0f * p.scale_log2);
+#pragma unroll
+            for (int g = 0; g < G; ++g) qsum[nt][e][g] = __shfl_sync(0xffffffffu, sums[g], from) * p.scale_log2;
+            row_hi[nt][e] = __shfl_sync(0xffffffffu, hi, from);
+            row_lo[nt][e] = __shfl_sync(0xffffffffu, lo, from);
+        }
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        hi_min = min(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, o));
+        lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
+    }
+
+    float acc[NT][MT][4];
+    float l[NT][2], z[NT][2][G], ref[NT][2];
+    float vscale = 1.0f, vbound = 0.0f;  // W = p * s * vscale; s up to vbound keeps it within f16
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[nt][e] = 0.0f;
+            ref[nt][e] = NO_REF;
+#pragma unroll
+            for (int g = 0; g < G; ++g) z[nt][e][g] = 0.0f;
+        }
+    }
+
+    uint32_t parity = 0;
+    int stage = 0;
+    bool gave_up = false;
+    int step = my_begin + warp;
+    for (; step < my_end; step += AT_WARPS) {
+        const int ahead = step + AT_STAGES * AT_WARPS;
+        const int next_page = page_of(ahead);  // asked for now, used after this step
+        if (!mbar_try_wait(&bars[stage], parity)) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&bars[stage], parity)) {
+                if (clock64() - t0 > AT_WAIT_LIMIT) {
+                    gave_up = true;
+                    break;
+                }
+            }
+            gave_up = __any_sync(0xffffffffu, gave_up);
+            if (gave_up) break;
+        }
+        __syncwarp();
+        const uint32_t have = valid[stage];
+        const uint8_t* base = ring + stage * L::STAGE;
+        const int token0 = (step0 + step) * AT_STEP;
+        constexpr int TILES = AT_STEP / KV4_TILE;
+        const bool edge = token0 + AT_STEP > hi_min || token0 < lo_max || have != (1u << TILES) - 1u;
+
+        // scores of both tiles, in units of log2
+        float sc[TILES][NT][4];
+        float sv[TILES][2][G], mv[TILES][2][G];  // the values' scales and minima of tokens r and r + 8
+        float top[NT][2], stop = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const uint8_t* tile = base + t * TILE;
+            float s[G][NT][4];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[g][nt][e] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < G / W; ++h) {
+                uint32_t wa[2 * W], wb[2 * W];
+                if constexpr (W == 2) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(tile + h * 1024 + lane * 16);
+                    const uint4 bb = *reinterpret_cast<const uint4*>(tile + h * 1024 + 512 + lane * 16);
+                    wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w;
+                    wb[0] = bb.x, wb[1] = bb.y, wb[2] = bb.z, wb[3] = bb.w;
+                } else {
+                    const uint2 a = *reinterpret_cast<const uint2*>(tile + lane * 8);
+                    const uint2 bb = *reinterpret_cast<const uint2*>(tile + 256 + lane * 8);
+                    wa[0] = a.x, wa[1] = a.y;
+                    wb[0] = bb.x, wb[1] = bb.y;
+                }
+#pragma unroll
+                for (int x = 0; x < 2 * W; ++x) {
+                    const int g = h * W + x / 2, u = x % 2;
+                    const uint32_t a8 = wa[x] >> 8, b8 = wb[x] >> 8;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_f16(s[g][nt], wa[x] & 0x000f000fu, wb[x] & 0x000f000fu, wa[x] & 0x00f000f0u, wb[x] & 0x00f000f0u,
+                                qf[nt][g][4 * u], qf[nt][g][4 * u + 1]);
+                        mma_f16(s[g][nt], a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
+                                qf[nt][g][4 * u + 2], qf[nt][g][4 * u + 3]);
+                    }
+                }
+            }
+            float sk[2][G], mk[2][G];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const __half2* kp = reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, 0)) + (r + 8 * e) * G;
+                const __half2* vp = reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, 1)) + (r + 8 * e) * G;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float2 a = __half22float2(kp[g]), bb = __half22float2(vp[g]);
+                    sk[e][g] = a.x, mk[e][g] = a.y;
+                    sv[t][e][g] = bb.x, mv[t][e][g] = bb.y;
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float dot = 0.0f, low = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        dot = fmaf(sk[e >> 1][g], s[g][nt][e], dot);
+                        low = fmaf(mk[e >> 1][g], qsum[nt][e & 1][g], low);
+                    }
+                    sc[t][nt][e] = fmaf(dot, qscale[nt][e & 1], low);
+                }
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int j = token0 + t * KV4_TILE + r + 8 * e;
+                    const bool dead = j >= sq.len || ((have >> t) & 1u) == 0u;  // nothing there, whatever the bytes say
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+                        if (dead) sv[t][e][g] = 0.0f, mv[t][e][g] = 0.0f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (dead || j >= row_hi[nt][x] || j < row_lo[nt][x]) sc[t][nt][2 * e + x] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                top[nt][0] = fmaxf(top[nt][0], fmaxf(sc[t][nt][0], sc[t][nt][2]));
+                top[nt][1] = fmaxf(top[nt][1], fmaxf(sc[t][nt][1], sc[t][nt][3]));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int g = 0; g < G; ++g) stop = fmaxf(stop, sv[t][e][g]);
+        }
+        bool grow = stop > vbound;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) grow = grow || top[nt][0] > ref[nt][0] + SLACK || top[nt][1] > ref[nt][1] + SLACK;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                stop = fmaxf(stop, __shfl_xor_sync(0xffffffffu, stop, o));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
+            }
+            float vmul = 1.0f;
+            if (stop > vbound) {  // W <= 2^SLACK * s * vscale: the largest scale seen goes to [2^10, 2^11)
+                const int ex = 10 - (static_cast<int>(__float_as_uint(stop) >> 23) - 127);
+                const float to = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+                vmul = vbound > 0.0f ? to / vscale : 1.0f;
+                vscale = to;
+                vbound = 2048.0f / to;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float fix[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float m = fmaxf(ref[nt][e], top[nt][e]);
+                    fix[e] = ex2(ref[nt][e] - m);
+                    ref[nt][e] = m;
+                    l[nt][e] *= fix[e];
+#pragma unroll
+                    for (int g = 0; g < G; ++g) z[nt][e][g] *= fix[e];
+                    fix[e] *= vmul;
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    acc[nt][j][0] *= fix[0], acc[nt][j][2] *= fix[0];
+                    acc[nt][j][1] *= fix[1], acc[nt][j][3] *= fix[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const uint8_t* tile = base + t * TILE + 8 * D;
+            uint32_t wf[NT][G][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float pr[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pr[e] = ex2(sc[t][nt][e] - ref[nt][e & 1]);
+                    l[nt][e & 1] += pr[e];
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float sw = sv[t][e >> 1][g], mw = mv[t][e >> 1][g];
+                        if (edge && sc[t][nt][e] == -INFINITY) sw = 0.0f, mw = 0.0f;  // a key this row does not see may hold anything
+                        w[e] = pr[e] * (sw * vscale);
+                        z[nt][e & 1][g] = fmaf(pr[e], mw, z[nt][e & 1][g]);
+                    }
+                    wf[nt][g][0] = movmatrix_trans(pack_half2(w[0], w[1]));
+                    wf[nt][g][1] = movmatrix_trans(pack_half2(w[2], w[3]));
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
+                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w0 = words[j], w8 = words[j] >> 8;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_f16(acc[nt][4 * g + j], w0 & 0x000f000fu, w0 & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u,
+                                wf[nt][g][0], wf[nt][g][1]);
+                }
+            }
+        }
+        __syncwarp();
+        if (ahead < my_end) fetch(ahead, next_page, stage);
+        if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
+    }
+    if (gave_up) {
+        if (lane == 0) atomicCAS(&g_kv4_attention_device_status, 0, 411);
+        // copies of this warp may still be in flight into its ring: wait for them, again within a limit
+        const long long t0 = clock64();
+        for (int s = 0; s < AT_STAGES; ++s) {
+            if (step + s * AT_WARPS >= my_end) break;
+            while (!mbar_try_wait(&bars[stage], parity) && clock64() - t0 < AT_WAIT_LIMIT) {
+            }
+            if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
+        }
+    }
+
+    // join the lanes, then the warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
+#pragma unroll
+                for (int g = 0; g < G; ++g) z[nt][e][g] += __shfl_xor_sync(0xffffffffu, z[nt][e][g], o);
+            }
+        }
+    __syncthreads();  // every warp has left its ring
+    float* join = reinterpret_cast<float*>(smem);  // [warp][row][D], then [warp][row] (ref, l)
+    float2* join_ml = reinterpret_cast<float2*>(join + AT_WARPS * ROWS * D);
+    const float unit = 16777216.0f / vscale;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float* row = join + (warp * ROWS + nt * 8 + 2 * c + e) * D;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                row[16 * j + r] = fmaf(acc[nt][j][e], unit, z[nt][e][j / 4]);
+                row[16 * j + 8 + r] = fmaf(acc[nt][j][2 + e], unit * 0.0625f, z[nt][e][j / 4]);
+            }
+            if (r == 0) join_ml[warp * ROWS + nt * 8 + 2 * c + e] = make_float2(ref[nt][e], l[nt][e]);
+        }
+    __syncthreads();
+    for (int at = threadIdx.x; at < rows * (D / 4); at += AT_WARPS * 32) {
+        const int row = at / (D / 4), d = at % (D / 4) * 4;
+        float m = NO_REF;
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) m = fmaxf(m, join_ml[w * ROWS + row].x);
+        float sum = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) {
+            const float2 ml = join_ml[w * ROWS + row];
+            const float f = ex2(ml.x - m);
+            const float4 x = *reinterpret_cast<const float4*>(join + (w * ROWS + row) * D + d);
+            sum = fmaf(ml.y, f, sum);
+            o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+        }
+        if (p.splits == 1) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int gr = rt * ROWS + row;
+            const int64_t q_row = sq.row0 + gr / p.group;
+            const int head = hk * p.group + gr % p.group;
+            const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * inv, o.y * inv), bb = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+            *reinterpret_cast<uint2*>(p.out + q_row * p.ldo + static_cast<int64_t>(head) * D + d) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&bb));
+            if (p.lse != nullptr && d == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+        } else {
+            const int64_t slot = (static_cast<int64_t>(tile_id) * p.splits + split) * ROWS + row;
+            *reinterpret_cast<float4*>(p.part_o + slot * D + d) = o;
+            if (d == 0) p.part_ml[slot] = make_float2(m, sum);
+        }
+    }
+}
+
+// Adds the slices of one block of rows, in slice order.  One warp per row.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int ROWS = 8 * NT;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int row = static_cast<int>(id % ROWS);
+    const int64_t tile_id = id / ROWS;
+    int rest = static_cast<int>(tile_id / p.row_tiles);
+    const int rt = static_cast<int>(tile_id % p.row_tiles);
+    const int hk = rest % p.cache.heads_kv, b = rest / p.cache.heads_kv;
+    if (b >= p.batch) return;
+    const Sequence sq = sequence_of(p, b);
+    const int gr = rt * ROWS + row;
+    if (gr >= sq.n * p.group) return;
+    const int64_t slot0 = tile_id * p.splits * ROWS + row;
+    float m = NO_REF;
+    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[slot0 + static_cast<int64_t>(s) * ROWS].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    constexpr int PER = D / 32;
+    float sum = 0.0f, acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t slot = slot0 + static_cast<int64_t>(s) * ROWS;
+        const float2 ml = p.part_ml[slot];
+        const float f = ex2(ml.x - m);
+        sum = fmaf(ml.y, f, sum);
+        const float* o = p.part_o + slot * D + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(o + e);
+            acc[e] = fmaf(x.x, f, acc[e]);
+            acc[e + 1] = fmaf(x.y, f, acc[e + 1]);
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t q_row = sq.row0 + gr / p.group;
+    const int head = hk * p.group + gr % p.group;
+    __nv_bfloat16* out = p.out + q_row * p.ldo + static_cast<int64_t>(head) * D + lane * PER;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) *reinterpret_cast<__nv_bfloat162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+    if (p.lse != nullptr && lane == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+struct Shape {
+    int nt, row_tiles, splits;
+    int64_t tiles;
+};
+
+constexpr int ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
+
+Shape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
+    Shape s;
+    const int64_t rows = max_q * (heads_q / heads_kv);
+    s.nt = rows > 8 && head_dim <= 128 ? 2 : 1;
+    s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
+    s.tiles = batch * heads_kv * s.row_tiles;
+    const int64_t steps = (max_kv + AT_STEP * AT_WARPS - 1) / (AT_STEP * AT_WARPS);  // of a CTA
+    const int64_t want = (ASSUMED_SMS * 8 + s.tiles - 1) / (s.tiles > 0 ? s.tiles : 1);
+    const int64_t most = (steps + 1) / 2;
+    s.splits = static_cast<int>(want < most ? want : most);
+    if (s.splits < 1) s.splits = 1;
+    return s;
+}
+
+template <int D, int NT>
+int32_t launch_d(AttnParams& p, const Shape& s, cudaStream_t stream) {
+    auto kern = kv4_attention_kernel<D, NT>;
+    using L = AttnSmem<D, NT>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return BQ_STATUS_LAUNCH_FAILURE;
+    }
+    kern<<<static_cast<unsigned>(s.tiles * s.splits), AT_WARPS * 32, L::TOTAL, stream>>>(p);
+    if (cudaPeekAtLastError() != cudaSuccess) return BQ_STATUS_LAUNCH_FAILURE;
+    if (s.splits > 1) {
+        kv4_attention_join_kernel<D, NT><<<static_cast<unsigned>((s.tiles * 8 * NT + 3) / 4), 128, 0, stream>>>(p);
+        if (cudaPeekAtLastError() != cudaSuccess) return BQ_STATUS_LAUNCH_FAILURE;
+    }
+    return BQ_STATUS_OK;
+}
+
+}  // namespace
+
+bool kv4_attention_fits(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim) {
+    if (batch == 0 || max_q == 0) return true;
+    const Shape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
+    return s.tiles * 16 <= 0x7fffffff && s.tiles * s.splits <= 0x7fffffff;
+}
+
+size_t kv4_attention_workspace_bytes(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv,
+                                     int32_t head_dim) {
+    const Shape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
+    if (s.splits <= 1) return 0;
+    return static_cast<size_t>(s.tiles) * s.splits * 8 * s.nt * (head_dim + 2) * 4;
+}
+
+int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
+    const Shape s = shape_of(g.batch, g.max_q, g.max_kv, g.heads_q, g.cache.heads_kv, g.cache.head_dim);
+    AttnParams p;
+    p.q = static_cast<const __nv_bfloat16*>(g.q);
+    p.ldq = g.ldq;
+    p.cu_q = g.cu_q;
+    p.cache = g.cache;
+    p.table = g.page_table;
+    p.ld_table = g.ld_table;
+    p.kv_lens = g.kv_lens;
+    p.out = static_cast<__nv_bfloat16*>(g.out);
+    p.ldo = g.ldo;
+    p.lse = g.lse;
+    p.scale_log2 = static_cast<float>(static_cast<double>(g.scale) * 1.4426950408889634);
+    p.causal = g.causal;
+    p.window = g.window;
+    p.batch = g.batch;
+    p.total_q = g.total_q;
+    p.max_q = g.max_q;
+    p.max_kv = g.max_kv;
+    p.heads_q = g.heads_q;
+    p.group = g.heads_q / g.cache.heads_kv;
+    p.row_tiles = s.row_tiles;
+    p.splits = s.splits;
+    p.part_o = static_cast<float*>(g.workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + s.tiles * s.splits * 8 * s.nt * g.cache.head_dim);
+    switch (g.cache.head_dim) {
+        case 64: return s.nt == 2 ? launch_d<64, 2>(p, s, stream) : launch_d<64, 1>(p, s, stream);
+        case 128: return s.nt == 2 ? launch_d<128, 2>(p, s, stream) : launch_d<128, 1>(p, s, stream);
+        case 256: return launch_d<256, 1>(p, s, stream);
+        default: return BQ_STATUS_UNSUPPORTED;
+    }
+}
+
+int32_t read_and_clear_kv4_attention_device_status() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kv4_attention_device_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) {
+        int zero = 0;
+        (void)cudaMemcpyToSymbol(g_kv4_attention_device_status, &zero, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace bq

@@ -523,6 +523,120 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * The attention step between the qkv and the output projection, over a paged cache in 4 bits (no counterpart behind the
+ * reference's quantized path; its cache and attention families hold keys and values in the activation type).
+ *
+ * THE CACHE.  `cache` is a 16-byte aligned buffer of `num_pages` pages, `page_stride` bytes apart (a multiple of 16, at least
+ * baracuda_kernels_kv4_page_bytes; larger where pages of several layers are interleaved).  A page holds `page_size` tokens (a
+ * multiple of 16) of every kv head, as [heads_kv][page_size / 16] tiles of 18 * head_dim bytes; head_dim is 64, 128 or 256.
+ * Each group of 64 channels of a token and head is 64 codes c in 0..15, an f16 scale s and an f16 minimum m; the value is
+ * s * c + m.  s = f16((max - min) / 15), m = f16(min), both cut to +-65504, c = clamp(rint_even((x - m) / s), 0, 15) (0 where
+ * s is 0); a minimum of zero is +0.  A NaN among the 64 makes all of them NaN; infinities are cut.  Within a tile, t = token (0..15), d = channel:
+ *   keys    8 * D bytes: with d = 64 g + 16 c + 8 u + 2 b + n, W = min(2, D / 64), h = g / W: nibble n (0 = low) of byte
+ *           (((h * 16 + t) * 4 + c) * W + g % W) * 8 + 4 u + b
+ *   values  8 * D bytes: with d = 64 h + 16 j + 8 n + r, t = 8 e + 2 c + o: nibble n of byte
+ *           h * 512 + (r * 4 + c) * 16 + 4 j + 2 o + e
+ *   (s, m)  of the keys [16][D / 64], then of the values [16][D / 64]
+ * A token's place is its slot, page * page_size + offset (int64).  Bytes of places that hold no token are never used, whatever
+ * they are.
+ *
+ * NORM AND ROTATION.  q is bf16 [tokens][heads_q * head_dim], k (and v) bf16 [tokens][heads_kv * head_dim], each with its own
+ * row pitch (elements), so all three may be columns of one qkv projection.  Per head:
+ *   y = (x * (1 / sqrt(mean(x^2) + eps))) * weight      (f32; the mean square summed in 64 bits; skipped where weight is NULL)
+ *   pair (a, b) -> (a * cos - b * sin, b * cos + a * sin)   over the first rot_dim channels (a multiple of 8, 0 = none): pair i
+ *       is channels (i, i + rot_dim / 2), or (2 i, 2 i + 1) with interleaved != 0
+ *   out = bf16(y)
+ * Weights are float[head_dim].  cos_sin is float [max_pos][rot_dim], the cosines of the rot_dim / 2 pairs and then their
+ * sines, 16-byte aligned.  positions is int32 [axes][pos_stride], axes 1..8; axis_of_pair is a HOST array of rot_dim / 2 axis
+ * numbers, copied by value into the launch (NULL: axis 0 for all), which serves sectioned as well as interleaved
+ * time / height / width layouts.  A position outside [0, max_pos) is cut to it and reported as device status 401.
+ * q_out and k_out may be q and k themselves.  q, k, v, q_out and k_out are 8-byte aligned with pitches of a multiple of 4
+ * elements (1).
+ *   *_qk_norm_rope_bf16_*             writes q_out and k_out.
+ *   *_qk_norm_rope_kv4_append_bf16_*  writes q_out, and the keys (normed, turned, rounded to bf16) and values to the cache.
+ *   *_kv4_append_bf16_*               writes keys and values to the cache as they are.
+ * The one-launch form leaves the bits of the two-launch sequence.  A negative slot leaves its token out of the cache (padding
+ * of a captured batch), a slot beyond the cache too, reported as device status 402.  The slots of one call are distinct; two
+ * tokens at one slot leave that slot unspecified.  Nothing else of the cache is written.
+ *
+ * READ.  *_kv4_read_bf16_* writes the bf16 values of the tokens at `slots` to k and v [tokens][heads_kv * head_dim] (16-byte
+ * aligned, pitches of a multiple of 8).  Rows of a negative slot are left as they are; beyond the cache: the same, and 402.
+ *
+ * ATTENTION.  q and out are bf16 [total_q][heads_q * head_dim] (16-byte aligned, pitches of a multiple of 8), heads_q a multiple
+ * of heads_kv, head h reading kv head h / (heads_q / heads_kv).  Sequence b has the query rows cu_q[b] .. cu_q[b + 1] (int32
+ * [batch + 1], any number from 0 to max_q) and kv_lens[b] tokens (int32, 0 to max_kv) in the cache, its own rows' included,
+ * on the pages page_table[b][0 ..] (int32, row pitch ld_table >= ceil(max_kv / page_size)).  Row i of n sees key j when
+ *   j < kv_lens[b], with causal != 0 also j <= kv_lens[b] - n + i, with window > 0 also j > kv_lens[b] - n + i - window.
+ * out = sum_j softmax_j(scale * q . k[j]) v[j], rounded once; a row that sees no key gets zeros.  lse, float
+ * [total_q][heads_q] or NULL, gets log sum_j exp(scale * q . k[j]), minus infinity for such a row.  Rows outside every sequence
+ * are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
+ * by them, and the workspace (16-byte aligned) needs no initialisation; two launches that may overlap need one each.
+ * Lengths beyond max_q, max_kv or total_q are cut and reported as device status 403; a page number outside [0, num_pages)
+ * where a key is seen leaves its keys out and is reported as 404.
+ * The same call gives the same bits every time.
+ * ------------------------------------------------------------------------- */
+size_t baracuda_kernels_kv4_page_bytes(int32_t page_size, int32_t heads_kv, int32_t head_dim); /* 0 where not served */
+
+int32_t baracuda_kernels_qk_norm_rope_bf16_sm100a_run(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+    const void* q, int64_t ldq, const void* k, int64_t ldk,
+    const void* q_weight, const void* k_weight, float eps,
+    const void* cos_sin, int32_t rot_dim, int32_t max_pos, int32_t interleaved,
+    const void* positions, int64_t pos_stride, int32_t axes, const uint8_t* axis_of_pair,
+    void* q_out, int64_t ldqo, void* k_out, int64_t ldko,
+    void* workspace, size_t workspace_bytes, void* stream);
+int32_t baracuda_kernels_qk_norm_rope_bf16_sm100a_can_implement(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t rot_dim, int32_t axes);
+size_t baracuda_kernels_qk_norm_rope_bf16_sm100a_workspace_size(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
+
+int32_t baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_run(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+    const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+    const void* q_weight, const void* k_weight, float eps,
+    const void* cos_sin, int32_t rot_dim, int32_t max_pos, int32_t interleaved,
+    const void* positions, int64_t pos_stride, int32_t axes, const uint8_t* axis_of_pair,
+    void* q_out, int64_t ldqo,
+    void* cache, int64_t page_stride, int32_t num_pages, int32_t page_size, const void* slots,
+    void* workspace, size_t workspace_bytes, void* stream);
+int32_t baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_can_implement(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t rot_dim, int32_t axes, int32_t page_size);
+size_t baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_workspace_size(
+    int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
+
+int32_t baracuda_kernels_kv4_append_bf16_sm100a_run(
+    int32_t tokens, int32_t heads_kv, int32_t head_dim,
+    const void* k, int64_t ldk, const void* v, int64_t ldv,
+    void* cache, int64_t page_stride, int32_t num_pages, int32_t page_size, const void* slots,
+    void* workspace, size_t workspace_bytes, void* stream);
+int32_t baracuda_kernels_kv4_append_bf16_sm100a_can_implement(
+    int32_t tokens, int32_t heads_kv, int32_t head_dim, int32_t page_size);
+size_t baracuda_kernels_kv4_append_bf16_sm100a_workspace_size(int32_t tokens, int32_t heads_kv, int32_t head_dim);
+
+int32_t baracuda_kernels_kv4_read_bf16_sm100a_run(
+    int32_t tokens, int32_t heads_kv, int32_t head_dim,
+    const void* cache, int64_t page_stride, int32_t num_pages, int32_t page_size, const void* slots,
+    void* k, int64_t ldk, void* v, int64_t ldv,
+    void* workspace, size_t workspace_bytes, void* stream);
+int32_t baracuda_kernels_kv4_read_bf16_sm100a_can_implement(
+    int32_t tokens, int32_t heads_kv, int32_t head_dim, int32_t page_size);
+size_t baracuda_kernels_kv4_read_bf16_sm100a_workspace_size(int32_t tokens, int32_t heads_kv, int32_t head_dim);
+
+int32_t baracuda_kernels_attention_kv4_bf16_sm100a_run(
+    int32_t batch, int32_t total_q, int32_t max_q, int32_t max_kv,
+    int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+    const void* q, int64_t ldq, const void* cu_q,
+    const void* cache, int64_t page_stride, int32_t num_pages, int32_t page_size,
+    const void* page_table, int64_t ld_table, const void* kv_lens,
+    float scale, int32_t causal, int32_t window,
+    void* out, int64_t ldo, void* lse,
+    void* workspace, size_t workspace_bytes, void* stream);
+int32_t baracuda_kernels_attention_kv4_bf16_sm100a_can_implement(
+    int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t page_size);
+size_t baracuda_kernels_attention_kv4_bf16_sm100a_workspace_size(
+    int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
+
+/* ---------------------------------------------------------------------------
  * Column-parallel (N-sharded) GEMM inside one NVLink box.  Rank r owns rows
  * [r*n_local, (r+1)*n_local) of the [N,K] weight and the matching scale_b slice;
  * activations and scale_a are replicated; every rank computes D[:, slice].
@@ -697,7 +811,9 @@ int32_t baracuda_q_nccl_all_gather_bytes(void* comm, int32_t world, const void* 
  * Diagnostics and test hooks (no counterpart in the reference).
  * device_status: synchronous read-and-clear of the word a kernel sets when one
  * of its bounded barrier waits ran out (0 = none; the code names the kernel and
- * the waiting role: 101..104 1-CTA GEMM, 111..115 CTA-pair GEMM, 121..123 cluster split-K GEMM, 201..207 streaming GEMVs, 299 the self-test, 301 the peer barrier).  Call it after synchronising the stream.
+ * the waiting role: 101..104 1-CTA GEMM, 111..115 CTA-pair GEMM, 121..123 cluster split-K GEMM, 201..207 streaming GEMVs, 299 the self-test, 301 the peer barrier, 401 / 402 a position / a slot out of
+ * range in the norm, rotation, append and read kernels, 403 / 404 a length / a page number out of range in the attention over
+ * the 4-bit cache, 411 its bounded waits).  Call it after synchronising the stream.
  * set_tuning: forces a kernel choice for the CALLING THREAD only (thread-local; other threads' launches are not
  * affected, nothing process-wide is kept), so tests can run every kernel on the same shapes:
  *   key 0  GEMM tile: 0 automatic; 64, 128, 256 = 1-CTA kernel with that N-tile; 512 = the CTA-pair kernel;
