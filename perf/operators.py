@@ -384,7 +384,7 @@ def _plan(state, op):
     args = bq.QkNormRopeArgs(q=q, k=k, q_out=state["q_out"], cos_sin=state["cos_sin"], positions=state["positions"],
                              q_weight=state["q_weight"], k_weight=state["k_weight"], k_out=state.get("k_out"),
                              v=v if layout else None, cache=state.get("cache"), slots=state.get("slots"))
-    by_head = {n: state[n].unflatten(-1, (-1, case["dim"])) for n in ("q_out", "k_out") if n in state}
+    by_head = {n: state[n].unflatten(-1, (-1, case["dim"])) for n in ("q_out", "k_out", "k_read") if n in state}
     return plan, args, read, by_head
 
 
@@ -404,7 +404,7 @@ def _run_own(state, op):
     if op == "norm_rope":
         return {"q": by_head["q_out"], "k": by_head["k_out"]}
     read[0].run(None, None, read[1])  # what the cache then holds of these tokens
-    return {"q": by_head["q_out"], "k": state["k_read"], "v": state["v_read"]}
+    return {"q": by_head["q_out"], "k": by_head["k_read"], "v": state["v_read"]}
 
 
 # ------------------------------------------------------------------------------------------------ in 64 bits
