@@ -616,7 +616,7 @@ template <int D, int NT>
 int32_t launch_d(AttnParams& p, const Shape& s, cudaStream_t stream) {
     auto kern = kv4_attention_kernel<D, NT>;
     using L = AttnSmem<D, NT>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) {
+    if (L::TOTAL > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) {
         (void)cudaGetLastError();
         return BQ_STATUS_LAUNCH_FAILURE;
     }

@@ -29,56 +29,56 @@ from .vocab import (
 _BF16 = torch.bfloat16
 
 
-def _matrix(t: Optional[torch.Tensor], rows: int, cols: int, name: str) -> int:
-    """Row pitch of a bf16 device matrix of at least `rows` rows and exactly `cols` columns."""
+# A decode step is a few microseconds on the GPU, so a call costs the host little: every tensor is asked once for each property.
+def _device_of(t: Optional[torch.Tensor], name: str) -> int:
+    device = -1 if t is None else t.get_device()
+    if device < 0:
+        raise InvalidProblem(f"{name}: expected a device buffer")
+    return device
+
+
+def _matrix(t: Optional[torch.Tensor], rows: int, cols: int, name: str, device: int) -> tuple:
+    """(pointer, row pitch) of a bf16 matrix of at least `rows` rows and exactly `cols` columns on `device`."""
     if t is None:
         raise InvalidProblem(f"{name} is required")
-    if t.dtype is not _BF16 or not t.is_cuda:
-        raise InvalidProblem(f"{name}: expected a bfloat16 device matrix")
+    if t.dtype is not _BF16 or t.get_device() != device:
+        raise InvalidProblem(f"{name}: expected a bfloat16 device matrix, on the device of the others")
     shape = t.shape
-    if len(shape) != 2 or shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise InvalidProblem(f"{name}: expected [{rows}, {cols}] with unit column stride")
+    if len(shape) != 2 or shape[1] != cols:
+        raise InvalidProblem(f"{name}: expected [{rows}, {cols}], got {list(shape)}")
+    ld, unit = t.stride()
     if shape[0] < rows:
         raise BufferTooSmall(f"{name}: need {rows} rows, got {shape[0]}")
-    ld = t.stride(0)
-    if rows > 1 and ld < cols:
-        raise InvalidProblem(f"{name}: rows overlap")
-    return ld if ld >= cols else cols
+    if unit != 1 and cols > 1:
+        raise InvalidProblem(f"{name}: expected unit column stride")
+    if ld < cols:
+        if rows > 1:
+            raise InvalidProblem(f"{name}: rows overlap")
+        ld = cols
+    return t.data_ptr(), ld
 
 
-def _vector(t: Optional[torch.Tensor], dtype, elems: int, name: str) -> int:
-    """Pointer of a contiguous device vector of `dtype` with at least `elems` elements."""
+def _vector(t: Optional[torch.Tensor], dtype, elems: int, name: str, device: int) -> int:
+    """Pointer of a contiguous vector of `dtype` with at least `elems` elements on `device`."""
     if t is None:
         raise InvalidProblem(f"{name} is required")
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-        raise InvalidProblem(f"{name}: expected a contiguous {dtype} device buffer")
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise InvalidProblem(f"{name}: expected a contiguous {dtype} device buffer, on the device of the others")
     if t.numel() < elems:
         raise BufferTooSmall(f"{name}: need {elems} elements, buffer holds {t.numel()}")
     return t.data_ptr()
 
 
-class _Device:
-    """Makes the tensors' device the current one for a launch, and checks that they share it."""
-
-    def __init__(self, *tensors: Optional[torch.Tensor]):
-        index = None
-        for t in tensors:
-            if t is not None:
-                if index is None:
-                    index = t.get_device()
-                elif t.get_device() != index:
-                    raise InvalidProblem("tensors on different devices")
-        self.index = index
-
-    def call(self, stream, fn, *args) -> int:
-        def go() -> int:
-            s = torch.cuda.current_stream().cuda_stream if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
-            return fn(*args, s)
-
-        if torch.cuda.current_device() == self.index:
-            return go()
-        with torch.cuda.device(self.index):
-            return go()
+def _call(device: int, stream, fn, *args) -> int:
+    """fn(*args, stream) with the tensors' device as the current one; stream None is that device's current stream."""
+    if stream is None:
+        s = torch._C._cuda_getCurrentRawStream(device)
+    else:
+        s = stream if isinstance(stream, int) else stream.cuda_stream
+    if torch._C._cuda_getDevice() == device:
+        return fn(*args, s)
+    with torch.cuda.device(device):
+        return fn(*args, s)
 
 
 # --------------------------------------------------------------------------- the cache
@@ -95,20 +95,23 @@ class Kv4CacheDescriptor:
         return int(_lib.load().baracuda_kernels_kv4_page_bytes(self.page_size, self.heads_kv, self.head_dim))
 
 
-def _cache(t: Optional[torch.Tensor], d: Kv4CacheDescriptor, page_bytes: int) -> int:
-    """Page stride of the cache buffer."""
+def _cache(t: Optional[torch.Tensor], d: Kv4CacheDescriptor, page_bytes: int, device: int) -> tuple:
+    """(pointer, page stride, pages, page size) of the cache buffer."""
     if t is None:
         raise InvalidProblem("cache is required")
-    if t.dtype is not torch.uint8 or not t.is_cuda or t.dim() != 2 or t.stride(1) != 1:
-        raise InvalidProblem("cache: expected a uint8 device matrix [num_pages, page_bytes] with unit column stride")
-    if t.shape[0] < d.num_pages or t.shape[1] < page_bytes:
-        raise BufferTooSmall(f"cache: need [{d.num_pages}, {page_bytes}] bytes, got {list(t.shape)}")
-    stride = t.stride(0)
+    shape = t.shape
+    if t.dtype is not torch.uint8 or t.get_device() != device or len(shape) != 2:
+        raise InvalidProblem("cache: expected a uint8 matrix [num_pages, page_bytes] on the device of the others")
+    if shape[0] < d.num_pages or shape[1] < page_bytes:
+        raise BufferTooSmall(f"cache: need [{d.num_pages}, {page_bytes}] bytes, got {list(shape)}")
+    stride, unit = t.stride()
+    if unit != 1:
+        raise InvalidProblem("cache: expected unit column stride")
     if stride < page_bytes:
         if d.num_pages > 1:
             raise InvalidProblem("cache: pages overlap")
         stride = page_bytes
-    return stride
+    return t.data_ptr(), stride, d.num_pages, d.page_size
 
 
 def _check_cache(d: Kv4CacheDescriptor) -> int:
@@ -197,47 +200,45 @@ class QkNormRopePlan:
 
     def run(self, stream, workspace: Optional[torch.Tensor], args: QkNormRopeArgs) -> None:
         d = self.desc
-        t = d.tokens
+        t, hq, hkv, dim = d.tokens, d.heads_q, d.heads_kv, d.head_dim
         if t == 0:
             return
-        nq, nk = d.heads_q * d.head_dim, d.heads_kv * d.head_dim
-        q = q_out = None
-        ldq = ldqo = nq
-        if d.heads_q:
-            ldq, ldqo = _matrix(args.q, t, nq, "q"), _matrix(args.q_out, t, nq, "q_out")
-            q, q_out = args.q.data_ptr(), args.q_out.data_ptr()
-        ldk = _matrix(args.k, t, nk, "k")
-        wq = None if args.q_weight is None else _vector(args.q_weight, torch.float32, d.head_dim, "q_weight")
-        wk = None if args.k_weight is None else _vector(args.k_weight, torch.float32, d.head_dim, "k_weight")
-        table = positions = None
-        max_pos = 0
+        dev = _device_of(args.k, "k")
+        k, ldk = _matrix(args.k, t, hkv * dim, "k", dev)
+        q, ldq, q_out, ldqo = None, 0, None, 0
+        if hq:
+            q, ldq = _matrix(args.q, t, hq * dim, "q", dev)
+            q_out, ldqo = _matrix(args.q_out, t, hq * dim, "q_out", dev)
+        wq = wk = table = positions = None
+        if args.q_weight is not None:
+            wq = _vector(args.q_weight, torch.float32, dim, "q_weight", dev)
+        if args.k_weight is not None:
+            wk = _vector(args.k_weight, torch.float32, dim, "k_weight", dev)
+        max_pos = pos_stride = 0
         if self._rot:
-            table = _vector(args.cos_sin, torch.float32, self._rot, "cos_sin")
-            if args.cos_sin.dim() != 2 or args.cos_sin.shape[1] != self._rot:
+            table = _vector(args.cos_sin, torch.float32, self._rot, "cos_sin", dev)
+            shape = args.cos_sin.shape
+            if len(shape) != 2 or shape[1] != self._rot:
                 raise InvalidProblem(f"cos_sin: expected [max_pos, {self._rot}]")
-            max_pos = args.cos_sin.shape[0]
-            p = args.positions
-            if p is None or p.dtype is not torch.int32 or not p.is_cuda or not p.is_contiguous() or p.dim() not in (1, 2):
-                raise InvalidProblem("positions: expected a contiguous int32 device buffer [tokens] or [axes, tokens]")
-            if p.shape[-1] < t or (p.shape[0] if p.dim() == 2 else 1) < self._axes:
+            max_pos = shape[0]
+            positions = _vector(args.positions, torch.int32, 1, "positions", dev)
+            shape = args.positions.shape
+            pos_stride = shape[-1] if shape else 0
+            if len(shape) not in (1, 2):
+                raise InvalidProblem("positions: expected [tokens] or [axes, tokens]")
+            if pos_stride < t or (shape[0] if len(shape) == 2 else 1) < self._axes:
                 raise BufferTooSmall(f"positions: need [{self._axes}, {t}]")
-            positions, pos_stride = p.data_ptr(), p.shape[-1]
-        else:
-            pos_stride = t
-        turn = (wq, wk, d.eps, table, self._rot, max_pos, int(d.interleaved), positions, pos_stride, self._axes, self._axis_of_pair)
-        device = _Device(args.k, args.q, args.q_out, args.cos_sin, args.positions, args.q_weight, args.k_weight,
-                         *((args.k_out,) if d.cache is None else (args.v, args.cache, args.slots)))
-        head = (t, d.heads_q, d.heads_kv, d.head_dim, q, ldq, args.k.data_ptr(), ldk)
         if d.cache is None:
-            ldko = _matrix(args.k_out, t, nk, "k_out")
-            st = device.call(stream, self._fn, *head, *turn, q_out, ldqo, args.k_out.data_ptr(), ldko, None, 0)
+            k_out, ldko = _matrix(args.k_out, t, hkv * dim, "k_out", dev)
+            st = _call(dev, stream, self._fn, t, hq, hkv, dim, q, ldq, k, ldk, wq, wk, d.eps, table, self._rot, max_pos, d.interleaved,
+                       positions, pos_stride, self._axes, self._axis_of_pair, q_out, ldqo, k_out, ldko, None, 0)
         else:
-            ldv = _matrix(args.v, t, nk, "v")
-            stride = _cache(args.cache, d.cache, self._page_bytes)
-            slots = _vector(args.slots, torch.int64, t, "slots")
-            st = device.call(stream, self._fn, *head, args.v.data_ptr(), ldv, *turn, q_out, ldqo, args.cache.data_ptr(), stride,
-                             d.cache.num_pages, d.cache.page_size, slots, None, 0)
-        status_to_result(st, "QkNormRopePlan")
+            v, ldv = _matrix(args.v, t, hkv * dim, "v", dev)
+            st = _call(dev, stream, self._fn, t, hq, hkv, dim, q, ldq, k, ldk, v, ldv, wq, wk, d.eps, table, self._rot, max_pos,
+                       d.interleaved, positions, pos_stride, self._axes, self._axis_of_pair, q_out, ldqo,
+                       *_cache(args.cache, d.cache, self._page_bytes, dev), _vector(args.slots, torch.int64, t, "slots", dev), None, 0)
+        if st:
+            status_to_result(st, "QkNormRopePlan")
 
 
 @dataclass(frozen=True)
@@ -279,14 +280,11 @@ class Kv4AppendPlan:
         c, t = self.desc.cache, self.desc.tokens
         if t == 0:
             return
-        ldk = _matrix(args.k, t, c.heads_kv * c.head_dim, "k")
-        ldv = _matrix(args.v, t, c.heads_kv * c.head_dim, "v")
-        stride = _cache(args.cache, c, self._page_bytes)
-        slots = _vector(args.slots, torch.int64, t, "slots")
-        st = _Device(args.k, args.v, args.cache, args.slots).call(
-            stream, self._fn, t, c.heads_kv, c.head_dim, args.k.data_ptr(), ldk, args.v.data_ptr(), ldv, args.cache.data_ptr(),
-            stride, c.num_pages, c.page_size, slots, None, 0)
-        status_to_result(st, "Kv4AppendPlan")
+        dev, cols = _device_of(args.cache, "cache"), c.heads_kv * c.head_dim
+        st = _call(dev, stream, self._fn, t, c.heads_kv, c.head_dim, *_matrix(args.k, t, cols, "k", dev), *_matrix(args.v, t, cols, "v", dev),
+                   *_cache(args.cache, c, self._page_bytes, dev), _vector(args.slots, torch.int64, t, "slots", dev), None, 0)
+        if st:
+            status_to_result(st, "Kv4AppendPlan")
 
 
 @dataclass(frozen=True)
@@ -312,14 +310,12 @@ class Kv4ReadPlan(Kv4AppendPlan):
         c, t = self.desc.cache, self.desc.tokens
         if t == 0:
             return
-        ldk = _matrix(args.k, t, c.heads_kv * c.head_dim, "k")
-        ldv = _matrix(args.v, t, c.heads_kv * c.head_dim, "v")
-        stride = _cache(args.cache, c, self._page_bytes)
-        slots = _vector(args.slots, torch.int64, t, "slots")
-        st = _Device(args.k, args.v, args.cache, args.slots).call(
-            stream, self._fn, t, c.heads_kv, c.head_dim, args.cache.data_ptr(), stride, c.num_pages, c.page_size, slots,
-            args.k.data_ptr(), ldk, args.v.data_ptr(), ldv, None, 0)
-        status_to_result(st, "Kv4ReadPlan")
+        dev, cols = _device_of(args.cache, "cache"), c.heads_kv * c.head_dim
+        st = _call(dev, stream, self._fn, t, c.heads_kv, c.head_dim, *_cache(args.cache, c, self._page_bytes, dev),
+                   _vector(args.slots, torch.int64, t, "slots", dev), *_matrix(args.k, t, cols, "k", dev), *_matrix(args.v, t, cols, "v", dev),
+                   None, 0)
+        if st:
+            status_to_result(st, "Kv4ReadPlan")
 
 
 # --------------------------------------------------------------------------- attention
@@ -384,26 +380,37 @@ class Kv4AttentionPlan:
     def run(self, stream, workspace: Optional[torch.Tensor], args: Kv4AttentionArgs) -> None:
         d = self.desc
         c = d.cache
-        total = args.q.shape[0] if args.q.dim() == 2 else 0
+        total = args.q.shape[0]
         if d.batch == 0 or d.max_q == 0 or total == 0:
             return
-        cols = d.heads_q * c.head_dim
-        ldq, ldo = _matrix(args.q, total, cols, "q"), _matrix(args.out, total, cols, "out")
-        cu_q = _vector(args.cu_q, torch.int32, d.batch + 1, "cu_q")
-        kv_lens = _vector(args.kv_lens, torch.int32, d.batch, "kv_lens")
-        lse = None if args.lse is None else _vector(args.lse, torch.float32, total * d.heads_q, "lse")
+        dev, cols = _device_of(args.q, "q"), d.heads_q * c.head_dim
+        q, ldq = _matrix(args.q, total, cols, "q", dev)
+        out, ldo = _matrix(args.out, total, cols, "out", dev)
+        lse = None if args.lse is None else _vector(args.lse, torch.float32, total * d.heads_q, "lse", dev)
         table = args.page_table
-        if table is None or table.dtype is not torch.int32 or not table.is_cuda or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-            raise InvalidProblem("page_table: expected an int32 device matrix [batch, pages] with unit column stride")
-        if table.shape[0] < d.batch or table.shape[1] * c.page_size < d.max_kv:
-            raise BufferTooSmall(f"page_table: need [{d.batch}, {-(-d.max_kv // c.page_size)}], got {list(table.shape)}")
-        stride = _cache(args.cache, c, self._page_bytes)
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        if self._workspace > ws_bytes:
-            raise WorkspaceTooSmall(self._workspace, ws_bytes)
-        st = _Device(args.q, args.out, args.cu_q, args.kv_lens, table, args.cache, args.lse, workspace).call(
-            stream, self._fn, d.batch, total, d.max_q, d.max_kv, d.heads_q, c.heads_kv, c.head_dim, args.q.data_ptr(), ldq, cu_q,
-            args.cache.data_ptr(), stride, c.num_pages, c.page_size, table.data_ptr(), max(table.stride(0), table.shape[1]), kv_lens,
-            self._scale, int(d.causal), d.window, args.out.data_ptr(), ldo, lse,
-            None if workspace is None or ws_bytes == 0 else workspace.data_ptr(), ws_bytes)
-        status_to_result(st, "Kv4AttentionPlan")
+        if table is None or table.dtype is not torch.int32 or table.get_device() != dev:
+            raise InvalidProblem("page_table: expected an int32 matrix [batch, pages] on the device of the others")
+        shape = table.shape
+        if len(shape) != 2 or shape[0] < d.batch or shape[1] * c.page_size < d.max_kv:
+            raise BufferTooSmall(f"page_table: need [{d.batch}, {-(-d.max_kv // c.page_size)}], got {list(shape)}")
+        ld_table, unit = table.stride()
+        if shape[1] > 1 and unit != 1:
+            raise InvalidProblem("page_table: expected unit column stride")
+        if ld_table < shape[1]:
+            if d.batch > 1:
+                raise InvalidProblem("page_table: rows overlap")
+            ld_table = shape[1]
+        ws, ws_bytes = None, 0
+        if self._workspace:
+            if workspace is not None:
+                ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+                if workspace.get_device() != dev or not workspace.is_contiguous():
+                    raise InvalidProblem("workspace: expected a contiguous device buffer, on the device of the others")
+            if self._workspace > ws_bytes:
+                raise WorkspaceTooSmall(self._workspace, ws_bytes)
+        st = _call(dev, stream, self._fn, d.batch, total, d.max_q, d.max_kv, d.heads_q, c.heads_kv, c.head_dim, q, ldq,
+                   _vector(args.cu_q, torch.int32, d.batch + 1, "cu_q", dev), *_cache(args.cache, c, self._page_bytes, dev), table.data_ptr(),
+                   ld_table, _vector(args.kv_lens, torch.int32, d.batch, "kv_lens", dev), self._scale, d.causal, d.window, out, ldo, lse, ws,
+                   ws_bytes)
+        if st:
+            status_to_result(st, "Kv4AttentionPlan")
