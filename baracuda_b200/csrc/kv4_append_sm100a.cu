@@ -3,11 +3,12 @@
 //   (a, b) -> (a * cos - b * sin, b * cos + a * sin)                (channel pairs; angle by the position on the pair's axis)
 //   out = bf16(...)                                                 (one rounding, queries and dense keys)
 //   s = f16((max - min) / 15), m = f16(min), c = clamp(rint((x - m) / s), 0, 15)    (per 64 channels of the bf16 keys and values)
-// Every step is one IEEE rounding in f32, in this order, except the mean square: it is summed as pairs of f32 numbers (about 44
+// Every step is one IEEE rounding in f32, in this order.  The mean square of a key is summed as pairs of f32 numbers (about 44
 // bits) and rounded once, so its bits do not depend on the order of the sum and a key next to the border of two codes gets the
-// same code from this kernel, from the two-call sequence and from any other evaluation.
-// Bound: bytes (each element read and written once).  A head is D / 8 lanes of 8 channels, held as two quads that contain
-// whole rotation pairs, so nothing is exchanged between lanes but the sums and the groups' extrema.
+// same code from this kernel, from the two-call sequence and from any other evaluation; of a query it is an f32 sum.
+// Bound: bytes (each element read and written once), once the instructions per head are few: a head is D / 16 lanes of 16
+// channels, which contain whole rotation pairs, so nothing is exchanged between lanes but the sums and the groups' extrema; a
+// warp takes twice 512 / D heads of one token, whose sums share their exchanges, division and square root.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,11 +24,13 @@ namespace {
 __device__ int g_kv4_append_device_status = 0;
 
 constexpr int NR_THREADS = 256;
+constexpr int NR_IT = 2;          // heads of a lane group where there are many tokens
+constexpr int NR_MIN_BLOCKS = 4;  // resident blocks then: 115 us for 8191 tokens of 64 + 8 + 8 heads with the read-back, 122 with 3, 135 with 4 heads and 2 blocks
 
 struct NormRopeParams {
     NormRopeDesc g;
-    int jobs_q, jobs_kv;  // warps of one token: its queries, then its keys, then (to the cache) its values
-    uint8_t axis[128];    // of each rotation pair
+    uint32_t jobs_q, jobs_kv, jobs;  // warps of one token: its queries, then its keys, then (to the cache) its values; all
+    uint64_t axis[2][3];             // axis of each rotation pair: bit b of pair i at bit i % 64 of axis[i / 64][b]
 };
 
 // Two f32 numbers in one register pair; each operation rounds each of them once.
@@ -133,170 +136,259 @@ __device__ __forceinline__ uint32_t codes4(uint2 x, float m, float s, float inv,
 
 enum : int { HEAD_Q = 0, HEAD_K = 1, HEAD_V = 2 };
 
-// 1 / rms of IT heads per lane group from the lanes' squares.  The 8 squares of a lane are exact (16 bits each); they are added
-// with two-sums, so that sum and error together hold about 44 bits whatever the order.  With IT = 4 the lanes trade heads on
-// the way: after two exchanges each lane goes on with one head, and one division and square root serve four.
-template <int LPH, int IT>
-__device__ __forceinline__ void inverse_rms(const uint2 (&raw)[IT][2], float eps, int l, float (&r)[IT]) {
-    float s[IT], e[IT];
+// The 16 channels of a lane: quads q[0], q[2] from one place on and q[1], q[3] from another.
+struct Lane16 {
+    uint2 q[4];
+};
+
+// A lane's sum of squares; EXACT with the part that an f32 does not hold in `err`.
+template <bool EXACT>
+__device__ __forceinline__ float squares(const Lane16& x, float& err) {
+    if constexpr (EXACT) {  // squares of bf16 are exact
+        f32x2 low = 0ull, part[4];
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-        const f32x2 a = unpack2(raw[i][0].x), b = unpack2(raw[i][0].y), c = unpack2(raw[i][1].x), d = unpack2(raw[i][1].y);
-        f32x2 low = 0ull;
-        const f32x2 ab = two_sum2(mul2(a, a), mul2(b, b), low), cd = two_sum2(mul2(c, c), mul2(d, d), low);
-        const float2 t = each(two_sum2(ab, cd, low)), lo = each(low);
-        e[i] = __fadd_rn(lo.x, lo.y);
-        s[i] = two_sum(t.x, t.y, e[i]);
-    }
-    float sum = s[0], err = e[0];
-    int o = LPH / 2;
-    if constexpr (IT == 4) {
-        const bool up = (l & o) != 0;  // keeps heads 2 and 3
-        f32x2 err2 = both(up ? e[2] : e[0], up ? e[3] : e[1]);
-        const f32x2 mine = both(up ? s[2] : s[0], up ? s[3] : s[1]);
-        const f32x2 theirs = both(__shfl_xor_sync(0xffffffffu, up ? s[0] : s[2], o), __shfl_xor_sync(0xffffffffu, up ? s[1] : s[3], o));
-        err2 = add2(err2, both(__shfl_xor_sync(0xffffffffu, up ? e[0] : e[2], o), __shfl_xor_sync(0xffffffffu, up ? e[1] : e[3], o)));
-        const float2 two = each(two_sum2(mine, theirs, err2)), terr = each(err2);
-        o >>= 1;
-        const bool odd = (l & o) != 0;  // keeps the second of its two
-        err = __fadd_rn(odd ? terr.y : terr.x, __shfl_xor_sync(0xffffffffu, odd ? terr.x : terr.y, o));
-        sum = two_sum(odd ? two.y : two.x, __shfl_xor_sync(0xffffffffu, odd ? two.x : two.y, o), err);
-        o >>= 1;
-    }
-#pragma unroll
-    for (int x = IT == 4 ? LPH / 8 : LPH / 2; x > 0; x >>= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, sum, x), other_err = __shfl_xor_sync(0xffffffffu, err, x);
-        err = __fadd_rn(err, other_err);
-        sum = two_sum(sum, other, err);
-    }
-    const float mean = __fadd_rn(sum, err) * (1.0f / (8 * LPH));
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, eps)));
-    if constexpr (IT == 4) {
-#pragma unroll
-        for (int i = 0; i < IT; ++i) r[i] = __shfl_sync(0xffffffffu, inv, (i >> 1) * (LPH / 2) + (i & 1) * (LPH / 4), LPH);
+        for (int i = 0; i < 4; ++i) {
+            const f32x2 a = unpack2(x.q[i].x), b = unpack2(x.q[i].y);
+            part[i] = two_sum2(mul2(a, a), mul2(b, b), low);
+        }
+        const float2 t = each(two_sum2(two_sum2(part[0], part[1], low), two_sum2(part[2], part[3], low), low)), lo = each(low);
+        err = __fadd_rn(lo.x, lo.y);
+        return two_sum(t.x, t.y, err);
     } else {
-        r[0] = inv;
+        f32x2 a = 0ull, b = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x2 u = unpack2(x.q[i].x), v = unpack2(x.q[i].y);
+            a = fma2(u, u, a);
+            b = fma2(v, v, b);
+        }
+        const float2 t = each(add2(a, b));
+        return t.x + t.y;
     }
 }
 
-template <int D, int IT>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
-    constexpr int LPH = D / 8;     // lanes of a head
-    constexpr int HPW = 32 / LPH;  // heads of a warp
+// 1 / rms of IT heads per lane group.  The lanes trade heads first: with four, each lane goes on with one after two exchanges, so
+// the other exchanges and the root serve four.  EXACT (keys): division and square root rounded, as the definition says; queries
+// take the reciprocal root at once.
+template <int LPH, int IT, bool EXACT>
+__device__ __forceinline__ void inverse_rms(const Lane16 (&x)[IT], float eps, int l, float (&r)[IT]) {
+    float s[IT], e[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) e[i] = 0.0f, s[i] = squares<EXACT>(x[i], e[i]);
+    auto join = [&](float& sum, float& err, float other, float other_err) {
+        if constexpr (EXACT) {
+            err = __fadd_rn(err, other_err);
+            sum = two_sum(sum, other, err);
+        } else {
+            sum += other;
+        }
+    };
+    auto trade = [&](float v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); };
+    int left = IT;
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) {
+        if (left > 1) {  // keep one half of the heads
+            left /= 2;
+            const bool up = (l & o) != 0;
+#pragma unroll
+            for (int i = 0; i < left; ++i) {
+                const float give = up ? s[i] : s[left + i], give_err = up ? e[i] : e[left + i];
+                if (up) s[i] = s[left + i], e[i] = e[left + i];
+                join(s[i], e[i], trade(give, o), EXACT ? trade(give_err, o) : 0.0f);
+            }
+        } else {
+            join(s[0], e[0], trade(s[0], o), EXACT ? trade(e[0], o) : 0.0f);
+        }
+    }
+    float inv;
+    if constexpr (EXACT) {
+        inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fadd_rn(s[0], e[0]) * (1.0f / (16 * LPH)), eps)));
+    } else {
+        inv = rsqrtf(fmaf(s[0], 1.0f / (16 * LPH), eps));
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int from = IT == 4 ? (i >> 1) * (LPH / 2) + (i & 1) * (LPH / 4) : IT == 2 ? i * (LPH / 2) : 0;
+        r[i] = IT == 1 ? inv : __shfl_sync(0xffffffffu, inv, from, LPH);
+    }
+}
+
+// Angles of 4 rotation pairs.
+struct Turn {
+    f32x2 c[2], s[2];
+};
+__device__ __forceinline__ f32x2 minus(f32x2 v) { return v ^ 0x8000000080000000ull; }
+
+// Two quads as rotation pairs: of quad a's channels with quad b's, or of neighbours within each (4 pairs in either case).
+// EXACT (keys): products and sums rounded one by one; queries join them.
+template <bool EXACT>
+__device__ __forceinline__ void turn_halves(f32x2 (&a)[2], f32x2 (&b)[2], const Turn& t) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const f32x2 u = a[e], v = b[e];
+        if constexpr (EXACT) {
+            a[e] = add_products(mul2(u, t.c[e]), minus(mul2(v, t.s[e])));
+            b[e] = add_products(mul2(v, t.c[e]), mul2(u, t.s[e]));
+        } else {
+            a[e] = fma2(u, t.c[e], minus(mul2(v, t.s[e])));
+            b[e] = fma2(v, t.c[e], mul2(u, t.s[e]));
+        }
+    }
+}
+template <bool EXACT>
+__device__ __forceinline__ void turn_neighbours(f32x2 (&a)[2], f32x2 (&b)[2], const Turn& t) {
+    const float2 a0 = each(a[0]), a1 = each(a[1]), b0 = each(b[0]), b1 = each(b[1]);
+    f32x2 u[2] = {both(a0.x, a1.x), both(b0.x, b1.x)}, v[2] = {both(a0.y, a1.y), both(b0.y, b1.y)};
+    turn_halves<EXACT>(u, v, t);
+    const float2 u0 = each(u[0]), v0 = each(v[0]), u1 = each(u[1]), v1 = each(v[1]);
+    a[0] = both(u0.x, v0.x), a[1] = both(u0.y, v0.y);
+    b[0] = both(u1.x, v1.x), b[1] = both(u1.y, v1.y);
+}
+
+// Norm and rotation of IT heads in place.
+template <int LPH, int IT, bool EXACT>
+__device__ __forceinline__ void norm_and_turn(Lane16 (&x)[IT], const float* weight, const f32x2 (&w)[4][2], float eps, int l, bool interleaved,
+                                              bool turns, bool turns_second, const Turn (&t)[2]) {
+    float r[IT];
+    if (weight != nullptr) inverse_rms<LPH, IT, EXACT>(x, eps, l, r);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        f32x2 y[4][2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q][0] = unpack2(x[i].q[q].x), y[q][1] = unpack2(x[i].q[q].y);
+        if (weight != nullptr) {
+            const f32x2 r2 = both(r[i], r[i]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) y[q][e] = mul2(mul2(y[q][e], r2), w[q][e]);
+        }
+        if (interleaved) {  // pairs 8 l .. lie in quads 0 and 2, 8 l + 4 .. in 1 and 3
+            if (turns) turn_neighbours<EXACT>(y[0], y[2], t[0]);
+            if (turns_second) turn_neighbours<EXACT>(y[1], y[3], t[1]);
+        } else {
+            if (turns) turn_halves<EXACT>(y[0], y[1], t[0]);
+            if (turns_second) turn_halves<EXACT>(y[2], y[3], t[1]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[i].q[q] = make_uint2(pack2(y[q][0]), pack2(y[q][1]));
+    }
+}
+
+// WIDE: 16-byte accesses, no lane mixes rotated and other channels.
+template <int D, int IT, bool WIDE>
+__global__ void __launch_bounds__(NR_THREADS, IT == 1 ? 1 : NR_MIN_BLOCKS) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+    constexpr int LPH = D / 16;    // lanes of a head
+    constexpr int HPW = 32 / LPH;  // heads of a warp at a time
     constexpr int G = D / KV4_GROUP;
     const NormRopeDesc& g = p.g;
     const int lane = threadIdx.x & 31;
     const int sub = lane / LPH, l = lane % LPH;
-    const int jobs = p.jobs_q + p.jobs_kv * (g.to_cache ? 2 : 1);
-    const int64_t warp = static_cast<int64_t>(blockIdx.x) * (NR_THREADS / 32) + (threadIdx.x >> 5);
-    const int64_t token = warp / jobs;
-    if (token >= g.tokens) return;
-    int job = static_cast<int>(warp - token * jobs);
+    const uint32_t warp = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5);
+    const uint32_t token = warp / p.jobs;
+    if (token >= static_cast<uint32_t>(g.tokens)) return;
+    uint32_t job = warp - token * p.jobs;
     const int kind = job < p.jobs_q ? HEAD_Q : job < p.jobs_q + p.jobs_kv ? HEAD_K : HEAD_V;  // of the whole warp
     job -= kind == HEAD_Q ? 0 : kind == HEAD_K ? p.jobs_q : p.jobs_q + p.jobs_kv;
-    const int first = job * HPW * IT + sub;
+    const int begin = static_cast<int>(job) * HPW * IT, first = begin + sub;
     const int heads = kind == HEAD_Q ? g.heads_q : g.heads_kv;
 
-    // channels of this lane, two quads: rotation lanes hold 4 pairs, the others 8 channels in a row; values hold d and d + 8
-    const bool turns = kind != HEAD_V && l < g.rot_dim / 8;
-    int d0 = 8 * l, d1 = 8 * l + 4;
-    if (turns && !g.interleaved) d0 = 4 * l, d1 = g.rot_dim / 2 + 4 * l;
-    if (kind == HEAD_V) d0 = 16 * (l >> 1) + 4 * (l & 1), d1 = d0 + 8;
+    // where this lane's quads lie: rotated halves hold pairs 8 l .. 8 l + 7, everything else 16 channels in a row
+    const int half = g.rot_dim / 2;
+    const bool turns = kind != HEAD_V && 8 * l < half, turns_second = WIDE ? turns : kind != HEAD_V && 8 * l + 4 < half;  // first, last 4 pairs
+    int d[4] = {16 * l, 16 * l + 8, 16 * l + 4, 16 * l + 12};
+    if (turns && !g.interleaved) {
+        d[0] = 8 * l, d[1] = half + 8 * l;
+        d[2] = turns_second ? d[0] + 4 : g.rot_dim, d[3] = turns_second ? d[1] + 4 : g.rot_dim + 4;
+    }
 
-    // all loads first: IT heads in flight per lane
-    const __nv_bfloat16* from = kind == HEAD_Q   ? static_cast<const __nv_bfloat16*>(g.q) + token * g.ldq
-                                : kind == HEAD_K ? static_cast<const __nv_bfloat16*>(g.k) + token * g.ldk
-                                                 : static_cast<const __nv_bfloat16*>(g.v) + token * g.ldv;
-    uint2 raw[IT][2];
+    // all loads first: IT heads in flight per lane (the last head again where there is none)
+    const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(kind == HEAD_Q ? g.q : kind == HEAD_K ? g.k : g.v) +
+                                static_cast<int64_t>(token) * (kind == HEAD_Q ? g.ldq : kind == HEAD_K ? g.ldk : g.ldv);
+    Lane16 x[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-        const int h = first + i * HPW;
-        raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
-        if (h < heads) {
-            raw[i][0] = *reinterpret_cast<const uint2*>(from + static_cast<int64_t>(h) * D + d0);
-            raw[i][1] = *reinterpret_cast<const uint2*>(from + static_cast<int64_t>(h) * D + d1);
+        const __nv_bfloat16* at = from + min(first + i * HPW, heads - 1) * D;
+        if constexpr (WIDE) {
+            const uint4 a = *reinterpret_cast<const uint4*>(at + d[0]), b = *reinterpret_cast<const uint4*>(at + d[1]);
+            x[i].q[0] = make_uint2(a.x, a.y), x[i].q[2] = make_uint2(a.z, a.w);
+            x[i].q[1] = make_uint2(b.x, b.y), x[i].q[3] = make_uint2(b.z, b.w);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[i].q[q] = *reinterpret_cast<const uint2*>(at + d[q]);
         }
     }
     if (kind != HEAD_V) {
-        f32x2 c[2], s[2], ns[2];  // of this lane's 4 pairs
-        c[0] = c[1] = both(1.0f, 1.0f);
-        s[0] = s[1] = ns[0] = ns[1] = 0ull;
+        Turn t[2] = {};
         if (turns) {
-            const int half = g.rot_dim / 2;
-            float4 cv, sv;
-            if (g.axes == 1) {
-                int pos = g.positions[token];
+            // the axes of this lane's 8 pairs, 8 bits for each bit of the axis
+            uint32_t ax[3] = {0u, 0u, 0u};
+            if (g.axes > 1) {
+#pragma unroll
+                for (int bit = 0; bit < 3; ++bit) ax[bit] = static_cast<uint32_t>((l < 8 ? p.axis[0][bit] : p.axis[1][bit]) >> ((8 * l) & 63)) & 255u;
+            }
+            auto row_of = [&](int e) {
+                const uint32_t axis = ((ax[0] >> e) & 1u) | (((ax[1] >> e) & 1u) << 1) | (((ax[2] >> e) & 1u) << 2);
+                int pos = g.positions[axis * g.pos_stride + token];
                 if (pos < 0 || pos >= g.max_pos) {
                     atomicCAS(&g_kv4_append_device_status, 0, 401);
                     pos = pos < 0 ? 0 : g.max_pos - 1;
                 }
-                const float* row = g.cos_sin + static_cast<int64_t>(pos) * g.rot_dim + 4 * l;
-                cv = __ldg(reinterpret_cast<const float4*>(row));
-                sv = __ldg(reinterpret_cast<const float4*>(row + half));
-            } else {
-                float t[2][4];
+                return g.cos_sin + static_cast<int64_t>(pos) * g.rot_dim + 8 * l;
+            };
+            const bool same = ((ax[0] + 1u) & 254u) == 0u && ((ax[1] + 1u) & 254u) == 0u && ((ax[2] + 1u) & 254u) == 0u;  // each 0 or 255
+            if (same && turns_second) {  // the rule with sections: 8 pairs in a row lie on one axis
+                const float* row = row_of(0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    int pos = g.positions[p.axis[4 * l + e] * g.pos_stride + token];
-                    if (pos < 0 || pos >= g.max_pos) {
-                        atomicCAS(&g_kv4_append_device_status, 0, 401);
-                        pos = pos < 0 ? 0 : g.max_pos - 1;
-                    }
-                    const float* row = g.cos_sin + static_cast<int64_t>(pos) * g.rot_dim + 4 * l + e;
-                    t[0][e] = __ldg(row);
-                    t[1][e] = __ldg(row + half);
+                for (int n = 0; n < 2; ++n) {
+                    const float4 cv = __ldg(reinterpret_cast<const float4*>(row + 4 * n)), sv = __ldg(reinterpret_cast<const float4*>(row + half + 4 * n));
+                    t[n].c[0] = both(cv.x, cv.y), t[n].c[1] = both(cv.z, cv.w);
+                    t[n].s[0] = both(sv.x, sv.y), t[n].s[1] = both(sv.z, sv.w);
                 }
-                cv = make_float4(t[0][0], t[0][1], t[0][2], t[0][3]);
-                sv = make_float4(t[1][0], t[1][1], t[1][2], t[1][3]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    if (n == 1 && !turns_second) break;
+                    float v[2][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float* row = row_of(4 * n + e) + 4 * n + e;
+                        v[0][e] = __ldg(row);
+                        v[1][e] = __ldg(row + half);
+                    }
+                    t[n].c[0] = both(v[0][0], v[0][1]), t[n].c[1] = both(v[0][2], v[0][3]);
+                    t[n].s[0] = both(v[1][0], v[1][1]), t[n].s[1] = both(v[1][2], v[1][3]);
+                }
             }
-            c[0] = both(cv.x, cv.y), c[1] = both(cv.z, cv.w);
-            s[0] = both(sv.x, sv.y), s[1] = both(sv.z, sv.w);
-            ns[0] = both(-sv.x, -sv.y), ns[1] = both(-sv.z, -sv.w);
         }
         const float* weight = kind == HEAD_Q ? g.q_weight : g.k_weight;
-        float r[IT];
-        f32x2 w[4];
+        f32x2 w[4][2];
         if (weight != nullptr) {
-            const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight + d0)), w1 = __ldg(reinterpret_cast<const float4*>(weight + d1));
-            w[0] = both(w0.x, w0.y), w[1] = both(w0.z, w0.w), w[2] = both(w1.x, w1.y), w[3] = both(w1.z, w1.w);
-            inverse_rms<LPH, IT>(raw, g.eps, l, r);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(weight + d[q]));
+                w[q][0] = both(v.x, v.y), w[q][1] = both(v.z, v.w);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            f32x2 x[4] = {unpack2(raw[i][0].x), unpack2(raw[i][0].y), unpack2(raw[i][1].x), unpack2(raw[i][1].y)};
-            if (weight != nullptr) {
-                const f32x2 r2 = both(r[i], r[i]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = mul2(mul2(x[e], r2), w[e]);
-            }
-            if (turns) {
-                if (g.interleaved) {  // neighbours: gather the pairs' first and second channels, and back
-                    const float2 x0 = each(x[0]), x1 = each(x[1]), x2 = each(x[2]), x3 = each(x[3]);
-                    const f32x2 a0 = both(x0.x, x1.x), b0 = both(x0.y, x1.y), a1 = both(x2.x, x3.x), b1 = both(x2.y, x3.y);
-                    const float2 p0 = each(add_products(mul2(a0, c[0]), mul2(b0, ns[0]))), q0 = each(add_products(mul2(b0, c[0]), mul2(a0, s[0])));
-                    const float2 p1 = each(add_products(mul2(a1, c[1]), mul2(b1, ns[1]))), q1 = each(add_products(mul2(b1, c[1]), mul2(a1, s[1])));
-                    x[0] = both(p0.x, q0.x), x[1] = both(p0.y, q0.y), x[2] = both(p1.x, q1.x), x[3] = both(p1.y, q1.y);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const f32x2 a = x[e], b = x[2 + e];
-                        x[e] = add_products(mul2(a, c[e]), mul2(b, ns[e]));
-                        x[2 + e] = add_products(mul2(b, c[e]), mul2(a, s[e]));
-                    }
-                }
-            }
-            raw[i][0] = make_uint2(pack2(x[0]), pack2(x[1]));
-            raw[i][1] = make_uint2(pack2(x[2]), pack2(x[3]));
+        if (kind == HEAD_Q) {
+            norm_and_turn<LPH, IT, false>(x, weight, w, g.eps, l, g.interleaved != 0, turns, turns_second, t);
+        } else {
+            norm_and_turn<LPH, IT, true>(x, weight, w, g.eps, l, g.interleaved != 0, turns, turns_second, t);
         }
         if (kind == HEAD_Q || !g.to_cache) {
-            __nv_bfloat16* out = kind == HEAD_Q ? static_cast<__nv_bfloat16*>(g.q_out) + token * g.ldqo
-                                                : static_cast<__nv_bfloat16*>(g.k_out) + token * g.ldko;
+            __nv_bfloat16* out = kind == HEAD_Q ? static_cast<__nv_bfloat16*>(g.q_out) + static_cast<int64_t>(token) * g.ldqo
+                                                : static_cast<__nv_bfloat16*>(g.k_out) + static_cast<int64_t>(token) * g.ldko;
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
                 const int h = first + i * HPW;
-                if (h < heads) {
-                    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(h) * D + d0) = raw[i][0];
-                    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(h) * D + d1) = raw[i][1];
+                if (h >= heads) return;
+                __nv_bfloat16* at = out + h * D;
+                if constexpr (WIDE) {
+                    *reinterpret_cast<uint4*>(at + d[0]) = make_uint4(x[i].q[0].x, x[i].q[0].y, x[i].q[2].x, x[i].q[2].y);
+                    *reinterpret_cast<uint4*>(at + d[1]) = make_uint4(x[i].q[1].x, x[i].q[1].y, x[i].q[3].x, x[i].q[3].y);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(at + d[q]) = x[i].q[q];
                 }
             }
             return;
@@ -306,62 +398,84 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_cons
     // keys and values into the cache
     const int64_t slot = g.slots[token];
     if (slot < 0) return;
-    const int64_t page = slot / g.cache.page_size;
-    const int off = static_cast<int>(slot - page * g.cache.page_size);
-    if (page >= g.cache.num_pages) {
+    if (slot >= static_cast<int64_t>(g.cache.num_pages) * g.cache.page_size) {
         atomicCAS(&g_kv4_append_device_status, 0, 402);
         return;
     }
+    int64_t page;
+    if (slot >> 32 == 0) {
+        page = static_cast<uint32_t>(slot) / static_cast<uint32_t>(g.cache.page_size);
+    } else {
+        page = slot / g.cache.page_size;
+    }
+    const int off = static_cast<int>(slot - page * g.cache.page_size);
     uint8_t* tile = g.cache.base + page * g.cache.page_stride + (off / KV4_TILE) * kv4_tile_bytes(D);
     const int64_t head_stride = static_cast<int64_t>(g.cache.page_size / KV4_TILE) * kv4_tile_bytes(D);
     const int at = off % KV4_TILE;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int h = first + i * HPW;
-        if (job * HPW * IT + i * HPW >= heads) break;  // of the whole warp
+        if (begin + i * HPW >= heads) break;  // of the whole warp
         // the groups' extrema over the bf16 values as (max, -min), one exchange for both
-        uint32_t ext[G];
-        const uint32_t hi0 = max_bf16x2(raw[i][0].x, raw[i][0].y), hi1 = max_bf16x2(raw[i][1].x, raw[i][1].y);
-        const uint32_t lo0 = max_bf16x2(raw[i][0].x ^ 0x80008000u, raw[i][0].y ^ 0x80008000u);
-        const uint32_t lo1 = max_bf16x2(raw[i][1].x ^ 0x80008000u, raw[i][1].y ^ 0x80008000u);
-        const uint32_t e0 = max_bf16x2(__byte_perm(hi0, lo0, 0x5410), __byte_perm(hi0, lo0, 0x7632));
-        const uint32_t e1 = max_bf16x2(__byte_perm(hi1, lo1, 0x5410), __byte_perm(hi1, lo1, 0x7632));
-        float sc[G], mn[G];
+        uint32_t ext[4];
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-            ext[q] = max_bf16x2((d0 >> 6) == q ? e0 : 0xff80ff80u, (d1 >> 6) == q ? e1 : 0xff80ff80u);
-#pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ext[q] = max_bf16x2(ext[q], __shfl_xor_sync(0xffffffffu, ext[q], o));
-            const float hi = __uint_as_float(ext[q] << 16), lo = -__uint_as_float(ext[q] & 0xffff0000u);
-            sc[q] = __half2float(__float2half_rn(min_nan(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), KV4_F16_MAX)));
-            mn[q] = __fadd_rn(__half2float(__float2half_rn(max_nan(min_nan(lo, KV4_F16_MAX), -KV4_F16_MAX))), 0.0f);  // no -0: one form of a zero
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t hi = max_bf16x2(x[i].q[q].x, x[i].q[q].y), lo = max_bf16x2(x[i].q[q].x ^ 0x80008000u, x[i].q[q].y ^ 0x80008000u);
+            ext[q] = max_bf16x2(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
         }
-        float s0 = sc[0], m0 = mn[0], s1 = sc[0], m1 = mn[0];
+        float sc[G], mn[G], rc[G];
+        bool plain = true;
 #pragma unroll
-        for (int q = 1; q < G; ++q) {
-            if ((d0 >> 6) == q) s0 = sc[q], m0 = mn[q];
-            if ((d1 >> 6) == q) s1 = sc[q], m1 = mn[q];
+        for (int n = 0; n < G; ++n) {
+            uint32_t m = 0xff80ff80u;  // minus infinity
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if ((d[q] >> 6) == n) m = max_bf16x2(m, ext[q]);
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) m = max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float hi = __uint_as_float(m << 16), lo = -__uint_as_float(m & 0xffff0000u);
+            sc[n] = __half2float(__float2half_rn(min_nan(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), KV4_F16_MAX)));
+            mn[n] = __fadd_rn(__half2float(__float2half_rn(max_nan(min_nan(lo, KV4_F16_MAX), -KV4_F16_MAX))), 0.0f);  // no -0: one form of a zero
+            rc[n] = __fdiv_rn(1.0f, sc[n]);
+            plain = plain && sc[n] > 0.0f && sc[n] < KV4_F16_MAX && fabsf(mn[n]) < KV4_F16_MAX;
         }
-        const bool plain0 = s0 > 0.0f && s0 < KV4_F16_MAX && fabsf(m0) < KV4_F16_MAX, plain1 = s1 > 0.0f && s1 < KV4_F16_MAX && fabsf(m1) < KV4_F16_MAX;
-        const bool plain = __all_sync(0xffffffffu, (plain0 && plain1) || h >= heads);
-        const uint32_t k0 = codes4(raw[i][0], m0, s0, __fdiv_rn(1.0f, s0), plain), k1 = codes4(raw[i][1], m1, s1, __fdiv_rn(1.0f, s1), plain);
+        plain = __all_sync(0xffffffffu, plain || h >= heads);
         if (h >= heads) continue;
-        uint8_t* to = tile + h * head_stride;
-        if (kind == HEAD_K) {  // bytes 0, 1 and 2, 3 of each quad share a byte
-            const uint32_t b0 = k0 | (k0 >> 4), b1 = k1 | (k1 >> 4);
-            *reinterpret_cast<uint16_t*>(to + kv4_key_byte<D>(at, d0)) = static_cast<uint16_t>(__byte_perm(b0, 0u, 0x4420));
-            *reinterpret_cast<uint16_t*>(to + kv4_key_byte<D>(at, d1)) = static_cast<uint16_t>(__byte_perm(b1, 0u, 0x4420));
-        } else {  // channels d and d + 8 share a byte
-            const uint32_t bytes = k0 | (k1 << 4);
-            uint8_t* v = to + kv4_value_byte<D>(at, d0);
+        uint32_t code[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[64 * e] = static_cast<uint8_t>(bytes >> (8 * e));
+        for (int q = 0; q < 4; ++q) {
+            float s = sc[0], m = mn[0], rec = rc[0];
+#pragma unroll
+            for (int n = 1; n < G; ++n)
+                if ((d[q] >> 6) == n) s = sc[n], m = mn[n], rec = rc[n];
+            code[q] = codes4(x[i].q[q], m, s, rec, plain);
+        }
+        uint8_t* to = tile + h * head_stride;
+        if (kind == HEAD_K) {  // neighbouring channels share a byte; bytes 0 and 2 of each word below
+            uint32_t b[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) b[q] = code[q] | (code[q] >> 4);
+            if constexpr (WIDE) {  // 8 channels in a row, 4 bytes
+                *reinterpret_cast<uint32_t*>(to + kv4_key_byte<D>(at, d[0])) = __byte_perm(b[0], b[2], 0x6420);
+                *reinterpret_cast<uint32_t*>(to + kv4_key_byte<D>(at, d[1])) = __byte_perm(b[1], b[3], 0x6420);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<uint16_t*>(to + kv4_key_byte<D>(at, d[q])) = static_cast<uint16_t>(__byte_perm(b[q], 0u, 0x4420));
+            }
+        } else {  // channels d and d + 8 share a byte
+            uint8_t* v = to + kv4_value_byte<D>(at, d[0]);
+            const uint32_t lo = code[0] | (code[1] << 4), hi = code[2] | (code[3] << 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[64 * e] = static_cast<uint8_t>(lo >> (8 * e));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[64 * (4 + e)] = static_cast<uint8_t>(hi >> (8 * e));
         }
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-            if (l == q) {
-                const __half2 pair = __floats2half2_rn(sc[q], mn[q]);
-                *reinterpret_cast<__half2*>(to + kv4_pair_offset(D, kind == HEAD_V) + (at * G + q) * 4) = pair;
+        for (int n = 0; n < G; ++n) {
+            if (l == n) {
+                const __half2 pair = __floats2half2_rn(sc[n], mn[n]);
+                *reinterpret_cast<__half2*>(to + kv4_pair_offset(D, kind == HEAD_V) + (at * G + n) * 4) = pair;
             }
         }
     }
@@ -369,20 +483,24 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_cons
 
 template <int D>
 int32_t launch_norm_rope_d(NormRopeParams& p, cudaStream_t stream) {
-    constexpr int HPW = 256 / D;
+    constexpr int HPW = 512 / D;
+    const NormRopeDesc& g = p.g;
     auto go = [&](auto kern, int it) {
-        p.jobs_q = (p.g.heads_q + HPW * it - 1) / (HPW * it);
-        p.jobs_kv = (p.g.heads_kv + HPW * it - 1) / (HPW * it);
-        const int64_t jobs = p.jobs_q + p.jobs_kv * (p.g.to_cache ? 2 : 1);
-        const int64_t blocks = (jobs * p.g.tokens + NR_THREADS / 32 - 1) / (NR_THREADS / 32);
-        if (blocks > 0x7fffffff) return static_cast<int32_t>(BQ_STATUS_UNSUPPORTED);
+        p.jobs_q = (g.heads_q + HPW * it - 1) / (HPW * it);
+        p.jobs_kv = (g.heads_kv + HPW * it - 1) / (HPW * it);
+        p.jobs = p.jobs_q + p.jobs_kv * (g.to_cache ? 2 : 1);
+        const int64_t blocks = (static_cast<int64_t>(p.jobs) * g.tokens + NR_THREADS / 32 - 1) / (NR_THREADS / 32);
+        if (blocks * (NR_THREADS / 32) > 0xffffffffll) return static_cast<int32_t>(BQ_STATUS_UNSUPPORTED);  // counted in 32 bits
         kern<<<static_cast<unsigned>(blocks), NR_THREADS, 0, stream>>>(p);
         return static_cast<int32_t>(cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE);
     };
-    // few tokens: one head per lane group, as many warps as there are; many: four, for bytes in flight and one look at the angles
-    const int64_t heads = p.g.heads_q + static_cast<int64_t>(p.g.heads_kv) * (p.g.to_cache ? 2 : 1);
-    if (heads * p.g.tokens < 16384) return go(norm_rope_kernel<D, 1>, 1);
-    return go(norm_rope_kernel<D, 4>, 4);
+    auto aligned = [](const void* ptr, int64_t ld) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && ld % 8 == 0; };
+    const bool wide = g.rot_dim % 16 == 0 && aligned(g.q, g.ldq) && aligned(g.k, g.ldk) && aligned(g.q_out, g.ldqo) &&
+                      (g.to_cache ? aligned(g.v, g.ldv) : aligned(g.k_out, g.ldko));
+    // few tokens: one head per lane group, as many warps as there are; many: several, for bytes in flight and one look at the angles
+    const int64_t heads = g.heads_q + static_cast<int64_t>(g.heads_kv) * (g.to_cache ? 2 : 1);
+    if (heads * g.tokens < 16384) return wide ? go(norm_rope_kernel<D, 1, true>, 1) : go(norm_rope_kernel<D, 1, false>, 1);
+    return wide ? go(norm_rope_kernel<D, NR_IT, true>, NR_IT) : go(norm_rope_kernel<D, NR_IT, false>, NR_IT);
 }
 
 // One lane of the reader holds 8 channels of one token and head: keys 8 in a row (one word), values r = 0..7 of one nibble
@@ -441,7 +559,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 int32_t launch_qk_norm_rope(const NormRopeDesc& g, cudaStream_t stream) {
     NormRopeParams p = {};
     p.g = g;
-    for (int i = 0; i < 128; ++i) p.axis[i] = (g.axis_of_pair != nullptr && i < g.rot_dim / 2) ? g.axis_of_pair[i] : 0;
+    for (int i = 0; g.axis_of_pair != nullptr && i < g.rot_dim / 2; ++i)
+        for (int bit = 0; bit < 3; ++bit) p.axis[i / 64][bit] |= static_cast<uint64_t>((g.axis_of_pair[i] >> bit) & 1) << (i % 64);
     p.g.axis_of_pair = nullptr;
     switch (g.head_dim) {
         case 64: return launch_norm_rope_d<64>(p, stream);

@@ -531,20 +531,20 @@ def test_a_layers_attention_step_between_its_quantized_projections():
 
 
 def test_norm_and_rotation_round_step_by_step():
-    """The stated f32 steps, each rounded once, in plain torch operations: the same bits (codes of the cache depend on them)."""
+    """The stated f32 steps of the keys, each rounded once, in plain torch operations: the same bits (the cache's codes depend on them)."""
     t, heads, dim = 3000, 8, 128
     g = _gen(17)
     x = (_randn(g, t, (heads + 1) * dim) * torch.exp(_randn(g, (heads + 1) * dim))).to(BF16)
-    q, k = x[:, : heads * dim], x[:, heads * dim :]
+    k, q = x[:, : heads * dim], x[:, heads * dim :]
     w = 1 + 0.3 * _randn(g, dim)
     angles = _angles(1000, dim)
     positions = torch.randint(0, 1000, (t,), generator=g, device="cuda", dtype=torch.int32)
     for interleaved in (False, True):
         for weight in (w, None):
             q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-            bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(t, heads, 1, dim, interleaved=interleaved, eps=1e-6)).run(
+            bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(t, 1, heads, dim, interleaved=interleaved, eps=1e-6)).run(
                 None, None, bq.QkNormRopeArgs(q=q, k=k, q_out=q_out, k_out=k_out, q_weight=weight, k_weight=weight, cos_sin=angles, positions=positions))
-            y = q.reshape(t, heads, dim)
+            y = k.reshape(t, heads, dim)
             if weight is not None:
                 mean = (y.double().square().sum(-1, keepdim=True) / dim).float()
                 y = y.float() * (1.0 / torch.sqrt(mean + 1e-6)) * weight
@@ -553,4 +553,4 @@ def test_norm_and_rotation_round_step_by_step():
             a, b = (y[..., 0::2], y[..., 1::2]) if interleaved else y.chunk(2, -1)
             one, two = a * c - b * s, b * c + a * s
             want = torch.stack([one, two], -1).flatten(-2) if interleaved else torch.cat([one, two], -1)
-            assert torch.equal(q_out.reshape(t, heads, dim), want.to(BF16))
+            assert torch.equal(k_out.reshape(t, heads, dim), want.to(BF16))
