@@ -2,7 +2,8 @@
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * weight                    (per head; skipped without a weight)
 //   (a, b) -> (a * cos - b * sin, b * cos + a * sin)                (channel pairs; angle by the position on the pair's axis)
 //   out = bf16(...)                                                 (one rounding, queries and dense keys)
-//   s = f16((max - min) / 15), m = f16(min), c = clamp(rint((x - m) / s), 0, 15)    (per 64 channels of the bf16 keys and values)
+//   s = f16((max - min) / 15), m = f16(min), c = clamp(rint((x - m) / s), 0, 15)    (per 64 channels of the bf16 keys and values;
+//   max and min cut to +-32768)
 // Every step is one IEEE rounding in f32, in this order.  The mean square of a key is summed as pairs of f32 numbers (about 44
 // bits) and rounded once, so its bits do not depend on the order of the sum and a key next to the border of two codes gets the
 // same code from this kernel, from the two-call sequence and from any other evaluation; of a query it is an f32 sum.
@@ -107,7 +108,7 @@ __device__ __forceinline__ uint2 pack4(const float* x) {
 }
 
 // Codes of a quad of bf16 channels, one byte each: c = clamp(rint((x - m) / s), 0, 15), the quotient rounded once.
-// For scales and minima that were not cut (`plain`) the quotient comes from the reciprocal: with q near (x - m) / s the
+// For groups within the cut, of more than one value (`plain`), the quotient comes from the reciprocal: with q near (x - m) / s the
 // remainder r = (x - m) - q s is exact, and q + r / s, off by less than 2^-46 of itself before its one rounding, rounds as the
 // quotient does: s has 11 significant bits, so a quotient of 24 bits by s is at least 2^-36 away from where the rounding changes.
 __device__ __forceinline__ uint32_t codes4(uint2 x, float m, float s, float inv, bool plain) {
@@ -433,11 +434,12 @@ __global__ void __launch_bounds__(NR_THREADS, IT == 1 ? 1 : NR_MIN_BLOCKS) norm_
                 if ((d[q] >> 6) == n) m = max_bf16x2(m, ext[q]);
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) m = max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float hi = __uint_as_float(m << 16), lo = -__uint_as_float(m & 0xffff0000u);
-            sc[n] = __half2float(__float2half_rn(min_nan(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), KV4_F16_MAX)));
-            mn[n] = __fadd_rn(__half2float(__float2half_rn(max_nan(min_nan(lo, KV4_F16_MAX), -KV4_F16_MAX))), 0.0f);  // no -0: one form of a zero
+            const float hi = max_nan(min_nan(__uint_as_float(m << 16), KV4_CUT), -KV4_CUT);
+            const float lo = max_nan(min_nan(-__uint_as_float(m & 0xffff0000u), KV4_CUT), -KV4_CUT);
+            sc[n] = __half2float(__float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)));
+            mn[n] = __fadd_rn(__half2float(__float2half_rn(lo)), 0.0f);  // no -0: one form of a zero
             rc[n] = __fdiv_rn(1.0f, sc[n]);
-            plain = plain && sc[n] > 0.0f && sc[n] < KV4_F16_MAX && fabsf(mn[n]) < KV4_F16_MAX;
+            plain = plain && sc[n] > 0.0f && hi < KV4_CUT && lo > -KV4_CUT;
         }
         plain = __all_sync(0xffffffffu, plain || h >= heads);
         if (h >= heads) continue;

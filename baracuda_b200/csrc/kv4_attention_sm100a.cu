@@ -22,8 +22,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/baracuda_kernels_q.h"
-#include "kv4_format.cuh"
-#include "ptx_sm100a.cuh"
+#include "kv4_attention.cuh"
 
 namespace bq {
 
@@ -35,33 +34,8 @@ constexpr int AT_WARPS = 4;
 constexpr int AT_STAGES = 3;
 constexpr int AT_STEP = 32;  // tokens of a warp's step
 constexpr float SLACK = 4.0f;
-constexpr float NO_REF = -1.0e30f;
-constexpr long long AT_WAIT_LIMIT = 2000000000LL;  // cycles: about a second
+constexpr int AT_ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
 
-struct AttnParams {
-    const __nv_bfloat16* q;
-    int64_t ldq;
-    const int32_t* cu_q;
-    Kv4Cache cache;
-    const int32_t* table;
-    int64_t ld_table;
-    const int32_t* kv_lens;
-    __nv_bfloat16* out;
-    int64_t ldo;
-    float* lse;
-    float scale_log2;  // scale * log2(e)
-    int32_t causal, window;
-    int32_t batch, total_q, max_q, max_kv, heads_q, group;
-    int32_t row_tiles, splits;
-    float* part_o;   // [tile][split][rows][D]
-    float2* part_ml; // [tile][split][rows]
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -73,29 +47,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// A sequence as this launch sees it: query rows [row0, row0 + n), len keys.  Lengths beyond what the caller announced are cut
-// (and reported), so that no read or write leaves the buffers.
-struct Sequence {
-    int row0, n, len;
-};
-__device__ __forceinline__ Sequence sequence_of(const AttnParams& p, int b) {
-    Sequence s;
-    int end = p.cu_q[b + 1];
-    s.row0 = p.cu_q[b];
-    s.len = p.kv_lens[b];
-    if (s.row0 < 0 || end > p.total_q || end - s.row0 > p.max_q || s.len > p.max_kv) atomicCAS(&g_kv4_attention_device_status, 0, 403);
-    s.row0 = max(s.row0, 0);
-    end = min(end, p.total_q);
-    s.n = max(0, min(end - s.row0, p.max_q));
-    s.len = max(0, min(s.len, p.max_kv));
-    return s;
-}
-
 template <int D, int NT>
 struct AttnSmem {
     static constexpr int STAGE = (AT_STEP / KV4_TILE) * kv4_tile_bytes(D);
@@ -125,7 +76,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
     const int rt = id % p.row_tiles;
     id /= p.row_tiles;
     const int hk = id % p.cache.heads_kv, b = id / p.cache.heads_kv;
-    const Sequence sq = sequence_of(p, b);
+    const Sequence sq = sequence_of(p, b, &g_kv4_attention_device_status);
     const int rows = min(ROWS, sq.n * p.group - rt * ROWS);  // row = query index * group + head in group
     if (rows <= 0) return;
 
@@ -265,7 +216,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             l[nt][e] = 0.0f;
-            ref[nt][e] = NO_REF;
+            ref[nt][e] = KV4_NO_REF;
 #pragma unroll
             for (int g = 0; g < G; ++g) z[nt][e][g] = 0.0f;
         }
@@ -281,7 +232,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
         if (!mbar_try_wait(&bars[stage], parity)) {
             const long long t0 = clock64();
             while (!mbar_try_wait(&bars[stage], parity)) {
-                if (clock64() - t0 > AT_WAIT_LIMIT) {
+                if (clock64() - t0 > KV4_WAIT_LIMIT) {
                     gave_up = true;
                     break;
                 }
@@ -478,7 +429,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
         const long long t0 = clock64();
         for (int s = 0; s < AT_STAGES; ++s) {
             if (step + s * AT_WARPS >= my_end) break;
-            while (!mbar_try_wait(&bars[stage], parity) && clock64() - t0 < AT_WAIT_LIMIT) {
+            while (!mbar_try_wait(&bars[stage], parity) && clock64() - t0 < KV4_WAIT_LIMIT) {
             }
             if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
         }
@@ -515,7 +466,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
     __syncthreads();
     for (int at = threadIdx.x; at < rows * (D / 4); at += AT_WARPS * 32) {
         const int row = at / (D / 4), d = at % (D / 4) * 4;
-        float m = NO_REF;
+        float m = KV4_NO_REF;
 #pragma unroll
         for (int w = 0; w < AT_WARPS; ++w) m = fmaxf(m, join_ml[w * ROWS + row].x);
         float sum = 0.0f;
@@ -546,23 +497,23 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
 }
 
 // Adds the slices of one block of rows, in slice order.  One warp per row.
-template <int D, int NT>
+template <int D>
 __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr int ROWS = 8 * NT;
+    const int rows_of_tile = p.tile_rows;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    const int row = static_cast<int>(id % ROWS);
-    const int64_t tile_id = id / ROWS;
+    const int row = static_cast<int>(id % rows_of_tile);
+    const int64_t tile_id = id / rows_of_tile;
     int rest = static_cast<int>(tile_id / p.row_tiles);
     const int rt = static_cast<int>(tile_id % p.row_tiles);
     const int hk = rest % p.cache.heads_kv, b = rest / p.cache.heads_kv;
     if (b >= p.batch) return;
-    const Sequence sq = sequence_of(p, b);
-    const int gr = rt * ROWS + row;
+    const Sequence sq = sequence_of(p, b, &g_kv4_attention_device_status);
+    const int gr = rt * rows_of_tile + row;
     if (gr >= sq.n * p.group) return;
-    const int64_t slot0 = tile_id * p.splits * ROWS + row;
-    float m = NO_REF;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[slot0 + static_cast<int64_t>(s) * ROWS].x);
+    const int64_t slot0 = tile_id * p.splits * rows_of_tile + row;
+    float m = KV4_NO_REF;
+    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[slot0 + static_cast<int64_t>(s) * rows_of_tile].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     constexpr int PER = D / 32;
@@ -570,7 +521,7 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.0f;
     for (int s = 0; s < p.splits; ++s) {
-        const int64_t slot = slot0 + static_cast<int64_t>(s) * ROWS;
+        const int64_t slot = slot0 + static_cast<int64_t>(s) * rows_of_tile;
         const float2 ml = p.part_ml[slot];
         const float f = ex2(ml.x - m);
         sum = fmaf(ml.y, f, sum);
@@ -591,29 +542,32 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     if (p.lse != nullptr && lane == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
 }
 
-struct Shape {
-    int nt, row_tiles, splits;
-    int64_t tiles;
-};
-
-constexpr int ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
-
-Shape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
-    Shape s;
+// Which kernel and how the work is cut.  Up to 16 rows of a kv head the codes go to mma.sync as they are (8 rows where D is 256: its
+// accumulators take the registers); beyond, keys and values are brought to f16 in shared memory for tcgen05 blocks of 128 rows,
+// or two of them from 129 rows on (D <= 128).  Slices fill the SMs where there are few blocks.
+AttnShape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
+    AttnShape s;
     const int64_t rows = max_q * (heads_q / heads_kv);
-    s.nt = rows > 8 && head_dim <= 128 ? 2 : 1;
-    s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
+    s.tensor = rows > (head_dim <= 128 ? 16 : 8);
+    s.tile_rows = s.tensor ? (rows > 128 && head_dim <= 128 ? 256 : 128) : (rows > 8 ? 16 : 8);
+    s.row_tiles = static_cast<int>((rows + s.tile_rows - 1) / s.tile_rows);
     s.tiles = batch * heads_kv * s.row_tiles;
-    const int64_t steps = (max_kv + AT_STEP * AT_WARPS - 1) / (AT_STEP * AT_WARPS);  // of a CTA
-    const int64_t want = (ASSUMED_SMS * 8 + s.tiles - 1) / (s.tiles > 0 ? s.tiles : 1);
-    const int64_t most = (steps + 1) / 2;
+    int64_t want, most;
+    if (s.tensor) {  // one block per SM; a slice has at least 512 keys
+        want = AT_ASSUMED_SMS / (s.tiles > 0 ? s.tiles : 1);
+        most = max_kv / 512;
+    } else {
+        const int64_t steps = (max_kv + AT_STEP * AT_WARPS - 1) / (AT_STEP * AT_WARPS);  // of a CTA
+        want = (AT_ASSUMED_SMS * 8 + s.tiles - 1) / (s.tiles > 0 ? s.tiles : 1);
+        most = (steps + 1) / 2;
+    }
     s.splits = static_cast<int>(want < most ? want : most);
     if (s.splits < 1) s.splits = 1;
     return s;
 }
 
 template <int D, int NT>
-int32_t launch_d(AttnParams& p, const Shape& s, cudaStream_t stream) {
+int32_t launch_rows(const AttnParams& p, const AttnShape& s, cudaStream_t stream) {
     auto kern = kv4_attention_kernel<D, NT>;
     using L = AttnSmem<D, NT>;
     if (L::TOTAL > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) {
@@ -621,31 +575,41 @@ int32_t launch_d(AttnParams& p, const Shape& s, cudaStream_t stream) {
         return BQ_STATUS_LAUNCH_FAILURE;
     }
     kern<<<static_cast<unsigned>(s.tiles * s.splits), AT_WARPS * 32, L::TOTAL, stream>>>(p);
-    if (cudaPeekAtLastError() != cudaSuccess) return BQ_STATUS_LAUNCH_FAILURE;
-    if (s.splits > 1) {
-        kv4_attention_join_kernel<D, NT><<<static_cast<unsigned>((s.tiles * 8 * NT + 3) / 4), 128, 0, stream>>>(p);
-        if (cudaPeekAtLastError() != cudaSuccess) return BQ_STATUS_LAUNCH_FAILURE;
+    return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
+}
+
+template <int D>
+int32_t launch_d(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
+    int32_t st;
+    if (s.tensor) {
+        st = launch_kv4_prompt(p, s, stream);
+    } else if constexpr (D <= 128) {
+        st = s.tile_rows == 16 ? launch_rows<D, 2>(p, s, stream) : launch_rows<D, 1>(p, s, stream);
+    } else {
+        st = launch_rows<D, 1>(p, s, stream);
     }
-    return BQ_STATUS_OK;
+    if (st != BQ_STATUS_OK || s.splits == 1) return st;
+    kv4_attention_join_kernel<D><<<static_cast<unsigned>((s.tiles * s.tile_rows + 3) / 4), 128, 0, stream>>>(p);
+    return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
 }
 
 }  // namespace
 
 bool kv4_attention_fits(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim) {
     if (batch == 0 || max_q == 0) return true;
-    const Shape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
-    return s.tiles * 16 <= 0x7fffffff && s.tiles * s.splits <= 0x7fffffff;
+    const AttnShape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
+    return s.tiles * s.tile_rows <= 0x7fffffff && s.tiles * s.splits <= 0x7fffffff;
 }
 
 size_t kv4_attention_workspace_bytes(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv,
                                      int32_t head_dim) {
-    const Shape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
+    const AttnShape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
     if (s.splits <= 1) return 0;
-    return static_cast<size_t>(s.tiles) * s.splits * 8 * s.nt * (head_dim + 2) * 4;
+    return static_cast<size_t>(s.tiles) * s.splits * s.tile_rows * (head_dim + 2) * 4;
 }
 
 int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
-    const Shape s = shape_of(g.batch, g.max_q, g.max_kv, g.heads_q, g.cache.heads_kv, g.cache.head_dim);
+    const AttnShape s = shape_of(g.batch, g.max_q, g.max_kv, g.heads_q, g.cache.heads_kv, g.cache.head_dim);
     AttnParams p;
     p.q = static_cast<const __nv_bfloat16*>(g.q);
     p.ldq = g.ldq;
@@ -668,12 +632,13 @@ int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
     p.group = g.heads_q / g.cache.heads_kv;
     p.row_tiles = s.row_tiles;
     p.splits = s.splits;
+    p.tile_rows = s.tile_rows;
     p.part_o = static_cast<float*>(g.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + s.tiles * s.splits * 8 * s.nt * g.cache.head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + s.tiles * s.splits * s.tile_rows * g.cache.head_dim);
     switch (g.cache.head_dim) {
-        case 64: return s.nt == 2 ? launch_d<64, 2>(p, s, stream) : launch_d<64, 1>(p, s, stream);
-        case 128: return s.nt == 2 ? launch_d<128, 2>(p, s, stream) : launch_d<128, 1>(p, s, stream);
-        case 256: return launch_d<256, 1>(p, s, stream);
+        case 64: return launch_d<64>(p, s, stream);
+        case 128: return launch_d<128>(p, s, stream);
+        case 256: return launch_d<256>(p, s, stream);
         default: return BQ_STATUS_UNSUPPORTED;
     }
 }
@@ -685,7 +650,8 @@ int32_t read_and_clear_kv4_attention_device_status() {
         int zero = 0;
         (void)cudaMemcpyToSymbol(g_kv4_attention_device_status, &zero, sizeof(int));
     }
-    return v;
+    const int prompt = read_and_clear_kv4_prompt_device_status();
+    return v != 0 ? v : prompt;
 }
 
 }  // namespace bq

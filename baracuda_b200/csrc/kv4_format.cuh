@@ -25,7 +25,7 @@ namespace bq {
 
 constexpr int KV4_GROUP = 64;  // channels that share a scale and a minimum
 constexpr int KV4_TILE = 16;   // tokens of a tile
-constexpr float KV4_F16_MAX = 65504.0f;
+constexpr float KV4_CUT = 32768.0f;  // channels beyond are cut: every value of the cache is then a finite f16 number
 
 __host__ __device__ constexpr int kv4_tile_bytes(int d) { return 18 * d; }
 __host__ __device__ constexpr int kv4_pair_offset(int d, int values) { return 16 * d + values * d; }

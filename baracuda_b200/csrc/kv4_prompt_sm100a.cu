@@ -1,0 +1,643 @@
+// Attention of many query rows (prompts, chunks of them, batches of drafted tokens) over the 4-bit cache: the formulas of
+// kv4_attention_sm100a.cu on tcgen05.
+//
+// A CTA takes 128 or 256 rows (query index x head of the kv head's group) of one sequence and kv head and walks the keys in
+// steps of KT.  Keys and values become f16 in shared memory once per step, for all rows:
+//   k'[t] = f16(s * c + m), one fused operation per pair; the keys' channels keep the order in which the masks leave them
+//   (0 4 1 5 2 6 3 7 of each 8), which the queries are given too: a product does not mind.
+//   v' likewise, but stored by channel with the tokens in a row, as the masks leave pairs of tokens: both products have
+//   operands whose contraction index is contiguous, in the 128-byte swizzle.
+// S = Q K'^T (f16 x f16 -> f32 in TMEM), one softmax thread per row reads S, writes P (f16) over it in TMEM, O += P V' with P as
+// the operand from TMEM.  Queries are brought to f16 by a power of two per row (exact unless 2^-38 of the row's largest).
+// Roundings to 16 bits: k', v' and P, 2^-11 each, and the output.
+// The softmax reads S twice, first for the maximum: a row's reference moves only when a score exceeds it by 2^SLACK, and O is
+// rescaled (TMEM -> registers -> TMEM) only then.
+//
+// Two row blocks (256 rows, D <= 128): while one block's softmax runs, the tensor core works on the other.  One row block
+// (128 rows; D = 256, or few rows): S is double-buffered instead, the next step's S is computed under this step's softmax.
+// Warps: 4 softmax warps per row block, the other 8 or 4 of twelve bring keys and values to f16, one issues the MMAs.
+// Every mbarrier wait is bounded (status 412..416).
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/baracuda_kernels_q.h"
+#include "kv4_attention.cuh"
+
+namespace bq {
+
+namespace {
+
+__device__ int g_kv4_prompt_device_status = 0;
+
+constexpr float PR_SLACK = 7.0f;  // p <= 2^(SLACK + LIFT) stays within f16
+constexpr float PR_LIFT = 8.0f;   // f16's range below the reference: 2^-22 in full precision
+constexpr int PR_WARPS = 13;
+constexpr int PR_THREADS = PR_WARPS * 32;
+
+template <int D, int NQ>
+struct PromptCfg {
+    static constexpr int KT = D == 256 ? 64 : 128;  // keys of a step
+    static constexpr int SOFTMAX_WARPS = 4 * NQ;
+    static constexpr int FEED_WARPS = 12 - SOFTMAX_WARPS;
+    static constexpr int Q_BYTES = NQ * 128 * D * 2;
+    static constexpr int K_BYTES = KT * D * 2;  // V the same
+    static constexpr int K_OFF = Q_BYTES;
+    static constexpr int V_OFF = K_OFF + 2 * K_BYTES;
+    static constexpr int BAR_OFF = V_OFF + 2 * K_BYTES;
+    static constexpr int FLAG_OFF = BAR_OFF + 192;           // [2][dead, nan][KT / 16] halfwords
+    static constexpr int TOTAL = FLAG_OFF + 2 * 2 * 8 * 2 + 1024;  // + alignment slack
+    static constexpr uint32_t S_COL = NQ * D;                // TMEM columns: O of each block, then two S
+};
+
+struct PromptBars {
+    uint64_t kfull[2], vfull[2], kfree[2], vfree[2], sfull[2], pready[2], pvdone[2], qfull, done;
+    uint32_t tmem_slot;
+    uint32_t abort_word;
+};
+static_assert(sizeof(PromptBars) <= 192, "fits");
+
+__device__ __forceinline__ void give_up(volatile uint32_t* abort_word, int code) {
+    *abort_word = 1u;
+    atomicCAS(&g_kv4_prompt_device_status, 0, code);
+}
+
+// kind::f16, f16 operands, f32 accumulator, both K-major; A from shared memory or from TMEM.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));  // (a & mask) | bits
+    return r;
+}
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+// The 8 codes of a word as 4 pairs of f16 values s * c + m: pairs (0, 4), (1, 5), (2, 6), (3, 7), where nibbles 0, 2, 4, 6 take
+// (s, m) of `even` and 1, 3, 5, 7 the same (keys: one scale; values: nibble parity is a channel, the pair two tokens, and the
+// shifted half two further tokens, hence four parameters).
+__device__ __forceinline__ void expand(uint32_t w, __half2 s_lo, __half2 m_lo, __half2 s_hi, __half2 m_hi, uint32_t (&out)[4]) {
+    const uint32_t w8 = w >> 8;
+    const __half2 k1024 = as_h2(0xe400e400u), k16 = as_h2(0x2c002c00u), k64 = as_h2(0xd400d400u);  // -1024, 1 / 16, -64
+    // 1024 + c and 1024 + 16 c as f16, then c, both exact
+    const __half2 c0 = __hadd2(as_h2(lop_and_or(w, 0x000f000fu, 0x64006400u)), k1024);
+    const __half2 c1 = __hfma2(as_h2(lop_and_or(w, 0x00f000f0u, 0x64006400u)), k16, k64);
+    const __half2 c2 = __hadd2(as_h2(lop_and_or(w8, 0x000f000fu, 0x64006400u)), k1024);
+    const __half2 c3 = __hfma2(as_h2(lop_and_or(w8, 0x00f000f0u, 0x64006400u)), k16, k64);
+    out[0] = h2(__hfma2(c0, s_lo, m_lo));
+    out[1] = h2(__hfma2(c1, s_lo, m_lo));
+    out[2] = h2(__hfma2(c2, s_hi, m_hi));
+    out[3] = h2(__hfma2(c3, s_hi, m_hi));
+}
+
+template <int D, int NQ>
+__global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ AttnParams p) {
+    using C = PromptCfg<D, NQ>;
+    constexpr int KT = C::KT;
+    constexpr int G = D / KV4_GROUP;
+    constexpr int W = D >= 128 ? 2 : 1;
+    constexpr int TILE = kv4_tile_bytes(D);
+    constexpr int ROWS = 128 * NQ;
+    extern __shared__ uint8_t pr_smem_raw[];
+    uint8_t* smem = pr_smem_raw + ((1024u - (smem_u32(pr_smem_raw) & 1023u)) & 1023u);
+    PromptBars* bar = reinterpret_cast<PromptBars*>(smem + C::BAR_OFF);
+    volatile uint32_t* abort_word = &bar->abort_word;
+    uint16_t* flags = reinterpret_cast<uint16_t*>(smem + C::FLAG_OFF);  // [stage][0 dead, 1 nan][tile of 16 keys]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // blocks of late rows see the most keys: they go first
+    int id = blockIdx.x;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int rt = p.row_tiles - 1 - id % p.row_tiles;
+    id /= p.row_tiles;
+    const int hk = id % p.cache.heads_kv, b = id / p.cache.heads_kv;
+    const int64_t tile_id = (static_cast<int64_t>(b) * p.cache.heads_kv + hk) * p.row_tiles + rt;
+    const Sequence sq = sequence_of(p, b, &g_kv4_prompt_device_status);
+    const int all_rows = sq.n * p.group;
+    const int rows = min(ROWS, all_rows - rt * ROWS);
+    if (rows <= 0) return;
+    const int past = sq.len - sq.n;
+    const int i_first = rt * ROWS / p.group, i_last = (rt * ROWS + rows - 1) / p.group;
+    const int hi_all = max(0, p.causal ? min(sq.len, past + i_last + 1) : sq.len);
+    const int lo_all = p.window > 0 ? max(0, past + i_first - p.window + 1) : 0;
+    const int step0 = lo_all / KT, steps = max(0, (hi_all + KT - 1) / KT - step0);
+    const int per = (steps + p.splits - 1) / p.splits;
+    const int begin = step0 + min(split * per, steps);
+    const int n = max(0, min(per, steps - split * per));
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar->kfull[s], C::FEED_WARPS);
+            mbar_init(&bar->vfull[s], C::FEED_WARPS);
+            mbar_init(&bar->kfree[s], 1);
+            mbar_init(&bar->vfree[s], 1);
+            mbar_init(&bar->sfull[s], 1);
+            mbar_init(&bar->pready[s], 4);
+            mbar_init(&bar->pvdone[s], 1);
+        }
+        mbar_init(&bar->qfull, C::SOFTMAX_WARPS);
+        mbar_init(&bar->done, 1);
+        bar->abort_word = 0u;
+        fence_barrier_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == PR_WARPS - 1) {
+        tmem_alloc(&bar->tmem_slot, 512);
+        tmem_relinquish_alloc_permit();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = bar->tmem_slot;
+
+    if (warp < C::SOFTMAX_WARPS) {
+        // ---------------------------------------------------------------- softmax: one thread per row
+        const int t = warp >> 2;                         // row block
+        const int in_block = threadIdx.x & 127;
+        const int row = rt * ROWS + t * 128 + in_block;  // of the sequence and kv head
+        const bool there = row < all_rows;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 TMEM lanes
+        const int i = row / p.group;
+        const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
+        const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
+        // the query row to f16 in shared memory, by a power of two of its own
+        const int64_t q_row = sq.row0 + (there ? i : 0);
+        const int head = hk * p.group + (there ? row % p.group : 0);
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row * p.ldq + static_cast<int64_t>(head) * D);
+        float top = 0.0f;
+        if (there) {
+#pragma unroll 4
+            for (int w = 0; w < D / 8; ++w) {
+                const uint4 raw = __ldg(src + w);
+                const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v[e] << 16)), fabsf(__uint_as_float(v[e] & 0xffff0000u))));
+            }
+        }
+        int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
+        ex = max(-100, min(100, ex));
+        if (top == 0.0f || top > 3.0e38f) ex = 0;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
+        const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f);
+        uint8_t* q_smem = smem + t * 128 * D * 2;
+#pragma unroll 4
+        for (int w = 0; w < D / 8; ++w) {
+            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+            if (there) raw = __ldg(src + w);
+            const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(v[e] << 16) * down, x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u) * down;
+            *reinterpret_cast<uint4*>(q_smem + (w >> 3) * (128 * 128) + in_block * 128 + (((w & 7) ^ (in_block & 7)) << 4)) =
+                make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->qfull);
+
+        // rows of this block that exist see at least [lo_max, hi_min)
+        const int last_there = min(all_rows, rt * ROWS + t * 128 + 128) - 1;  // may lie before the block's first row
+        const int first_i = (rt * ROWS + t * 128) / p.group, last_i = last_there / p.group;
+        const int hi_min = p.causal ? min(sq.len, past + first_i + 1) : sq.len;
+        const int lo_max = p.window > 0 ? max(0, past + last_i - p.window + 1) : 0;
+        const uint32_t o_tmem = tmem + lanes + t * D;
+        float ref = KV4_NO_REF, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int slot = NQ == 2 ? t : j & 1;
+            const uint32_t slot_parity = (NQ == 2 ? j : j >> 1) & 1;
+            const uint32_t s_tmem = tmem + lanes + C::S_COL + slot * KT;
+            if (!mbar_wait_bounded(&bar->vfull[j & 1], (j >> 1) & 1, abort_word, KV4_WAIT_LIMIT) ||
+                !mbar_wait_bounded(&bar->sfull[slot], slot_parity, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 412);
+                ok = false;
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = true;
+            tc_fence_after_sync();
+            const int key0 = (begin + j) * KT;
+            // keys that hold nothing (no page) and keys whose values are NaN, one bit each
+            uint32_t dead[KT / 32], bad[KT / 32], any = 0u;
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                dead[x] = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
+                bad[x] = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
+                any |= dead[x] | bad[x];
+            }
+            const bool edge = key0 + KT > hi_min || key0 < lo_max || any != 0u;
+            float mx = -INFINITY;
+            uint32_t s[32];
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                tmem_ld_wait();
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int key = key0 + 32 * x + e;
+                        if (key < hi && key >= lo && ((dead[x] >> e) & 1u) == 0u) mx = fmaxf(mx, __uint_as_float(s[e]));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+                }
+            }
+            mx *= factor;
+            if (__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
+                const float to = mx > ref + PR_SLACK ? mx : ref;
+                const float fix = ex2(ref - to);
+                ref = to;
+                l *= fix;
+                if (j > 0) {
+                    if (!mbar_wait_bounded(&bar->pvdone[t], (j - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                        give_up(abort_word, 413);
+                        ok = false;
+                    }
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (int x = 0; x < D / 32; ++x) {
+                        tmem_ld_32x32b_x32(o_tmem + 32 * x, s);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * fix);
+                        tmem_st_32x32b_x32(o_tmem + 32 * x, s);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            const float base = PR_LIFT - ref;
+#pragma unroll
+            for (int x = 0; x < KT / 32; ++x) {
+                tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                tmem_ld_wait();
+                uint32_t pk[16];
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x0 = fmaf(__uint_as_float(s[e]), factor, base), x1 = fmaf(__uint_as_float(s[e + 1]), factor, base);
+                    if (edge) {
+                        const int key = key0 + 32 * x + e;
+                        if ((bad[x] >> e) & 1u) x0 = NAN;
+                        if ((bad[x] >> (e + 1)) & 1u) x1 = NAN;
+                        if (key >= hi || key < lo || ((dead[x] >> e) & 1u)) x0 = -INFINITY;
+                        if (key + 1 >= hi || key + 1 < lo || ((dead[x] >> (e + 1)) & 1u)) x1 = -INFINITY;
+                    }
+                    const float p0 = ex2(x0), p1 = ex2(x1);
+                    sum0 += p0;
+                    sum1 += p1;
+                    pk[e / 2] = pack_half2(p0, p1);
+                }
+                l += sum0 + sum1;
+                tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
+            }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->pready[slot]);
+        }
+        // ---------------------------------------------------------------- output
+        if (n > 0 && ok && *abort_word == 0u) {
+            if (!mbar_wait_bounded(&bar->pvdone[t], (n - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 414);
+                ok = false;
+            }
+            tc_fence_after_sync();
+        }
+        ok = __all_sync(0xffffffffu, ok && *abort_word == 0u);
+        if (ok) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t part = (tile_id * p.splits + split) * ROWS + t * 128 + in_block;
+            __nv_bfloat16* out = p.out + q_row * p.ldo + static_cast<int64_t>(head) * D;
+#pragma unroll 1
+            for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(o_tmem + 32 * x, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (there && p.splits == 1) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
+                            v[y] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        *reinterpret_cast<uint4*>(out + 32 * x + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                } else if (there) {
+                    uint4* to = reinterpret_cast<uint4*>(p.part_o + part * D + 32 * x);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) to[e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+                __syncwarp();
+            }
+            if (there) {
+                const float m = l == 0.0f ? KV4_NO_REF : ref - PR_LIFT;
+                if (p.splits > 1) {
+                    p.part_ml[part] = make_float2(m, l);
+                } else if (p.lse != nullptr) {
+                    p.lse[q_row * p.heads_q + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------------------------------------------------------- keys and values to f16
+        constexpr int TILES = KT / KV4_TILE / C::FEED_WARPS > 0 ? KT / KV4_TILE / C::FEED_WARPS : 1;  // of 16 keys per warp and step
+        const int feeder = warp - C::SOFTMAX_WARPS;
+        const int r = lane >> 2, c = lane & 3;
+        const bool works = feeder * TILES < KT / KV4_TILE;
+        const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
+        const int tiles_per_page = p.cache.page_size / KV4_TILE;
+        const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
+        uint32_t raw_k[TILES][2][2 * G], raw_v[TILES][4 * G];
+        __half2 par_k[TILES][2][G], par_v[TILES][4][G];
+        bool have[TILES];
+        auto load = [&](int j) {
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) {
+                const int tile = (begin + j) * (KT / KV4_TILE) + feeder * TILES + x;
+                have[x] = false;
+                const uint8_t* at = nullptr;
+                if (works && tile * KV4_TILE < hi_all) {
+                    const int page = table[tile / tiles_per_page];
+                    if (page >= 0 && page < p.cache.num_pages) {
+                        have[x] = true;
+                        at = head_base + static_cast<int64_t>(page) * p.cache.page_stride + (tile % tiles_per_page) * TILE;
+                    } else {
+                        atomicCAS(&g_kv4_prompt_device_status, 0, 404);
+                    }
+                }
+                if (have[x]) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {  // keys r and r + 8
+                        if constexpr (W == 2) {
+#pragma unroll
+                            for (int h = 0; h < G / 2; ++h) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(at + h * 1024 + e * 512 + lane * 16);
+                                raw_k[x][e][4 * h] = v.x, raw_k[x][e][4 * h + 1] = v.y, raw_k[x][e][4 * h + 2] = v.z, raw_k[x][e][4 * h + 3] = v.w;
+                            }
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(at + e * 256 + lane * 8);
+                            raw_k[x][e][0] = v.x, raw_k[x][e][1] = v.y;
+                        }
+#pragma unroll
+                        for (int g = 0; g < G; ++g)
+                            par_k[x][e][g] = *reinterpret_cast<const __half2*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g) * 4);
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * D + g * 512 + lane * 16);
+                        raw_v[x][4 * g] = v.x, raw_v[x][4 * g + 1] = v.y, raw_v[x][4 * g + 2] = v.z, raw_v[x][4 * g + 3] = v.w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)  // tokens 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
+                            par_v[x][e][g] = *reinterpret_cast<const __half2*>(at + kv4_pair_offset(D, 1) + ((2 * c + (e & 1) + 8 * (e >> 1)) * G + g) * 4);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int g = 0; g < G; ++g) raw_k[x][e][2 * g] = raw_k[x][e][2 * g + 1] = 0u, par_k[x][e][g] = as_h2(0u);
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) raw_v[x][4 * g + e] = 0u, par_v[x][e][g] = as_h2(0u);
+                }
+            }
+        };
+        if (n > 0) load(0);
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int stage = j & 1;
+            if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 415);
+                ok = false;
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            uint8_t* k_smem = smem + C::K_OFF + stage * C::K_BYTES;
+            if (works) {
+#pragma unroll
+                for (int x = 0; x < TILES; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = (feeder * TILES + x) * KV4_TILE + r + 8 * e;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const __half2 s2 = __low2half2(par_k[x][e][g]), m2 = __high2half2(par_k[x][e][g]);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                uint32_t o[4];
+                                expand(raw_k[x][e][2 * g + u], s2, m2, s2, m2, o);
+                                *reinterpret_cast<uint4*>(k_smem + g * (KT * 128) + key * 128 + (((2 * c + u) ^ (key & 7)) << 4)) =
+                                    make_uint4(o[0], o[1], o[2], o[3]);
+                            }
+                        }
+                    }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->kfull[stage]);
+
+            if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 415);
+                ok = false;
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            uint8_t* v_smem = smem + C::V_OFF + stage * C::K_BYTES;
+            if (works) {
+#pragma unroll
+                for (int x = 0; x < TILES; ++x) {
+                    const int in_step = feeder * TILES + x;
+                    const int key0 = (begin + j) * KT + in_step * KV4_TILE;
+                    // values of keys beyond the sequence and NaN values are zeroed: a zero weight times NaN would reach every row
+                    uint32_t nan_bits = 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
+                        const bool beyond = key0 + tok >= sq.len;
+                        bool nan = false;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float2 sm = __half22float2(par_v[x][e][g]);
+                            nan = nan || isnan(sm.x) || isnan(sm.y);
+                        }
+                        if (beyond || nan) {
+#pragma unroll
+                            for (int g = 0; g < G; ++g) par_v[x][e][g] = as_h2(0u);
+                        }
+                        if (nan && !beyond) nan_bits |= 1u << tok;
+                    }
+                    nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 1);
+                    nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
+                    if (lane == 0) {
+                        flags[stage * 16 + in_step] = have[x] || key0 >= hi_all ? 0u : 0xffffu;
+                        flags[stage * 16 + 8 + in_step] = static_cast<uint16_t>(nan_bits);
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const __half2 s_lo = __lows2half2(par_v[x][0][g], par_v[x][1][g]), m_lo = __highs2half2(par_v[x][0][g], par_v[x][1][g]);
+                        const __half2 s_hi = __lows2half2(par_v[x][2][g], par_v[x][3][g]), m_hi = __highs2half2(par_v[x][2][g], par_v[x][3][g]);
+#pragma unroll
+                        for (int jj = 0; jj < 4; ++jj) {
+                            uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
+                            expand(raw_v[x][4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
+                            const int ch = 64 * g + 16 * jj + r;
+                            const int chunk = 2 * (in_step & 3);
+                            uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + ch * 128 + 4 * c;
+                            *reinterpret_cast<uint32_t*>(row + ((chunk ^ r) << 4)) = o[0];
+                            *reinterpret_cast<uint32_t*>(row + 8 * 128 + ((chunk ^ r) << 4)) = o[1];
+                            *reinterpret_cast<uint32_t*>(row + (((chunk + 1) ^ r) << 4)) = o[2];
+                            *reinterpret_cast<uint32_t*>(row + 8 * 128 + (((chunk + 1) ^ r) << 4)) = o[3];
+                        }
+                    }
+                }
+            }
+            if (j + 1 < n) load(j + 1);  // in flight while the next stage is waited for
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->vfull[stage]);
+        }
+    } else if (lane == 0) {
+        // ---------------------------------------------------------------- MMA issue: one thread
+        constexpr uint32_t IDESC_S = idesc_f16(128, KT), IDESC_O = idesc_f16(128, D);
+        bool ok = true;
+        auto wait = [&](uint64_t* what, uint32_t parity) {
+            if (ok && !mbar_wait_bounded(what, parity, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 416);
+                ok = false;
+            }
+            return ok;
+        };
+        auto scores = [&](int t, int j, int slot) {
+            const uint32_t q = smem_u32(smem) + t * 128 * D * 2, k = smem_u32(smem) + C::K_OFF + (j & 1) * C::K_BYTES;
+#pragma unroll 4
+            for (int ks = 0; ks < D / 16; ++ks)
+                umma_f16_ss(tmem + C::S_COL + slot * KT, umma_desc_kmajor_sw128(q + (ks >> 2) * (128 * 128) + (ks & 3) * 32),
+                            umma_desc_kmajor_sw128(k + (ks >> 2) * (KT * 128) + (ks & 3) * 32), IDESC_S, ks > 0);
+        };
+        auto output = [&](int t, int j, int slot) {
+            const uint32_t v = smem_u32(smem) + C::V_OFF + (j & 1) * C::K_BYTES;
+#pragma unroll 4
+            for (int ks = 0; ks < KT / 16; ++ks)
+                umma_f16_ts(tmem + t * D, tmem + C::S_COL + slot * KT + ks * 8,
+                            umma_desc_kmajor_sw128(v + (ks >> 2) * (D * 128) + (ks & 3) * 32), IDESC_O, j > 0 || ks > 0);
+        };
+        if (n > 0 && wait(&bar->qfull, 0)) {
+            // A score tile may overwrite the P of an earlier step: MMAs of one thread run in the order of their issue.
+            const int ahead = NQ == 2 ? 1 : 2;
+            for (int j = 0; j < ahead && j < n && wait(&bar->kfull[j & 1], 0); ++j) {
+                tc_fence_after_sync();
+                for (int t = 0; t < NQ; ++t) {
+                    const int slot = NQ == 2 ? t : j & 1;
+                    scores(t, j, slot);
+                    umma_commit(&bar->sfull[slot]);
+                }
+                umma_commit(&bar->kfree[j & 1]);
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                const int next = j + ahead;
+                if (!wait(&bar->vfull[j & 1], (j >> 1) & 1)) break;
+                for (int t = 0; t < NQ; ++t) {
+                    const int slot = NQ == 2 ? t : j & 1;
+                    if (!wait(&bar->pready[slot], (NQ == 2 ? j : j >> 1) & 1)) break;
+                    tc_fence_after_sync();
+                    output(t, j, slot);
+                    umma_commit(&bar->pvdone[t]);
+                    if (t == NQ - 1) umma_commit(&bar->vfree[j & 1]);
+                    if (next < n) {
+                        if (t == 0 && !wait(&bar->kfull[next & 1], (next >> 1) & 1)) break;
+                        tc_fence_after_sync();
+                        scores(t, next, slot);
+                        umma_commit(&bar->sfull[slot]);
+                        if (t == NQ - 1) umma_commit(&bar->kfree[next & 1]);
+                    }
+                }
+            }
+            // nothing of this thread's may be in flight when the TMEM is given back
+            umma_commit(&bar->done);
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&bar->done, 0u) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == PR_WARPS - 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int D, int NQ>
+int32_t launch_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stream) {
+    auto kern = kv4_prompt_kernel<D, NQ>;
+    constexpr int bytes = PromptCfg<D, NQ>::TOTAL;
+    static_assert(bytes <= 232448, "shared memory of an SM");
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return BQ_STATUS_LAUNCH_FAILURE;
+    }
+    kern<<<static_cast<unsigned>(s.tiles * s.splits), PR_THREADS, bytes, stream>>>(p);
+    return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
+}
+
+}  // namespace
+
+int32_t launch_kv4_prompt(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
+    switch (p.cache.head_dim) {
+        case 64: return s.tile_rows == 256 ? launch_prompt<64, 2>(p, s, stream) : launch_prompt<64, 1>(p, s, stream);
+        case 128: return s.tile_rows == 256 ? launch_prompt<128, 2>(p, s, stream) : launch_prompt<128, 1>(p, s, stream);
+        case 256: return launch_prompt<256, 1>(p, s, stream);
+        default: return BQ_STATUS_UNSUPPORTED;
+    }
+}
+
+int32_t read_and_clear_kv4_prompt_device_status() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kv4_prompt_device_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) {
+        int zero = 0;
+        (void)cudaMemcpyToSymbol(g_kv4_prompt_device_status, &zero, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace bq

@@ -530,8 +530,9 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
  * baracuda_kernels_kv4_page_bytes; larger where pages of several layers are interleaved).  A page holds `page_size` tokens (a
  * multiple of 16) of every kv head, as [heads_kv][page_size / 16] tiles of 18 * head_dim bytes; head_dim is 64, 128 or 256.
  * Each group of 64 channels of a token and head is 64 codes c in 0..15, an f16 scale s and an f16 minimum m; the value is
- * s * c + m.  s = f16((max - min) / 15), m = f16(min), both cut to +-65504, c = clamp(rint_even((x - m) / s), 0, 15) (0 where
- * s is 0); a minimum of zero is +0.  A NaN among the 64 makes all of them NaN; infinities are cut.  Within a tile, t = token (0..15), d = channel:
+ * s * c + m.  With max and min of the 64 cut to +-32768 (so that every value is a finite f16 number), s = f16((max - min) / 15),
+ * m = f16(min), c = clamp(rint_even((x - m) / s), 0, 15) (0 where
+ * s is 0); a minimum of zero is +0.  A NaN among the 64 makes all of them NaN.  Within a tile, t = token (0..15), d = channel:
  *   keys    8 * D bytes: with d = 64 g + 16 c + 8 u + 2 b + n, W = min(2, D / 64), h = g / W: nibble n (0 = low) of byte
  *           (((h * 16 + t) * 4 + c) * W + g % W) * 8 + 4 u + b
  *   values  8 * D bytes: with d = 64 h + 16 j + 8 n + r, t = 8 e + 2 c + o: nibble n of byte

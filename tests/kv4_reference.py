@@ -41,9 +41,9 @@ def unpack(cache, page, heads, dim):
 def quantize(x):
     """x [..., dim] bf16 -> (codes, s, m) float64, s and m rounded to f16 from f32 as the format says."""
     x = x.float().unflatten(-1, (-1, 64))
-    low, high = x.amin(-1), x.amax(-1)
-    s = ((high - low) / 15.0).clamp(max=65504.0).half().double()
-    m = low.clamp(-65504.0, 65504.0).half().double() + 0.0  # a zero minimum is +0
+    low, high = x.amin(-1).clamp(-32768.0, 32768.0), x.amax(-1).clamp(-32768.0, 32768.0)
+    s = ((high - low) / 15.0).half().double()
+    m = low.half().double() + 0.0  # a zero minimum is +0
     codes = torch.round((x.double() - m.unsqueeze(-1)) / s.unsqueeze(-1)).clamp(0, 15)
     codes = torch.where((s > 0).unsqueeze(-1), codes, torch.zeros_like(codes))
     return codes.flatten(-2), s, m
