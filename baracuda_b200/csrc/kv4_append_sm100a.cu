@@ -34,33 +34,6 @@ struct NormRopeParams {
     uint64_t axis[2][3];             // axis of each rotation pair: bit b of pair i at bit i % 64 of axis[i / 64][b]
 };
 
-// Two f32 numbers in one register pair; each operation rounds each of them once.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 both(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 each(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 // The sum of two rounded products: scalar additions, since the assembler joins a packed product and a packed sum into one
 // operation with one rounding.
 __device__ __forceinline__ f32x2 add_products(f32x2 a, f32x2 b) {

@@ -43,6 +43,33 @@ __device__ __forceinline__ int kv4_value_byte(int t, int d) {
     return 8 * D + (d >> 6) * 512 + ((d & 7) * 4 + ((t & 7) >> 1)) * 16 + ((d & 63) >> 4) * 4 + (t & 1) * 2 + (t >> 3);
 }
 
+// Two f32 numbers in one register pair; each operation rounds each of them once.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 both(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 each(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 struct Kv4Cache {
     uint8_t* base;
     int64_t page_stride;  // bytes, a multiple of 16

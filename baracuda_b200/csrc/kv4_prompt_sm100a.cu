@@ -15,7 +15,7 @@
 //
 // Two row blocks (256 rows, D <= 128): while one block's softmax runs, the tensor core works on the other.  One row block
 // (128 rows; D = 256, or few rows): S is double-buffered instead, the next step's S is computed under this step's softmax.
-// Warps: 4 softmax warps per row block, the other 8 or 4 of twelve bring keys and values to f16, one issues the MMAs.
+// Warps: 4 softmax warps per row block, 4 bring keys and 4 bring values to f16, one issues the MMAs.
 // Every mbarrier wait is bounded (status 412..416).
 
 #include <cuda_bf16.h>
@@ -33,14 +33,15 @@ __device__ int g_kv4_prompt_device_status = 0;
 
 constexpr float PR_SLACK = 7.0f;  // p <= 2^(SLACK + LIFT) stays within f16
 constexpr float PR_LIFT = 8.0f;   // f16's range below the reference: 2^-22 in full precision
-constexpr int PR_WARPS = 13;
-constexpr int PR_THREADS = PR_WARPS * 32;
 
 template <int D, int NQ>
 struct PromptCfg {
     static constexpr int KT = D == 256 ? 64 : 128;  // keys of a step
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    static constexpr int FEED_WARPS = 12 - SOFTMAX_WARPS;
+    static constexpr int FEED_WARPS = 4;                         // for keys, and as many for values
+    static constexpr int TILES = KT / KV4_TILE / FEED_WARPS;     // of 16 keys, of a feeding warp in a step
+    static constexpr int MMA_WARP = SOFTMAX_WARPS + 2 * FEED_WARPS;
+    static constexpr int THREADS = (MMA_WARP + 1) * 32;
     static constexpr int Q_BYTES = NQ * 128 * D * 2;
     static constexpr int K_BYTES = KT * D * 2;  // V the same
     static constexpr int K_OFF = Q_BYTES;
@@ -120,8 +121,15 @@ __device__ __forceinline__ void expand(uint32_t w, __half2 s_lo, __half2 m_lo, _
     out[3] = h2(__hfma2(c3, s_hi, m_hi));
 }
 
+// Bits of the 32 keys from `key` on that lie in [lo, hi).
+__device__ __forceinline__ uint32_t seen_keys(int key, int lo, int hi) {
+    const int from = max(lo - key, 0), to = min(hi - key, 32);
+    if (to <= 0 || from >= 32) return 0u;
+    return (to == 32 ? 0xffffffffu : (1u << to) - 1u) & (0xffffffffu << from);
+}
+
 template <int D, int NQ>
-__global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kernel(const __grid_constant__ AttnParams p) {
     using C = PromptCfg<D, NQ>;
     constexpr int KT = C::KT;
     constexpr int G = D / KV4_GROUP;
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_
         fence_barrier_init();
         fence_proxy_async_smem();
     }
-    if (warp == PR_WARPS - 1) {
+    if (warp == C::MMA_WARP) {
         tmem_alloc(&bar->tmem_slot, 512);
         tmem_relinquish_alloc_permit();
     }
@@ -249,29 +257,31 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_
             tc_fence_after_sync();
             const int key0 = (begin + j) * KT;
             // keys that hold nothing (no page) and keys whose values are NaN, one bit each
-            uint32_t dead[KT / 32], bad[KT / 32], any = 0u;
+            uint32_t any = 0u;
 #pragma unroll
-            for (int x = 0; x < KT / 32; ++x) {
-                dead[x] = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
-                bad[x] = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
-                any |= dead[x] | bad[x];
-            }
+            for (int x = 0; x < KT / 32; ++x)
+                any |= reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x] | reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
             const bool edge = key0 + KT > hi_min || key0 < lo_max || any != 0u;
             float mx = -INFINITY;
             uint32_t s[32];
+            if (edge) {
+#pragma unroll 1
+                for (int x = 0; x < KT / 32; ++x) {
+                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                    tmem_ld_wait();
+                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
 #pragma unroll
-            for (int x = 0; x < KT / 32; ++x) {
-                tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
-                tmem_ld_wait();
-                if (edge) {
+                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, ((seen >> e) & 1u) ? __uint_as_float(s[e]) : -INFINITY);
+                }
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int key = key0 + 32 * x + e;
-                        if (key < hi && key >= lo && ((dead[x] >> e) & 1u) == 0u) mx = fmaxf(mx, __uint_as_float(s[e]));
-                    }
-                } else {
+                for (int x = 0; x < KT / 32; ++x) {
+                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                    tmem_ld_wait();
+                    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+                    for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
             }
             mx *= factor;
@@ -299,30 +309,45 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_
                 }
             }
             const float base = PR_LIFT - ref;
+            const f32x2 factor2 = both(factor, factor), base2 = both(base, base);
+            f32x2 sum[2] = {0ull, 0ull};
+            if (edge) {
+#pragma unroll 1
+                for (int x = 0; x < KT / 32; ++x) {
+                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                    tmem_ld_wait();
+                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
+                    const uint32_t bad = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
+                    uint32_t pk[16];
 #pragma unroll
-            for (int x = 0; x < KT / 32; ++x) {
-                tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
-                tmem_ld_wait();
-                uint32_t pk[16];
-                float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x0 = fmaf(__uint_as_float(s[e]), factor, base), x1 = fmaf(__uint_as_float(s[e + 1]), factor, base);
-                    if (edge) {
-                        const int key = key0 + 32 * x + e;
-                        if ((bad[x] >> e) & 1u) x0 = NAN;
-                        if ((bad[x] >> (e + 1)) & 1u) x1 = NAN;
-                        if (key >= hi || key < lo || ((dead[x] >> e) & 1u)) x0 = -INFINITY;
-                        if (key + 1 >= hi || key + 1 < lo || ((dead[x] >> (e + 1)) & 1u)) x1 = -INFINITY;
+                    for (int e = 0; e < 32; e += 2) {
+                        float2 v = each(fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), factor2, base2));
+                        v.x = ((seen >> e) & 1u) == 0u ? -INFINITY : ((bad >> e) & 1u) ? NAN : v.x;
+                        v.y = ((seen >> (e + 1)) & 1u) == 0u ? -INFINITY : ((bad >> (e + 1)) & 1u) ? NAN : v.y;
+                        const float p0 = ex2(v.x), p1 = ex2(v.y);
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(p0, p1));
+                        pk[e / 2] = pack_half2(p0, p1);
                     }
-                    const float p0 = ex2(x0), p1 = ex2(x1);
-                    sum0 += p0;
-                    sum1 += p1;
-                    pk[e / 2] = pack_half2(p0, p1);
+                    tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
                 }
-                l += sum0 + sum1;
-                tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
+            } else {
+#pragma unroll
+                for (int x = 0; x < KT / 32; ++x) {
+                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                    tmem_ld_wait();
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 v = each(fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), factor2, base2));
+                        const float p0 = ex2(v.x), p1 = ex2(v.y);
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(p0, p1));
+                        pk[e / 2] = pack_half2(p0, p1);
+                    }
+                    tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
+                }
             }
+            const float2 total = each(add2(sum[0], sum[1]));
+            l += total.x + total.y;
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -378,161 +403,170 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_
                 }
             }
         }
-    } else if (warp < 12) {
-        // ---------------------------------------------------------------- keys and values to f16
-        constexpr int TILES = KT / KV4_TILE / C::FEED_WARPS > 0 ? KT / KV4_TILE / C::FEED_WARPS : 1;  // of 16 keys per warp and step
-        const int feeder = warp - C::SOFTMAX_WARPS;
+    } else if (warp < C::MMA_WARP) {
+        // ---------------------------------------------------------------- keys, or values, to f16
+        constexpr int TILES = C::TILES, STEP_TILES = KT / KV4_TILE;
+        const bool values = warp >= C::SOFTMAX_WARPS + C::FEED_WARPS;
+        const int feeder = (warp - C::SOFTMAX_WARPS) % C::FEED_WARPS;
         const int r = lane >> 2, c = lane & 3;
-        const bool works = feeder * TILES < KT / KV4_TILE;
         const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
         const int tiles_per_page = p.cache.page_size / KV4_TILE;
-        const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
-        uint32_t raw_k[TILES][2][2 * G], raw_v[TILES][4 * G];
-        __half2 par_k[TILES][2][G], par_v[TILES][4][G];
-        bool have[TILES];
-        auto load = [&](int j) {
+        const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE + (values ? 8 * D : 0);
+        // lane i looks up the i-th of the next 32 tiles of this warp: the page, and the tile's place in it
+        int64_t ahead = -1;
+        auto look_up = [&](int j) {
+            const int tile = (begin + j + lane / TILES) * STEP_TILES + feeder * TILES + lane % TILES;
+            ahead = -1;
+            if (j + lane / TILES < n && tile * KV4_TILE < hi_all) {
+                const int at = tile / tiles_per_page, page = table[at];
+                if (page >= 0 && page < p.cache.num_pages) {
+                    ahead = static_cast<int64_t>(page) * p.cache.page_stride + (tile - at * tiles_per_page) * TILE;
+                } else {
+                    atomicCAS(&g_kv4_prompt_device_status, 0, 404);
+                }
+            }
+        };
+        // a step's codes and (s, m) pairs of this lane: of the keys r and r + 8, or of the tokens 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
+        struct Raw {
+            uint32_t word[TILES][4 * G];
+            uint32_t pair[TILES][4 * G];  // keys use half of them
+            bool have[TILES];
+        };
+        auto load = [&](Raw& raw, int j) {
+            if (j % (32 / TILES) == 0) look_up(j);
 #pragma unroll
             for (int x = 0; x < TILES; ++x) {
-                const int tile = (begin + j) * (KT / KV4_TILE) + feeder * TILES + x;
-                have[x] = false;
-                const uint8_t* at = nullptr;
-                if (works && tile * KV4_TILE < hi_all) {
-                    const int page = table[tile / tiles_per_page];
-                    if (page >= 0 && page < p.cache.num_pages) {
-                        have[x] = true;
-                        at = head_base + static_cast<int64_t>(page) * p.cache.page_stride + (tile % tiles_per_page) * TILE;
-                    } else {
-                        atomicCAS(&g_kv4_prompt_device_status, 0, 404);
+                const int64_t where = __shfl_sync(0xffffffffu, ahead, (j % (32 / TILES)) * TILES + x);
+                raw.have[x] = where >= 0;
+#pragma unroll
+                for (int e = 0; e < 4 * G; ++e) raw.word[x][e] = raw.pair[x][e] = 0u;
+                if (where < 0) continue;
+                const uint8_t* at = head_base + where;
+                if (W == 2 || values) {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {  // values: group g; keys: key r or r + 8 (odd g) of the groups g, g + 1 / g - 1, g
+                        const uint4 v = *reinterpret_cast<const uint4*>(at + g * 512 + lane * 16);
+                        raw.word[x][4 * g] = v.x, raw.word[x][4 * g + 1] = v.y, raw.word[x][4 * g + 2] = v.z, raw.word[x][4 * g + 3] = v.w;
                     }
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + lane * 8), w = *reinterpret_cast<const uint2*>(at + 256 + lane * 8);
+                    raw.word[x][0] = v.x, raw.word[x][1] = v.y, raw.word[x][2] = w.x, raw.word[x][3] = w.y;
                 }
-                if (have[x]) {
+                // from here the pairs: keys [16][G] at 16 D of the tile, values behind them
+                const uint32_t* pairs = reinterpret_cast<const uint32_t*>(at + (values ? 9 * D : 16 * D));
+                if (values) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {  // keys r and r + 8
-                        if constexpr (W == 2) {
+                    for (int e = 0; e < 2; ++e)
 #pragma unroll
-                            for (int h = 0; h < G / 2; ++h) {
-                                const uint4 v = *reinterpret_cast<const uint4*>(at + h * 1024 + e * 512 + lane * 16);
-                                raw_k[x][e][4 * h] = v.x, raw_k[x][e][4 * h + 1] = v.y, raw_k[x][e][4 * h + 2] = v.z, raw_k[x][e][4 * h + 3] = v.w;
-                            }
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(at + e * 256 + lane * 8);
-                            raw_k[x][e][0] = v.x, raw_k[x][e][1] = v.y;
+                        for (int y = 0; y < G; ++y) {  // two tokens in a row, 2 G words
+                            const uint2 v = *reinterpret_cast<const uint2*>(pairs + (2 * c + 8 * e) * G + 2 * y);
+                            raw.pair[x][2 * G * e + 2 * y] = v.x, raw.pair[x][2 * G * e + 2 * y + 1] = v.y;
                         }
-#pragma unroll
-                        for (int g = 0; g < G; ++g)
-                            par_k[x][e][g] = *reinterpret_cast<const __half2*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g) * 4);
-                    }
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * D + g * 512 + lane * 16);
-                        raw_v[x][4 * g] = v.x, raw_v[x][4 * g + 1] = v.y, raw_v[x][4 * g + 2] = v.z, raw_v[x][4 * g + 3] = v.w;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)  // tokens 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
-                            par_v[x][e][g] = *reinterpret_cast<const __half2*>(at + kv4_pair_offset(D, 1) + ((2 * c + (e & 1) + 8 * (e >> 1)) * G + g) * 4);
-                    }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int g = 0; g < G; ++g) raw_k[x][e][2 * g] = raw_k[x][e][2 * g + 1] = 0u, par_k[x][e][g] = as_h2(0u);
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) raw_v[x][4 * g + e] = 0u, par_v[x][e][g] = as_h2(0u);
+                        for (int g = 0; g < G; ++g) raw.pair[x][G * e + g] = pairs[(r + 8 * e) * G + g];
                 }
             }
         };
-        if (n > 0) load(0);
-        bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            const int stage = j & 1;
-            if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
-                give_up(abort_word, 415);
-                ok = false;
-            }
-            if (!__all_sync(0xffffffffu, ok)) break;
-            uint8_t* k_smem = smem + C::K_OFF + stage * C::K_BYTES;
-            if (works) {
+        auto convert_keys = [&](const Raw& raw, uint8_t* k_smem) {
 #pragma unroll
-                for (int x = 0; x < TILES; ++x)
+            for (int x = 0; x < TILES; ++x)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = (feeder * TILES + x) * KV4_TILE + r + 8 * e;
+                for (int e = 0; e < 2; ++e) {
+                    const int key = (feeder * TILES + x) * KV4_TILE + r + 8 * e;
+                    uint8_t* row = k_smem + key * 128;
 #pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            const __half2 s2 = __low2half2(par_k[x][e][g]), m2 = __high2half2(par_k[x][e][g]);
+                    for (int g = 0; g < G; ++g) {
+                        const __half2 sm = as_h2(raw.pair[x][G * e + g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
 #pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                uint32_t o[4];
-                                expand(raw_k[x][e][2 * g + u], s2, m2, s2, m2, o);
-                                *reinterpret_cast<uint4*>(k_smem + g * (KT * 128) + key * 128 + (((2 * c + u) ^ (key & 7)) << 4)) =
-                                    make_uint4(o[0], o[1], o[2], o[3]);
-                            }
+                        for (int u = 0; u < 2; ++u) {
+                            // 16-byte chunk h of 512 * e holds groups W h .. W h + W - 1
+                            const uint32_t word = W == 2 ? raw.word[x][(g / 2 * 2 + e) * 4 + (g & 1) * 2 + u] : raw.word[x][2 * e + u];
+                            uint32_t o[4];
+                            expand(word, s2, m2, s2, m2, o);
+                            *reinterpret_cast<uint4*>(row + g * (KT * 128) + (((2 * c + u) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
                     }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar->kfull[stage]);
-
-            if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
-                give_up(abort_word, 415);
-                ok = false;
-            }
-            if (!__all_sync(0xffffffffu, ok)) break;
-            uint8_t* v_smem = smem + C::V_OFF + stage * C::K_BYTES;
-            if (works) {
+                }
+        };
+        auto convert_values = [&](Raw& raw, uint8_t* v_smem, int j, int stage) {
 #pragma unroll
-                for (int x = 0; x < TILES; ++x) {
-                    const int in_step = feeder * TILES + x;
-                    const int key0 = (begin + j) * KT + in_step * KV4_TILE;
-                    // values of keys beyond the sequence and NaN values are zeroed: a zero weight times NaN would reach every row
-                    uint32_t nan_bits = 0u;
+            for (int x = 0; x < TILES; ++x) {
+                const int in_step = feeder * TILES + x, key0 = (begin + j) * KT + in_step * KV4_TILE;
+                // values of keys beyond the sequence and NaN values are zeroed: a zero weight times NaN would reach every row
+                uint32_t top = 0u;
+#pragma unroll
+                for (int e = 0; e < 4 * G; ++e) top |= (raw.pair[x][e] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
+                uint32_t nan_bits = 0u;
+                if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len)) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
-                        const bool beyond = key0 + tok >= sq.len;
-                        bool nan = false;
+                        uint32_t ones = 0u;
 #pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            const float2 sm = __half22float2(par_v[x][e][g]);
-                            nan = nan || isnan(sm.x) || isnan(sm.y);
-                        }
+                        for (int g = 0; g < G; ++g) ones |= (raw.pair[x][G * e + g] & 0x7c007c00u) + 0x04000400u;
+                        const bool beyond = key0 + tok >= sq.len, nan = (ones & 0x80008000u) != 0u;
                         if (beyond || nan) {
 #pragma unroll
-                            for (int g = 0; g < G; ++g) par_v[x][e][g] = as_h2(0u);
+                            for (int g = 0; g < G; ++g) raw.pair[x][G * e + g] = 0u;
                         }
                         if (nan && !beyond) nan_bits |= 1u << tok;
                     }
                     nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 1);
                     nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
-                    if (lane == 0) {
-                        flags[stage * 16 + in_step] = have[x] || key0 >= hi_all ? 0u : 0xffffu;
-                        flags[stage * 16 + 8 + in_step] = static_cast<uint16_t>(nan_bits);
-                    }
+                }
+                if (lane == 0) {
+                    flags[stage * 16 + in_step] = raw.have[x] || key0 >= hi_all ? 0u : 0xffffu;
+                    flags[stage * 16 + 8 + in_step] = static_cast<uint16_t>(nan_bits);
+                }
+                uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + r * 128 + 4 * c;
+                const int at0 = ((2 * (in_step & 3)) ^ r) << 4, at1 = ((2 * (in_step & 3) + 1) ^ r) << 4;
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const __half2 s_lo = __lows2half2(par_v[x][0][g], par_v[x][1][g]), m_lo = __highs2half2(par_v[x][0][g], par_v[x][1][g]);
-                        const __half2 s_hi = __lows2half2(par_v[x][2][g], par_v[x][3][g]), m_hi = __highs2half2(par_v[x][2][g], par_v[x][3][g]);
+                for (int g = 0; g < G; ++g) {
+                    const __half2 t0 = as_h2(raw.pair[x][g]), t1 = as_h2(raw.pair[x][G + g]), t2 = as_h2(raw.pair[x][2 * G + g]), t3 = as_h2(raw.pair[x][3 * G + g]);
+                    const __half2 s_lo = __lows2half2(t0, t1), m_lo = __highs2half2(t0, t1), s_hi = __lows2half2(t2, t3), m_hi = __highs2half2(t2, t3);
 #pragma unroll
-                        for (int jj = 0; jj < 4; ++jj) {
-                            uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
-                            expand(raw_v[x][4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
-                            const int ch = 64 * g + 16 * jj + r;
-                            const int chunk = 2 * (in_step & 3);
-                            uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + ch * 128 + 4 * c;
-                            *reinterpret_cast<uint32_t*>(row + ((chunk ^ r) << 4)) = o[0];
-                            *reinterpret_cast<uint32_t*>(row + 8 * 128 + ((chunk ^ r) << 4)) = o[1];
-                            *reinterpret_cast<uint32_t*>(row + (((chunk + 1) ^ r) << 4)) = o[2];
-                            *reinterpret_cast<uint32_t*>(row + 8 * 128 + (((chunk + 1) ^ r) << 4)) = o[3];
-                        }
+                    for (int jj = 0; jj < 4; ++jj) {
+                        uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
+                        expand(raw.word[x][4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
+                        uint8_t* to = row + (64 * g + 16 * jj) * 128;
+                        *reinterpret_cast<uint32_t*>(to + at0) = o[0];
+                        *reinterpret_cast<uint32_t*>(to + 8 * 128 + at0) = o[1];
+                        *reinterpret_cast<uint32_t*>(to + at1) = o[2];
+                        *reinterpret_cast<uint32_t*>(to + 8 * 128 + at1) = o[3];
                     }
                 }
             }
-            if (j + 1 < n) load(j + 1);  // in flight while the next stage is waited for
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar->vfull[stage]);
+        };
+        uint64_t* full = values ? bar->vfull : bar->kfull;
+        uint64_t* free = values ? bar->vfree : bar->kfree;
+        uint8_t* operand = smem + (values ? C::V_OFF : C::K_OFF);
+        Raw raw[2];
+        if (n > 0) load(raw[0], 0);
+        bool ok = true;
+        for (int j0 = 0; ok && j0 < n; j0 += 2) {
+#pragma unroll
+            for (int stage = 0; stage < 2; ++stage) {  // step j0 + stage, from raw[stage]
+                const int j = j0 + stage;
+                if (j >= n) break;
+                if (j + 1 < n) load(raw[stage ^ 1], j + 1);  // in flight under this step's work
+                if (j >= 2 && !mbar_wait_bounded(&free[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                    give_up(abort_word, 415);
+                    ok = false;
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (values) {
+                    convert_values(raw[stage], operand + stage * C::K_BYTES, j, stage);
+                } else {
+                    convert_keys(raw[stage], operand + stage * C::K_BYTES);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[stage]);
+            }
         }
     } else if (lane == 0) {
         // ---------------------------------------------------------------- MMA issue: one thread
@@ -600,7 +634,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv4_prompt_kernel(const __grid_
     __syncwarp();
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == PR_WARPS - 1) {
+    if (warp == C::MMA_WARP) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
@@ -615,7 +649,7 @@ int32_t launch_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stre
         (void)cudaGetLastError();
         return BQ_STATUS_LAUNCH_FAILURE;
     }
-    kern<<<static_cast<unsigned>(s.tiles * s.splits), PR_THREADS, bytes, stream>>>(p);
+    kern<<<static_cast<unsigned>(s.tiles * s.splits), PromptCfg<D, NQ>::THREADS, bytes, stream>>>(p);
     return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
 }
 
