@@ -568,64 +568,77 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 if (lane == 0) mbar_arrive(&full[stage]);
             }
         }
-    } else if (lane == 0) {
-        // ---------------------------------------------------------------- MMA issue: one thread
+    } else {
+        // ---------------------------------------------------------------- MMA issue: the warp walks the steps, one lane issues
         constexpr uint32_t IDESC_S = idesc_f16(128, KT), IDESC_O = idesc_f16(128, D);
+        const bool leader = elect_one() != 0u;
+        const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(smem));
+        const uint64_t k_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::K_OFF), v_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::V_OFF);
         bool ok = true;
         auto wait = [&](uint64_t* what, uint32_t parity) {
             if (ok && !mbar_wait_bounded(what, parity, abort_word, KV4_WAIT_LIMIT)) {
                 give_up(abort_word, 416);
                 ok = false;
             }
+            ok = __all_sync(0xffffffffu, ok);
             return ok;
         };
+        // descriptors count addresses in 16 bytes: a 16-deep slice is 32 bytes on within a 128-byte block of 64
         auto scores = [&](int t, int j, int slot) {
-            const uint32_t q = smem_u32(smem) + t * 128 * D * 2, k = smem_u32(smem) + C::K_OFF + (j & 1) * C::K_BYTES;
-#pragma unroll 4
-            for (int ks = 0; ks < D / 16; ++ks)
-                umma_f16_ss(tmem + C::S_COL + slot * KT, umma_desc_kmajor_sw128(q + (ks >> 2) * (128 * 128) + (ks & 3) * 32),
-                            umma_desc_kmajor_sw128(k + (ks >> 2) * (KT * 128) + (ks & 3) * 32), IDESC_S, ks > 0);
+            const uint64_t q = q_desc + t * (128 * D * 2 / 16), k = k_desc + (j & 1) * (C::K_BYTES / 16);
+            const uint32_t to = tmem + C::S_COL + slot * KT;
+            if (leader) {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    umma_f16_ss(to, q + ((ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2), k + ((ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2), IDESC_S, ks > 0);
+                umma_commit(&bar->sfull[slot]);
+            }
+            __syncwarp();
         };
         auto output = [&](int t, int j, int slot) {
-            const uint32_t v = smem_u32(smem) + C::V_OFF + (j & 1) * C::K_BYTES;
-#pragma unroll 4
-            for (int ks = 0; ks < KT / 16; ++ks)
-                umma_f16_ts(tmem + t * D, tmem + C::S_COL + slot * KT + ks * 8,
-                            umma_desc_kmajor_sw128(v + (ks >> 2) * (D * 128) + (ks & 3) * 32), IDESC_O, j > 0 || ks > 0);
+            const uint64_t v = v_desc + (j & 1) * (C::K_BYTES / 16);
+            const uint32_t to = tmem + t * D, from = tmem + C::S_COL + slot * KT;
+            const uint32_t more = j > 0;
+            if (leader) {
+#pragma unroll
+                for (int ks = 0; ks < KT / 16; ++ks)
+                    umma_f16_ts(to, from + ks * 8, v + ((ks >> 2) * (D * 128 / 16) + (ks & 3) * 2), IDESC_O, ks > 0 ? 1u : more);
+                umma_commit(&bar->pvdone[t]);
+                if (t == NQ - 1) umma_commit(&bar->vfree[j & 1]);
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint64_t* what) {
+            if (leader) umma_commit(what);
+            __syncwarp();
         };
         if (n > 0 && wait(&bar->qfull, 0)) {
             // A score tile may overwrite the P of an earlier step: MMAs of one thread run in the order of their issue.
-            const int ahead = NQ == 2 ? 1 : 2;
+            constexpr int ahead = NQ == 2 ? 1 : 2;
             for (int j = 0; j < ahead && j < n && wait(&bar->kfull[j & 1], 0); ++j) {
                 tc_fence_after_sync();
-                for (int t = 0; t < NQ; ++t) {
-                    const int slot = NQ == 2 ? t : j & 1;
-                    scores(t, j, slot);
-                    umma_commit(&bar->sfull[slot]);
-                }
-                umma_commit(&bar->kfree[j & 1]);
+                for (int t = 0; t < NQ; ++t) scores(t, j, NQ == 2 ? t : j & 1);
+                commit(&bar->kfree[j & 1]);
             }
             for (int j = 0; ok && j < n; ++j) {
                 const int next = j + ahead;
                 if (!wait(&bar->vfull[j & 1], (j >> 1) & 1)) break;
+#pragma unroll
                 for (int t = 0; t < NQ; ++t) {
                     const int slot = NQ == 2 ? t : j & 1;
                     if (!wait(&bar->pready[slot], (NQ == 2 ? j : j >> 1) & 1)) break;
                     tc_fence_after_sync();
                     output(t, j, slot);
-                    umma_commit(&bar->pvdone[t]);
-                    if (t == NQ - 1) umma_commit(&bar->vfree[j & 1]);
                     if (next < n) {
                         if (t == 0 && !wait(&bar->kfull[next & 1], (next >> 1) & 1)) break;
                         tc_fence_after_sync();
                         scores(t, next, slot);
-                        umma_commit(&bar->sfull[slot]);
-                        if (t == NQ - 1) umma_commit(&bar->kfree[next & 1]);
+                        if (t == NQ - 1) commit(&bar->kfree[next & 1]);
                     }
                 }
             }
             // nothing of this thread's may be in flight when the TMEM is given back
-            umma_commit(&bar->done);
+            commit(&bar->done);
             const long long t0 = clock64();
             while (!mbar_try_wait(&bar->done, 0u) && clock64() - t0 < KV4_WAIT_LIMIT) {
             }
