@@ -38,9 +38,9 @@ template <int D, int NQ>
 struct PromptCfg {
     static constexpr int KT = D == 256 ? 64 : 128;  // keys of a step
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    static constexpr int FEED_WARPS = 4;                         // for keys, and as many for values
-    static constexpr int TILES = KT / KV4_TILE / FEED_WARPS;     // of 16 keys, of a feeding warp in a step
-    static constexpr int MMA_WARP = SOFTMAX_WARPS + 2 * FEED_WARPS;
+    static constexpr int FEED_WARPS = 8;
+    static constexpr int SHARES = FEED_WARPS / (KT / KV4_TILE);  // of a tile of 16 keys: whole tiles, or halves of its channels
+    static constexpr int MMA_WARP = SOFTMAX_WARPS + FEED_WARPS;
     static constexpr int THREADS = (MMA_WARP + 1) * 32;
     static constexpr int Q_BYTES = NQ * 128 * D * 2;
     static constexpr int K_BYTES = KT * D * 2;  // V the same
@@ -77,6 +77,19 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -140,15 +153,17 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     uint8_t* smem = pr_smem_raw + ((1024u - (smem_u32(pr_smem_raw) & 1023u)) & 1023u);
     PromptBars* bar = reinterpret_cast<PromptBars*>(smem + C::BAR_OFF);
     volatile uint32_t* abort_word = &bar->abort_word;
-    uint16_t* flags = reinterpret_cast<uint16_t*>(smem + C::FLAG_OFF);  // [stage][0 dead, 1 nan][tile of 16 keys]
+    constexpr int FLAGS = 16;
+    uint16_t* flags = reinterpret_cast<uint16_t*>(smem + C::FLAG_OFF);  // [stage][dead, nan][feeding warp], a bit per key
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // blocks of late rows see the most keys: they go first
     int id = blockIdx.x;
     const int split = id % p.splits;
     id /= p.splits;
-    const int rt = p.row_tiles - 1 - id % p.row_tiles;
-    id /= p.row_tiles;
+    const int pairs = p.batch * p.cache.heads_kv;
+    const int rt = p.row_tiles - 1 - id / pairs;
+    id %= pairs;
     const int hk = id % p.cache.heads_kv, b = id / p.cache.heads_kv;
     const int64_t tile_id = (static_cast<int64_t>(b) * p.cache.heads_kv + hk) * p.row_tiles + rt;
     const Sequence sq = sequence_of(p, b, &g_kv4_prompt_device_status);
@@ -257,10 +272,15 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             tc_fence_after_sync();
             const int key0 = (begin + j) * KT;
             // keys that hold nothing (no page) and keys whose values are NaN, one bit each
+            const uint32_t* gone = reinterpret_cast<const uint32_t*>(flags + (j & 1) * FLAGS);
+            const uint32_t* nans = gone + FLAGS / 4;
             uint32_t any = 0u;
 #pragma unroll
-            for (int x = 0; x < KT / 32; ++x)
-                any |= reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x] | reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
+            for (int x = 0; x < C::FEED_WARPS / 2; ++x) any |= gone[x] | nans[x];
+            auto bits_of = [](const uint32_t* w, int x) {  // of keys 32 x .. 32 x + 31
+                if constexpr (C::SHARES == 1) return w[x];
+                return ((w[2 * x] | (w[2 * x] >> 16)) & 0xffffu) | ((w[2 * x + 1] | (w[2 * x + 1] << 16)) & 0xffff0000u);
+            };
             const bool edge = key0 + KT > hi_min || key0 < lo_max || any != 0u;
             float mx = -INFINITY;
             uint32_t s[32];
@@ -269,20 +289,23 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 for (int x = 0; x < KT / 32; ++x) {
                     tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
                     tmem_ld_wait();
-                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
+                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~bits_of(gone, x);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) mx = fmaxf(mx, ((seen >> e) & 1u) ? __uint_as_float(s[e]) : -INFINITY);
                 }
-            } else {
+            } else {  // 16 columns are on their way while the 16 before are looked at
+                uint32_t v[2][16];
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_ld_32x32b_x16(s_tmem, v[0]);
 #pragma unroll
-                for (int x = 0; x < KT / 32; ++x) {
-                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                for (int x = 0; x < KT / 16; ++x) {
                     tmem_ld_wait();
-                    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+                    if (x + 1 < KT / 16) tmem_ld_32x32b_x16(s_tmem + 16 * (x + 1), v[(x + 1) & 1]);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
-                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    for (int e = 0; e < 16; e += 2)
+                        m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(v[x & 1][e])), __uint_as_float(v[x & 1][e + 1]));
                 }
+                mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             }
             mx *= factor;
             if (__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
@@ -316,8 +339,8 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 for (int x = 0; x < KT / 32; ++x) {
                     tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
                     tmem_ld_wait();
-                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16)[x];
-                    const uint32_t bad = reinterpret_cast<const uint32_t*>(flags + (j & 1) * 16 + 8)[x];
+                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~bits_of(gone, x);
+                    const uint32_t bad = bits_of(nans, x);
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
@@ -331,19 +354,21 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
                 }
             } else {
+                uint32_t v[2][16];
+                tmem_ld_32x32b_x16(s_tmem, v[0]);
 #pragma unroll
-                for (int x = 0; x < KT / 32; ++x) {
-                    tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
+                for (int x = 0; x < KT / 16; ++x) {
                     tmem_ld_wait();
-                    uint32_t pk[16];
+                    if (x + 1 < KT / 16) tmem_ld_32x32b_x16(s_tmem + 16 * (x + 1), v[(x + 1) & 1]);
+                    uint32_t pk[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 v = each(fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), factor2, base2));
-                        const float p0 = ex2(v.x), p1 = ex2(v.y);
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 w = each(fma2(both(__uint_as_float(v[x & 1][e]), __uint_as_float(v[x & 1][e + 1])), factor2, base2));
+                        const float p0 = ex2(w.x), p1 = ex2(w.y);
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(p0, p1));
                         pk[e / 2] = pack_half2(p0, p1);
                     }
-                    tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
+                    tmem_st_32x32b_x8(s_tmem + 8 * x, pk);  // over columns that have been read
                 }
             }
             const float2 total = each(add2(sum[0], sum[1]));
@@ -404,20 +429,20 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             }
         }
     } else if (warp < C::MMA_WARP) {
-        // ---------------------------------------------------------------- keys, or values, to f16
-        constexpr int TILES = C::TILES, STEP_TILES = KT / KV4_TILE;
-        const bool values = warp >= C::SOFTMAX_WARPS + C::FEED_WARPS;
-        const int feeder = (warp - C::SOFTMAX_WARPS) % C::FEED_WARPS;
+        // ---------------------------------------------------------------- keys and values to f16
+        // a warp's share of a step: one tile of 16 keys, or half of its channels (groups g0 .. g0 + GW - 1)
+        constexpr int STEP_TILES = KT / KV4_TILE, GW = G / C::SHARES;
+        const int feeder = warp - C::SOFTMAX_WARPS, in_step = feeder / C::SHARES, g0 = feeder % C::SHARES * GW;
         const int r = lane >> 2, c = lane & 3;
         const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
         const int tiles_per_page = p.cache.page_size / KV4_TILE;
-        const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE + (values ? 8 * D : 0);
-        // lane i looks up the i-th of the next 32 tiles of this warp: the page, and the tile's place in it
+        const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
+        // lane i looks up where this warp's tile lies in the i-th of the next 32 steps
         int64_t ahead = -1;
         auto look_up = [&](int j) {
-            const int tile = (begin + j + lane / TILES) * STEP_TILES + feeder * TILES + lane % TILES;
+            const int tile = (begin + j + lane) * STEP_TILES + in_step;
             ahead = -1;
-            if (j + lane / TILES < n && tile * KV4_TILE < hi_all) {
+            if (j + lane < n && tile * KV4_TILE < hi_all) {
                 const int at = tile / tiles_per_page, page = table[at];
                 if (page >= 0 && page < p.cache.num_pages) {
                     ahead = static_cast<int64_t>(page) * p.cache.page_stride + (tile - at * tiles_per_page) * TILE;
@@ -426,124 +451,115 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 }
             }
         };
-        // a step's codes and (s, m) pairs of this lane: of the keys r and r + 8, or of the tokens 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
+        // a step's codes and (s, m) pairs of this lane: of the keys r and r + 8, of the values of 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
         struct Raw {
-            uint32_t word[TILES][4 * G];
-            uint32_t pair[TILES][4 * G];  // keys use half of them
-            bool have[TILES];
+            uint32_t key[2][2 * GW], key_pair[2][GW];
+            uint32_t value[4 * GW], value_pair[4][GW];
+            bool have;
         };
         auto load = [&](Raw& raw, int j) {
-            if (j % (32 / TILES) == 0) look_up(j);
+            if ((j & 31) == 0) look_up(j);
+            const int64_t where = __shfl_sync(0xffffffffu, ahead, j & 31);
+            raw.have = where >= 0;
+            if (!raw.have) return;  // whatever is in the registers: its keys are masked, its values zeroed
+            const uint8_t* at = head_base + where;
 #pragma unroll
-            for (int x = 0; x < TILES; ++x) {
-                const int64_t where = __shfl_sync(0xffffffffu, ahead, (j % (32 / TILES)) * TILES + x);
-                raw.have[x] = where >= 0;
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (W == 2) {
 #pragma unroll
-                for (int e = 0; e < 4 * G; ++e) raw.word[x][e] = raw.pair[x][e] = 0u;
-                if (where < 0) continue;
-                const uint8_t* at = head_base + where;
-                if (W == 2 || values) {
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {  // values: group g; keys: key r or r + 8 (odd g) of the groups g, g + 1 / g - 1, g
-                        const uint4 v = *reinterpret_cast<const uint4*>(at + g * 512 + lane * 16);
-                        raw.word[x][4 * g] = v.x, raw.word[x][4 * g + 1] = v.y, raw.word[x][4 * g + 2] = v.z, raw.word[x][4 * g + 3] = v.w;
+                    for (int h = 0; h < GW / 2; ++h) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(at + (g0 / 2 + h) * 1024 + e * 512 + lane * 16);
+                        raw.key[e][4 * h] = v.x, raw.key[e][4 * h + 1] = v.y, raw.key[e][4 * h + 2] = v.z, raw.key[e][4 * h + 3] = v.w;
                     }
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g0) * 4);
+                    raw.key_pair[e][0] = v.x, raw.key_pair[e][1] = v.y;
                 } else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at + lane * 8), w = *reinterpret_cast<const uint2*>(at + 256 + lane * 8);
-                    raw.word[x][0] = v.x, raw.word[x][1] = v.y, raw.word[x][2] = w.x, raw.word[x][3] = w.y;
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + e * 256 + lane * 8);
+                    raw.key[e][0] = v.x, raw.key[e][1] = v.y;
+                    raw.key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + (r + 8 * e) * 4);
                 }
-                // from here the pairs: keys [16][G] at 16 D of the tile, values behind them
-                const uint32_t* pairs = reinterpret_cast<const uint32_t*>(at + (values ? 9 * D : 16 * D));
-                if (values) {
+            }
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+            for (int g = 0; g < GW; ++g) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * D + (g0 + g) * 512 + lane * 16);
+                raw.value[4 * g] = v.x, raw.value[4 * g + 1] = v.y, raw.value[4 * g + 2] = v.z, raw.value[4 * g + 3] = v.w;
+            }
 #pragma unroll
-                        for (int y = 0; y < G; ++y) {  // two tokens in a row, 2 G words
-                            const uint2 v = *reinterpret_cast<const uint2*>(pairs + (2 * c + 8 * e) * G + 2 * y);
-                            raw.pair[x][2 * G * e + 2 * y] = v.x, raw.pair[x][2 * G * e + 2 * y + 1] = v.y;
-                        }
+            for (int e = 0; e < 4; ++e) {
+                const uint8_t* pair = at + kv4_pair_offset(D, 1) + ((2 * c + (e & 1) + 8 * (e >> 1)) * G + g0) * 4;
+                if constexpr (W == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(pair);
+                    raw.value_pair[e][0] = v.x, raw.value_pair[e][1] = v.y;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int g = 0; g < G; ++g) raw.pair[x][G * e + g] = pairs[(r + 8 * e) * G + g];
+                    raw.value_pair[e][0] = *reinterpret_cast<const uint32_t*>(pair);
                 }
             }
         };
         auto convert_keys = [&](const Raw& raw, uint8_t* k_smem) {
 #pragma unroll
-            for (int x = 0; x < TILES; ++x)
+            for (int e = 0; e < 2; ++e) {
+                uint8_t* row = k_smem + (in_step * KV4_TILE + r + 8 * e) * 128;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = (feeder * TILES + x) * KV4_TILE + r + 8 * e;
-                    uint8_t* row = k_smem + key * 128;
+                for (int g = 0; g < GW; ++g) {
+                    const __half2 sm = as_h2(raw.key_pair[e][g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const __half2 sm = as_h2(raw.pair[x][G * e + g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            // 16-byte chunk h of 512 * e holds groups W h .. W h + W - 1
-                            const uint32_t word = W == 2 ? raw.word[x][(g / 2 * 2 + e) * 4 + (g & 1) * 2 + u] : raw.word[x][2 * e + u];
-                            uint32_t o[4];
-                            expand(word, s2, m2, s2, m2, o);
-                            *reinterpret_cast<uint4*>(row + g * (KT * 128) + (((2 * c + u) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
-                    }
-                }
-        };
-        auto convert_values = [&](Raw& raw, uint8_t* v_smem, int j, int stage) {
-#pragma unroll
-            for (int x = 0; x < TILES; ++x) {
-                const int in_step = feeder * TILES + x, key0 = (begin + j) * KT + in_step * KV4_TILE;
-                // values of keys beyond the sequence and NaN values are zeroed: a zero weight times NaN would reach every row
-                uint32_t top = 0u;
-#pragma unroll
-                for (int e = 0; e < 4 * G; ++e) top |= (raw.pair[x][e] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
-                uint32_t nan_bits = 0u;
-                if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len)) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
-                        uint32_t ones = 0u;
-#pragma unroll
-                        for (int g = 0; g < G; ++g) ones |= (raw.pair[x][G * e + g] & 0x7c007c00u) + 0x04000400u;
-                        const bool beyond = key0 + tok >= sq.len, nan = (ones & 0x80008000u) != 0u;
-                        if (beyond || nan) {
-#pragma unroll
-                            for (int g = 0; g < G; ++g) raw.pair[x][G * e + g] = 0u;
-                        }
-                        if (nan && !beyond) nan_bits |= 1u << tok;
-                    }
-                    nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 1);
-                    nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
-                }
-                if (lane == 0) {
-                    flags[stage * 16 + in_step] = raw.have[x] || key0 >= hi_all ? 0u : 0xffffu;
-                    flags[stage * 16 + 8 + in_step] = static_cast<uint16_t>(nan_bits);
-                }
-                uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + r * 128 + 4 * c;
-                const int at0 = ((2 * (in_step & 3)) ^ r) << 4, at1 = ((2 * (in_step & 3) + 1) ^ r) << 4;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const __half2 t0 = as_h2(raw.pair[x][g]), t1 = as_h2(raw.pair[x][G + g]), t2 = as_h2(raw.pair[x][2 * G + g]), t3 = as_h2(raw.pair[x][3 * G + g]);
-                    const __half2 s_lo = __lows2half2(t0, t1), m_lo = __highs2half2(t0, t1), s_hi = __lows2half2(t2, t3), m_hi = __highs2half2(t2, t3);
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
-                        uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
-                        expand(raw.word[x][4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
-                        uint8_t* to = row + (64 * g + 16 * jj) * 128;
-                        *reinterpret_cast<uint32_t*>(to + at0) = o[0];
-                        *reinterpret_cast<uint32_t*>(to + 8 * 128 + at0) = o[1];
-                        *reinterpret_cast<uint32_t*>(to + at1) = o[2];
-                        *reinterpret_cast<uint32_t*>(to + 8 * 128 + at1) = o[3];
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t o[4];
+                        expand(raw.key[e][2 * g + u], s2, m2, s2, m2, o);
+                        *reinterpret_cast<uint4*>(row + (g0 + g) * (KT * 128) + (((2 * c + u) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 }
             }
         };
-        uint64_t* full = values ? bar->vfull : bar->kfull;
-        uint64_t* free = values ? bar->vfree : bar->kfree;
-        uint8_t* operand = smem + (values ? C::V_OFF : C::K_OFF);
-        Raw raw[2];
+        auto convert_values = [&](Raw& raw, uint8_t* v_smem, int j, int stage) {
+            const int key0 = (begin + j) * KT + in_step * KV4_TILE;
+            // values of keys that are not there, and NaN values, are zeroed: a zero weight times NaN would reach every row
+            uint32_t top = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int g = 0; g < GW; ++g) top |= (raw.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
+            uint32_t nan_bits = 0u;
+            if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len || !raw.have)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
+                    uint32_t ones = 0u;
+#pragma unroll
+                    for (int g = 0; g < GW; ++g) ones |= (raw.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;
+                    const bool beyond = key0 + tok >= sq.len || !raw.have, nan = (ones & 0x80008000u) != 0u;
+                    if (beyond || nan) {
+#pragma unroll
+                        for (int g = 0; g < GW; ++g) raw.value_pair[e][g] = 0u;
+                    }
+                    if (nan && !beyond) nan_bits |= 1u << tok;
+                }
+                nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 1);
+                nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
+            }
+            if (lane == 0) {
+                flags[stage * FLAGS + feeder] = raw.have || key0 >= hi_all ? 0u : 0xffffu;
+                flags[stage * FLAGS + 8 + feeder] = static_cast<uint16_t>(nan_bits);
+            }
+            uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + r * 128 + 4 * c;
+            const int at0 = ((2 * (in_step & 3)) ^ r) << 4, at1 = ((2 * (in_step & 3) + 1) ^ r) << 4;
+#pragma unroll
+            for (int g = 0; g < GW; ++g) {
+                const __half2 t0 = as_h2(raw.value_pair[0][g]), t1 = as_h2(raw.value_pair[1][g]), t2 = as_h2(raw.value_pair[2][g]), t3 = as_h2(raw.value_pair[3][g]);
+                const __half2 s_lo = __lows2half2(t0, t1), m_lo = __highs2half2(t0, t1), s_hi = __lows2half2(t2, t3), m_hi = __highs2half2(t2, t3);
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
+                    expand(raw.value[4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
+                    uint8_t* to = row + (64 * (g0 + g) + 16 * jj) * 128;
+                    *reinterpret_cast<uint32_t*>(to + at0) = o[0];
+                    *reinterpret_cast<uint32_t*>(to + 8 * 128 + at0) = o[1];
+                    *reinterpret_cast<uint32_t*>(to + at1) = o[2];
+                    *reinterpret_cast<uint32_t*>(to + 8 * 128 + at1) = o[3];
+                }
+            }
+        };
+        Raw raw[2] = {};
         if (n > 0) load(raw[0], 0);
         bool ok = true;
         for (int j0 = 0; ok && j0 < n; j0 += 2) {
@@ -552,20 +568,26 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 const int j = j0 + stage;
                 if (j >= n) break;
                 if (j + 1 < n) load(raw[stage ^ 1], j + 1);  // in flight under this step's work
-                if (j >= 2 && !mbar_wait_bounded(&free[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
                     give_up(abort_word, 415);
                     ok = false;
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (values) {
-                    convert_values(raw[stage], operand + stage * C::K_BYTES, j, stage);
-                } else {
-                    convert_keys(raw[stage], operand + stage * C::K_BYTES);
-                }
+                convert_keys(raw[stage], smem + C::K_OFF + stage * C::K_BYTES);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[stage]);
+                if (lane == 0) mbar_arrive(&bar->kfull[stage]);
+                if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                    give_up(abort_word, 415);
+                    ok = false;
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                convert_values(raw[stage], smem + C::V_OFF + stage * C::K_BYTES, j, stage);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->vfull[stage]);
             }
         }
     } else {
