@@ -214,38 +214,47 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const int i = row / p.group;
         const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
         const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
-        // the query row to f16 in shared memory, by a power of two of its own
+        // this warp's 32 query rows to f16 in shared memory, each by a power of two of its own: D / 8 lanes read a row, and the
+        // thread of the row keeps its exponent
         const int64_t q_row = sq.row0 + (there ? i : 0);
         const int head = hk * p.group + (there ? row % p.group : 0);
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row * p.ldq + static_cast<int64_t>(head) * D);
-        float top = 0.0f;
-        if (there) {
-#pragma unroll 4
-            for (int w = 0; w < D / 8; ++w) {
-                const uint4 raw = __ldg(src + w);
-                const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+        constexpr int LPR = D / 8, RPI = 32 / LPR, BATCH = 4;  // lanes of a row, rows of a load, loads in flight
+        uint8_t* q_smem = smem + t * 128 * D * 2;
+        const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        int ex = 0;
+#pragma unroll 1
+        for (int b0 = 0; b0 < LPR; b0 += BATCH) {
+            uint4 raw[BATCH];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v[e] << 16)), fabsf(__uint_as_float(v[e] & 0xffff0000u))));
+            for (int y = 0; y < BATCH; ++y) {
+                const int from = (b0 + y) * RPI + lane / LPR;  // of the warp's 32
+                const int rr = __shfl_sync(0xffffffffu, static_cast<int>(q_row), from), hh = __shfl_sync(0xffffffffu, head, from);
+                const bool have = __shfl_sync(0xffffffffu, static_cast<int>(there), from) != 0;
+                raw[y] = make_uint4(0u, 0u, 0u, 0u);
+                if (have) raw[y] = __ldg(reinterpret_cast<const uint4*>(p.q + rr * p.ldq + static_cast<int64_t>(hh) * D) + lane % LPR);
+            }
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y) {
+                const uint32_t v[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
+                uint32_t top = 0u;  // the bits of |x| order as the numbers do
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, max((v[e] << 16) & 0x7fffffffu, v[e] & 0x7fff0000u));
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                int x = static_cast<int>(top >> 23) - 127 - 14;
+                x = top == 0u || top >= 0x7f800000u ? 0 : max(-100, min(100, x));
+                const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23) * sign;
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[2 * e] = __uint_as_float(v[e] << 16) * down, f[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u) * down;
+                const int w = lane % LPR, at = (warp & 3) * 32 + (b0 + y) * RPI + lane / LPR;
+                *reinterpret_cast<uint4*>(q_smem + (w >> 3) * (128 * 128) + at * 128 + (((w & 7) ^ (at & 7)) << 4)) =
+                    make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
+                const int mine = __shfl_sync(0xffffffffu, x, (lane % RPI) * LPR);
+                if (lane / RPI == b0 + y) ex = mine;
             }
         }
-        int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
-        ex = max(-100, min(100, ex));
-        if (top == 0.0f || top > 3.0e38f) ex = 0;
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
         const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f);
-        uint8_t* q_smem = smem + t * 128 * D * 2;
-#pragma unroll 4
-        for (int w = 0; w < D / 8; ++w) {
-            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-            if (there) raw = __ldg(src + w);
-            const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(v[e] << 16) * down, x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u) * down;
-            *reinterpret_cast<uint4*>(q_smem + (w >> 3) * (128 * 128) + in_block * 128 + (((w & 7) ^ (in_block & 7)) << 4)) =
-                make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
-        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->qfull);
@@ -390,32 +399,53 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         if (ok) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t part = (tile_id * p.splits + split) * ROWS + t * 128 + in_block;
-            __nv_bfloat16* out = p.out + q_row * p.ldo + static_cast<int64_t>(head) * D;
+            // the queries are no longer needed: their rows take this warp's output rows (bf16, or half of an f32 row at a time), and
+            // whole rows leave from there
+            constexpr int CHUNKS = D / 8;  // of 16 bytes in a row
+            auto place = [&](int r_, int w) { return q_smem + ((warp & 3) * 32 + r_) * (D * 2) + ((w ^ (r_ & 7)) << 4); };
+            const bool direct = p.splits == 1;
 #pragma unroll 1
-            for (int x = 0; x < D / 32; ++x) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld_32x32b_x32(o_tmem + 32 * x, o);
-                    tmem_ld_wait();
-                } else {
+            for (int half = 0; half < (direct ? 1 : 2); ++half) {
+#pragma unroll 1
+                for (int x = direct ? 0 : half * (D / 64); x < (direct ? D / 32 : (half + 1) * (D / 64)); ++x) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tmem_ld_32x32b_x32(o_tmem + 32 * x, o);
+                        tmem_ld_wait();
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0u;
-                }
-                if (there && p.splits == 1) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
-                            v[y] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                        *reinterpret_cast<uint4*>(out + 32 * x + e) = make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
                     }
-                } else if (there) {
-                    uint4* to = reinterpret_cast<uint4*>(p.part_o + part * D + 32 * x);
+                    if (direct) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) to[e / 4] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
+                                v[y] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            *reinterpret_cast<uint4*>(place(lane, 4 * x + e / 8)) = make_uint4(v[0], v[1], v[2], v[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<uint4*>(place(lane, 8 * (x - half * (D / 64)) + e / 4)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int y = 0; y < CHUNKS; ++y) {  // 32 chunks at a time
+                    const int from = (y * 32 + lane) / CHUNKS, w = lane % CHUNKS;
+                    const int rr = __shfl_sync(0xffffffffu, static_cast<int>(q_row), from), hh = __shfl_sync(0xffffffffu, head, from);
+                    const bool have = __shfl_sync(0xffffffffu, static_cast<int>(there), from) != 0;
+                    const uint4 v = *reinterpret_cast<const uint4*>(place(from, w));
+                    if (!have) continue;
+                    if (direct) {
+                        *(reinterpret_cast<uint4*>(p.out + rr * p.ldo + static_cast<int64_t>(hh) * D) + w) = v;
+                    } else {
+                        *(reinterpret_cast<uint4*>(p.part_o + (part - lane + from) * D + half * (D / 2)) + w) = v;
+                    }
                 }
                 __syncwarp();
             }
