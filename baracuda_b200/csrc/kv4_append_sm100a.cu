@@ -40,7 +40,6 @@ __device__ __forceinline__ f32x2 add_products(f32x2 a, f32x2 b) {
     const float2 x = each(a), y = each(b);
     return both(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
 }
-__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) { return fma2(b, 0xbf800000bf800000ull, a); }
 // a + b = sum + err exactly (Knuth's two-sum); `low` collects the errors.
 __device__ __forceinline__ f32x2 two_sum2(f32x2 a, f32x2 b, f32x2& low) {
     const f32x2 s = add2(a, b), t = sub2(s, a);

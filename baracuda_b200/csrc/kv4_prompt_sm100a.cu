@@ -31,6 +31,10 @@ namespace {
 
 __device__ int g_kv4_prompt_device_status = 0;
 
+#ifndef PR_POLY_MASK
+#define PR_POLY_MASK 14
+#define PR_POLY_AT 2
+#endif
 constexpr float PR_SLACK = 7.0f;  // p <= 2^(SLACK + LIFT) stays within f16
 constexpr float PR_LIFT = 8.0f;   // f16's range below the reference: 2^-22 in full precision
 
@@ -42,6 +46,10 @@ struct PromptCfg {
     static constexpr int SHARES = FEED_WARPS / (KT / KV4_TILE);  // of a tile of 16 keys: whole tiles, or halves of its channels
     static constexpr int MMA_WARP = SOFTMAX_WARPS + FEED_WARPS;
     static constexpr int THREADS = (MMA_WARP + 1) * 32;
+    // two row blocks: 17 warps leave 96 registers a thread at launch; the feeding warps hand a third of theirs to the softmax warps
+    static constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 128, FEED_REGS = 64;
+    static_assert(NQ == 1 || SOFTMAX_WARPS * SOFTMAX_REGS + FEED_WARPS * FEED_REGS + LAUNCH_REGS <= (MMA_WARP + 1) * LAUNCH_REGS,
+                  "the shares come out of what the block was launched with");
     static constexpr int Q_BYTES = NQ * 128 * D * 2;
     static constexpr int K_BYTES = KT * D * 2;  // V the same
     static constexpr int K_OFF = Q_BYTES;
@@ -78,18 +86,12 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_32x32b_x64(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
         : "r"(taddr)
         : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -116,6 +118,24 @@ __device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32
 }
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+// 2^x of a pair on the FMA units, x at most 16: n = rint(x), 2^(x - n) by the polynomial of degree 4 that is nearest in relative
+// error on [-1/2, 1/2] (Remez exchange; 2.7e-6 with its f32 roundings), n added to the exponent.  Below 2^-125 the result is no more
+// than that.  The special function unit gives 2 results per clock and quarter of an SM, 16 clocks for a warp, and would bound the
+// kernel at 4096 clocks for 256 rows x 128 keys; half of the exponentials are computed here.
+__device__ __forceinline__ float2 ex2_pair(float2 x) {
+    const f32x2 magic = both(12582912.0f, 12582912.0f), back = both(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
+    const f32x2 v = both(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+    const f32x2 t = add2(v, magic);
+    const f32x2 f = sub2(v, add2(t, back));
+    f32x2 p = both(0.009570102207362652f, 0.009570102207362652f);
+    p = fma2(p, f, both(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, both(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, both(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, both(0.9999992847442627f, 0.9999992847442627f));
+    const float2 r = each(p), n = each(t);
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+}
 
 // The 8 codes of a word as 4 pairs of f16 values s * c + m: pairs (0, 4), (1, 5), (2, 6), (3, 7), where nibbles 0, 2, 4, 6 take
 // (s, m) of `even` and 1, 3, 5, 7 the same (keys: one scale; values: nibble parity is a channel, the pair two tokens, and the
@@ -205,6 +225,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     const uint32_t tmem = bar->tmem_slot;
 
     if (warp < C::SOFTMAX_WARPS) {
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         // ---------------------------------------------------------------- softmax: one thread per row
         const int t = warp >> 2;                         // row block
         const int in_block = threadIdx.x & 127;
@@ -218,7 +239,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         // thread of the row keeps its exponent
         const int64_t q_row = sq.row0 + (there ? i : 0);
         const int head = hk * p.group + (there ? row % p.group : 0);
-        constexpr int LPR = D / 8, RPI = 32 / LPR, BATCH = 4;  // lanes of a row, rows of a load, loads in flight
+        constexpr int LPR = D / 8, RPI = 32 / LPR, BATCH = 8;  // lanes of a row, rows of a load, loads in flight
         uint8_t* q_smem = smem + t * 128 * D * 2;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
         int ex = 0;
@@ -291,65 +312,84 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 return ((w[2 * x] | (w[2 * x] >> 16)) & 0xffffu) | ((w[2 * x + 1] | (w[2 * x + 1] << 16)) & 0xffff0000u);
             };
             const bool edge = key0 + KT > hi_min || key0 < lo_max || any != 0u;
+            const f32x2 factor2 = both(factor, factor);
             float mx = -INFINITY;
-            uint32_t s[32];
-            if (edge) {
+            bool done = false;
+            if (!edge) {
+                // the common step in one reading: P with the reference as it is, and the maximum that tells whether it holds; P goes
+                // over S only then
+                const f32x2 base2 = both(PR_LIFT - ref, PR_LIFT - ref);
+                f32x2 sum[2] = {0ull, 0ull};
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                uint32_t pk[KT / 32][16];
+#pragma unroll
+                for (int x = 0; x < KT / 64; ++x) {
+                    uint32_t v[64];
+                    tmem_ld_32x32b_x64(s_tmem + 64 * x, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const float s0 = __uint_as_float(v[e]), s1 = __uint_as_float(v[e + 1]);
+                        m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], s0), s1);
+                        const float2 w = each(fma2(both(s0, s1), factor2, base2));
+                        const float2 pr = (e & PR_POLY_MASK) == PR_POLY_AT ? ex2_pair(w) : make_float2(ex2(w.x), ex2(w.y));
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(pr.x, pr.y));
+                        pk[2 * x + (e >> 5)][(e & 31) / 2] = pack_half2(pr.x, pr.y);
+                    }
+                }
+                mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor;
+                if (!__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
+                    done = true;
+#pragma unroll
+                    for (int x = 0; x < KT / 32; ++x) tmem_st_32x32b_x16(s_tmem + 16 * x, pk[x]);
+                    const float2 total = each(add2(sum[0], sum[1]));
+                    l += total.x + total.y;
+                }
+            } else {
 #pragma unroll 1
                 for (int x = 0; x < KT / 32; ++x) {
+                    uint32_t s[32];
                     tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
                     tmem_ld_wait();
                     const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~bits_of(gone, x);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) mx = fmaxf(mx, ((seen >> e) & 1u) ? __uint_as_float(s[e]) : -INFINITY);
                 }
-            } else {  // 16 columns are on their way while the 16 before are looked at
-                uint32_t v[2][16];
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tmem_ld_32x32b_x16(s_tmem, v[0]);
-#pragma unroll
-                for (int x = 0; x < KT / 16; ++x) {
-                    tmem_ld_wait();
-                    if (x + 1 < KT / 16) tmem_ld_32x32b_x16(s_tmem + 16 * (x + 1), v[(x + 1) & 1]);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2)
-                        m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(v[x & 1][e])), __uint_as_float(v[x & 1][e + 1]));
-                }
-                mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                mx *= factor;
             }
-            mx *= factor;
-            if (__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
-                const float to = mx > ref + PR_SLACK ? mx : ref;
-                const float fix = ex2(ref - to);
-                ref = to;
-                l *= fix;
-                if (j > 0) {
-                    if (!mbar_wait_bounded(&bar->pvdone[t], (j - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
-                        give_up(abort_word, 413);
-                        ok = false;
-                    }
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    tc_fence_after_sync();
+            if (!done) {
+                if (__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
+                    const float to = mx > ref + PR_SLACK ? mx : ref;
+                    const float fix = ex2(ref - to);
+                    ref = to;
+                    l *= fix;
+                    if (j > 0) {
+                        if (!mbar_wait_bounded(&bar->pvdone[t], (j - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                            give_up(abort_word, 413);
+                            ok = false;
+                        }
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        tc_fence_after_sync();
 #pragma unroll 1
-                    for (int x = 0; x < D / 32; ++x) {
-                        tmem_ld_32x32b_x32(o_tmem + 32 * x, s);
-                        tmem_ld_wait();
+                        for (int x = 0; x < D / 32; ++x) {
+                            uint32_t s[32];
+                            tmem_ld_32x32b_x32(o_tmem + 32 * x, s);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * fix);
-                        tmem_st_32x32b_x32(o_tmem + 32 * x, s);
+                            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * fix);
+                            tmem_st_32x32b_x32(o_tmem + 32 * x, s);
+                        }
+                        tmem_st_wait();
                     }
-                    tmem_st_wait();
                 }
-            }
-            const float base = PR_LIFT - ref;
-            const f32x2 factor2 = both(factor, factor), base2 = both(base, base);
-            f32x2 sum[2] = {0ull, 0ull};
-            if (edge) {
+                const f32x2 base2 = both(PR_LIFT - ref, PR_LIFT - ref);
+                f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll 1
                 for (int x = 0; x < KT / 32; ++x) {
+                    uint32_t s[32];
                     tmem_ld_32x32b_x32(s_tmem + 32 * x, s);
                     tmem_ld_wait();
-                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~bits_of(gone, x);
-                    const uint32_t bad = bits_of(nans, x);
+                    const uint32_t seen = seen_keys(key0 + 32 * x, lo, hi) & ~bits_of(gone, x), bad = bits_of(nans, x);
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
@@ -360,28 +400,11 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(p0, p1));
                         pk[e / 2] = pack_half2(p0, p1);
                     }
-                    tmem_st_32x32b_x16(s_tmem + 16 * x, pk);
+                    tmem_st_32x32b_x16(s_tmem + 16 * x, pk);  // over columns that have been read
                 }
-            } else {
-                uint32_t v[2][16];
-                tmem_ld_32x32b_x16(s_tmem, v[0]);
-#pragma unroll
-                for (int x = 0; x < KT / 16; ++x) {
-                    tmem_ld_wait();
-                    if (x + 1 < KT / 16) tmem_ld_32x32b_x16(s_tmem + 16 * (x + 1), v[(x + 1) & 1]);
-                    uint32_t pk[8];
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 w = each(fma2(both(__uint_as_float(v[x & 1][e]), __uint_as_float(v[x & 1][e + 1])), factor2, base2));
-                        const float p0 = ex2(w.x), p1 = ex2(w.y);
-                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(p0, p1));
-                        pk[e / 2] = pack_half2(p0, p1);
-                    }
-                    tmem_st_32x32b_x8(s_tmem + 8 * x, pk);  // over columns that have been read
-                }
+                const float2 total = each(add2(sum[0], sum[1]));
+                l += total.x + total.y;
             }
-            const float2 total = each(add2(sum[0], sum[1]));
-            l += total.x + total.y;
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -399,8 +422,10 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         if (ok) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t part = (tile_id * p.splits + split) * ROWS + t * 128 + in_block;
-            // the queries are no longer needed: their rows take this warp's output rows (bf16, or half of an f32 row at a time), and
-            // whole rows leave from there
+            // the queries are no longer needed (of any warp: the last MMA is over, or, where there was none, the block's warps have
+            // written theirs): their place takes this warp's output rows (bf16, or half of an f32 row at a time), and whole rows
+            // leave from there
+            if (n == 0) named_bar_sync(1 + t, 128);
             constexpr int CHUNKS = D / 8;  // of 16 bytes in a row
             auto place = [&](int r_, int w) { return q_smem + ((warp & 3) * 32 + r_) * (D * 2) + ((w ^ (r_ & 7)) << 4); };
             const bool direct = p.splits == 1;
@@ -440,10 +465,9 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     const int rr = __shfl_sync(0xffffffffu, static_cast<int>(q_row), from), hh = __shfl_sync(0xffffffffu, head, from);
                     const bool have = __shfl_sync(0xffffffffu, static_cast<int>(there), from) != 0;
                     const uint4 v = *reinterpret_cast<const uint4*>(place(from, w));
-                    if (!have) continue;
-                    if (direct) {
+                    if (have && direct) {
                         *(reinterpret_cast<uint4*>(p.out + rr * p.ldo + static_cast<int64_t>(hh) * D) + w) = v;
-                    } else {
+                    } else if (have) {
                         *(reinterpret_cast<uint4*>(p.part_o + (part - lane + from) * D + half * (D / 2)) + w) = v;
                     }
                 }
@@ -459,6 +483,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             }
         }
     } else if (warp < C::MMA_WARP) {
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEED_REGS));
         // ---------------------------------------------------------------- keys and values to f16
         // a warp's share of a step: one tile of 16 keys, or half of its channels (groups g0 .. g0 + GW - 1)
         constexpr int STEP_TILES = KT / KV4_TILE, GW = G / C::SHARES;
@@ -482,85 +507,90 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             }
         };
         // a step's codes and (s, m) pairs of this lane: of the keys r and r + 8, of the values of 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
-        struct Raw {
-            uint32_t key[2][2 * GW], key_pair[2][GW];
-            uint32_t value[4 * GW], value_pair[4][GW];
-            bool have;
-        };
-        auto load = [&](Raw& raw, int j) {
-            if ((j & 31) == 0) look_up(j);
+        uint32_t key[2][2 * GW] = {}, key_pair[2][GW] = {};
+        uint32_t value[4 * GW] = {}, value_pair[4][GW] = {};
+        bool have = false;  // the values' tile
+        auto place_of = [&](int j) -> const uint8_t* {
             const int64_t where = __shfl_sync(0xffffffffu, ahead, j & 31);
-            raw.have = where >= 0;
-            if (!raw.have) return;  // whatever is in the registers: its keys are masked, its values zeroed
-            const uint8_t* at = head_base + where;
+            return where < 0 ? nullptr : head_base + where;
+        };
+        auto load_keys = [&](int j) {
+            if ((j & 31) == 0) look_up(j);
+            const uint8_t* at = place_of(j);
+            if (at == nullptr) return;  // whatever is in the registers: these keys are masked
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 if constexpr (W == 2) {
 #pragma unroll
                     for (int h = 0; h < GW / 2; ++h) {
                         const uint4 v = *reinterpret_cast<const uint4*>(at + (g0 / 2 + h) * 1024 + e * 512 + lane * 16);
-                        raw.key[e][4 * h] = v.x, raw.key[e][4 * h + 1] = v.y, raw.key[e][4 * h + 2] = v.z, raw.key[e][4 * h + 3] = v.w;
+                        key[e][4 * h] = v.x, key[e][4 * h + 1] = v.y, key[e][4 * h + 2] = v.z, key[e][4 * h + 3] = v.w;
                     }
                     const uint2 v = *reinterpret_cast<const uint2*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g0) * 4);
-                    raw.key_pair[e][0] = v.x, raw.key_pair[e][1] = v.y;
+                    key_pair[e][0] = v.x, key_pair[e][1] = v.y;
                 } else {
                     const uint2 v = *reinterpret_cast<const uint2*>(at + e * 256 + lane * 8);
-                    raw.key[e][0] = v.x, raw.key[e][1] = v.y;
-                    raw.key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + (r + 8 * e) * 4);
+                    key[e][0] = v.x, key[e][1] = v.y;
+                    key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + (r + 8 * e) * 4);
                 }
             }
+        };
+        auto load_values = [&](int j) {
+            const uint8_t* at = place_of(j);
+            have = at != nullptr;
+            if (!have) return;  // as above: zeroed below
 #pragma unroll
             for (int g = 0; g < GW; ++g) {
                 const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * D + (g0 + g) * 512 + lane * 16);
-                raw.value[4 * g] = v.x, raw.value[4 * g + 1] = v.y, raw.value[4 * g + 2] = v.z, raw.value[4 * g + 3] = v.w;
+                value[4 * g] = v.x, value[4 * g + 1] = v.y, value[4 * g + 2] = v.z, value[4 * g + 3] = v.w;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint8_t* pair = at + kv4_pair_offset(D, 1) + ((2 * c + (e & 1) + 8 * (e >> 1)) * G + g0) * 4;
                 if constexpr (W == 2) {
                     const uint2 v = *reinterpret_cast<const uint2*>(pair);
-                    raw.value_pair[e][0] = v.x, raw.value_pair[e][1] = v.y;
+                    value_pair[e][0] = v.x, value_pair[e][1] = v.y;
                 } else {
-                    raw.value_pair[e][0] = *reinterpret_cast<const uint32_t*>(pair);
+                    value_pair[e][0] = *reinterpret_cast<const uint32_t*>(pair);
                 }
             }
         };
-        auto convert_keys = [&](const Raw& raw, uint8_t* k_smem) {
+        auto convert_keys = [&](uint8_t* k_smem) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 uint8_t* row = k_smem + (in_step * KV4_TILE + r + 8 * e) * 128;
 #pragma unroll
                 for (int g = 0; g < GW; ++g) {
-                    const __half2 sm = as_h2(raw.key_pair[e][g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
+                    const __half2 sm = as_h2(key_pair[e][g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         uint32_t o[4];
-                        expand(raw.key[e][2 * g + u], s2, m2, s2, m2, o);
+                        expand(key[e][2 * g + u], s2, m2, s2, m2, o);
                         *reinterpret_cast<uint4*>(row + (g0 + g) * (KT * 128) + (((2 * c + u) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 }
             }
         };
-        auto convert_values = [&](Raw& raw, uint8_t* v_smem, int j, int stage) {
+        auto convert_values = [&](uint8_t* v_smem, int j, int stage) {
             const int key0 = (begin + j) * KT + in_step * KV4_TILE;
             // values of keys that are not there, and NaN values, are zeroed: a zero weight times NaN would reach every row
             uint32_t top = 0u;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int g = 0; g < GW; ++g) top |= (raw.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
+                for (int g = 0; g < GW; ++g) top |= (value_pair[e][g] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
             uint32_t nan_bits = 0u;
-            if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len || !raw.have)) {
+            if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len || !have)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
                     uint32_t ones = 0u;
 #pragma unroll
-                    for (int g = 0; g < GW; ++g) ones |= (raw.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;
-                    const bool beyond = key0 + tok >= sq.len || !raw.have, nan = (ones & 0x80008000u) != 0u;
+                    for (int g = 0; g < GW; ++g) ones |= (value_pair[e][g] & 0x7c007c00u) + 0x04000400u;
+                    const bool beyond = key0 + tok >= sq.len || !have, nan = (ones & 0x80008000u) != 0u;
                     if (beyond || nan) {
 #pragma unroll
-                        for (int g = 0; g < GW; ++g) raw.value_pair[e][g] = 0u;
+                        for (int g = 0; g < GW; ++g) value_pair[e][g] = 0u;
                     }
                     if (nan && !beyond) nan_bits |= 1u << tok;
                 }
@@ -568,19 +598,19 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
             }
             if (lane == 0) {
-                flags[stage * FLAGS + feeder] = raw.have || key0 >= hi_all ? 0u : 0xffffu;
+                flags[stage * FLAGS + feeder] = have || key0 >= hi_all ? 0u : 0xffffu;
                 flags[stage * FLAGS + 8 + feeder] = static_cast<uint16_t>(nan_bits);
             }
             uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + r * 128 + 4 * c;
             const int at0 = ((2 * (in_step & 3)) ^ r) << 4, at1 = ((2 * (in_step & 3) + 1) ^ r) << 4;
 #pragma unroll
             for (int g = 0; g < GW; ++g) {
-                const __half2 t0 = as_h2(raw.value_pair[0][g]), t1 = as_h2(raw.value_pair[1][g]), t2 = as_h2(raw.value_pair[2][g]), t3 = as_h2(raw.value_pair[3][g]);
+                const __half2 t0 = as_h2(value_pair[0][g]), t1 = as_h2(value_pair[1][g]), t2 = as_h2(value_pair[2][g]), t3 = as_h2(value_pair[3][g]);
                 const __half2 s_lo = __lows2half2(t0, t1), m_lo = __highs2half2(t0, t1), s_hi = __lows2half2(t2, t3), m_hi = __highs2half2(t2, t3);
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
-                    expand(raw.value[4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
+                    expand(value[4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
                     uint8_t* to = row + (64 * (g0 + g) + 16 * jj) * 128;
                     *reinterpret_cast<uint32_t*>(to + at0) = o[0];
                     *reinterpret_cast<uint32_t*>(to + 8 * 128 + at0) = o[1];
@@ -589,36 +619,32 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 }
             }
         };
-        Raw raw[2] = {};
-        if (n > 0) load(raw[0], 0);
+        // the next step's keys are on their way under this step's values, and the other way round
+        if (n > 0) load_keys(0), load_values(0);
         bool ok = true;
-        for (int j0 = 0; ok && j0 < n; j0 += 2) {
-#pragma unroll
-            for (int stage = 0; stage < 2; ++stage) {  // step j0 + stage, from raw[stage]
-                const int j = j0 + stage;
-                if (j >= n) break;
-                if (j + 1 < n) load(raw[stage ^ 1], j + 1);  // in flight under this step's work
-                if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
-                    give_up(abort_word, 415);
-                    ok = false;
-                }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                convert_keys(raw[stage], smem + C::K_OFF + stage * C::K_BYTES);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar->kfull[stage]);
-                if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
-                    give_up(abort_word, 415);
-                    ok = false;
-                }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                convert_values(raw[stage], smem + C::V_OFF + stage * C::K_BYTES, j, stage);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar->vfull[stage]);
+        for (int j = 0; j < n; ++j) {
+            const int stage = j & 1;
+            if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 415);
+                ok = false;
             }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            convert_keys(smem + C::K_OFF + stage * C::K_BYTES);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->kfull[stage]);
+            // the look-up of the next 32 steps must not replace what this step's values still go by: they are loaded already
+            if (j + 1 < n) load_keys(j + 1);
+            if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                give_up(abort_word, 415);
+                ok = false;
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            convert_values(smem + C::V_OFF + stage * C::K_BYTES, j, stage);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->vfull[stage]);
+            if (j + 1 < n) load_values(j + 1);
         }
     } else {
         // ---------------------------------------------------------------- MMA issue: the warp walks the steps, one lane issues
@@ -710,6 +736,14 @@ int32_t launch_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stre
     auto kern = kv4_prompt_kernel<D, NQ>;
     constexpr int bytes = PromptCfg<D, NQ>::TOTAL;
     static_assert(bytes <= 232448, "shared memory of an SM");
+    if constexpr (NQ == 2) {
+        // the warps' shares of the registers are sums over what a launch gets: never start a build that gets another number
+        static const bool as_assumed = [kern] {
+            cudaFuncAttributes a;
+            return cudaFuncGetAttributes(&a, kern) == cudaSuccess && a.numRegs == PromptCfg<D, NQ>::LAUNCH_REGS;
+        }();
+        if (!as_assumed) return BQ_STATUS_LAUNCH_FAILURE;
+    }
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
         (void)cudaGetLastError();
         return BQ_STATUS_LAUNCH_FAILURE;

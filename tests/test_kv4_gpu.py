@@ -554,3 +554,14 @@ def test_norm_and_rotation_round_step_by_step():
             one, two = a * c - b * s, b * c + a * s
             want = torch.stack([one, two], -1).flatten(-2) if interleaved else torch.cat([one, two], -1)
             assert torch.equal(k_out.reshape(t, heads, dim), want.to(BF16))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows_without_keys(dim):
+    """Whole blocks of rows that see nothing, many of them at once and again and again: zeros, every time."""
+    p = Problem([(200, 30), (150, 0), (140, 20), (300, 64)], 8, 2, dim, 16, seed=31)
+    first = p.run()
+    p.check(first)
+    for _ in range(30):
+        again = p.run()
+        assert torch.equal(again.out, first.out) and torch.equal(again.lse, first.lse)
