@@ -4,22 +4,26 @@
 // Bound: the cache's bytes (144 per token and kv head at D = 128), which every other term hides behind as long as a token
 // costs few instructions.  So codes are never turned into numbers: both products run on mma.m16n8k16 with the codes as the A
 // operand in the form in which they lie in memory (f16 subnormals, one AND per pair; one shift per word), 16 tokens x 8 query
-// rows at a time, and scales and minima enter outside:
-//   q . k[t]  = sum_g s[t, g] * (q_g . c[t, g]) + m[t, g] * sum(q_g)           (S^T = C Q^T per group of 64 channels)
-//   sum_t p[t] v[t] = sum_t (p[t] s[t, g]) c[t, g] + sum_t p[t] m[t, g]         (O^T = C^T W, W = p * s in f16)
+// rows at a time, and scales and minima enter outside, per group g of 64 channels:
+//   q . k[t]  = sum_g s[t, g] * (q_g . c[t, g]) + sum_g m[t, g] * sum(q_g)      (S^T = C Q^T; the minima's part is one more product,
+//                                                                               of m and the sums as two f16 numbers each)
+//   sum_t p[t] v[t] = sum_t (p[t] s[t, g]) c[t, g] + sum_t p[t] m[t, g]         (O^T = C^T W, W = p * s in f16; again one more)
 // The query rows are brought to f16 by a power of two of their own (bf16 has 8 bits of precision, f16 11: exact unless 2^-38
-// of the row's largest), products and sums are f32.  W is rounded to f16 once, 2^-11 relative, after a power of two that keeps
-// it in range whatever the scales (vscale below).  The softmax is the one-pass form with a running reference: a warp rescales
-// only when a score exceeds the reference by more than 2^SLACK, so the common step has one vote instead of a reduction.
+// of the row's largest), products and sums are f32.  p and W are rounded to f16, 2^-11 each.  The softmax is the one-pass form
+// with a running reference, kept so that p lies at most at 2^cap, and cap so that W fits f16 whatever the scales: with the
+// largest p near 2^11, weights keep full precision down to 2^-25 of it.  The reference moves only when a p would exceed 2^cap,
+// so the common step has one vote instead of a reduction.
 //
 // Work: a CTA of 4 warps takes one (sequence, kv head, block of 8 or 16 query rows, slice of the keys); each warp streams its
-// own 32-token steps through a ring of three shared-memory stages filled by bulk copies (one lane per 16-token tile looks the
-// page up and issues the copy), so the main loop has no CTA-wide synchronisation.  Warps are joined in shared memory, slices
-// through the workspace by a second kernel (in slice order: the result does not depend on timing).
+// own 64-token steps through two shared-memory stages filled by bulk copies (one lane per 16-token tile issues the copy, the
+// pages of the next 32 tiles are looked up at once), so the main loop has no CTA-wide synchronisation.  Warps are joined in
+// shared memory, slices through the workspace by a second kernel (in slice order: the result does not depend on timing).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/baracuda_kernels_q.h"
 #include "kv4_attention.cuh"
@@ -30,10 +34,17 @@ namespace {
 
 __device__ int g_kv4_attention_device_status = 0;
 
+#ifndef AT_WAVES
+#define AT_WAVES 1
+#endif
+#ifndef AT_MINB
+#define AT_MINB 3
+#endif
 constexpr int AT_WARPS = 4;
-constexpr int AT_STAGES = 3;
-constexpr int AT_STEP = 32;  // tokens of a warp's step
-constexpr float SLACK = 4.0f;
+constexpr int AT_STAGES = 2;
+constexpr int AT_STEP = 64;  // tokens of a warp's step
+constexpr int AT_TILES = AT_STEP / KV4_TILE;
+constexpr float SLACK = 4.0f;  // a new reference leaves this many powers of two before the next
 constexpr int AT_ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -42,6 +53,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -49,7 +70,7 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 }
 template <int D, int NT>
 struct AttnSmem {
-    static constexpr int STAGE = (AT_STEP / KV4_TILE) * kv4_tile_bytes(D);
+    static constexpr int STAGE = AT_TILES * kv4_tile_bytes(D);
     static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
     static constexpr int JOIN = AT_WARPS * 8 * NT * (D + 2) * 4;
     static constexpr int BODY = RING > JOIN ? RING : JOIN;
@@ -59,7 +80,7 @@ struct AttnSmem {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB : 1) kv4_attention_kernel(const __grid_constant__ AttnParams p) {
     using L = AttnSmem<D, NT>;
     constexpr int G = D / KV4_GROUP;
     constexpr int W = D >= 128 ? 2 : 1;       // groups of a 16-byte chunk of keys
@@ -100,43 +121,44 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
     }
     __syncwarp();
 
-    // the lanes that fetch: lane t takes tile t of a step
+    // lane i knows where the i-th of the warp's next 32 tiles lies (-1: nowhere); lanes 0 .. 3 fetch the tiles of a step
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
     const int tiles_per_page = p.cache.page_size / KV4_TILE;
     const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
-    auto tile_of = [&](int step) { return (step0 + step) * (AT_STEP / KV4_TILE) + lane; };
-    auto page_of = [&](int step) {  // -1 where there is nothing to fetch
-        const int t = tile_of(step);
-        if (lane >= AT_STEP / KV4_TILE || step >= my_end || t * KV4_TILE >= hi_all) return -1;
-        const int page = table[t / tiles_per_page];
-        if (page < 0 || page >= p.cache.num_pages) {
-            atomicCAS(&g_kv4_attention_device_status, 0, 404);
-            return -1;
+    int64_t ahead = -1;
+    auto look_up = [&](int k) {  // of this warp's steps k .. k + 7
+        const int step = my_begin + warp + (k + lane / AT_TILES) * AT_WARPS;
+        const int tile = (step0 + step) * AT_TILES + lane % AT_TILES;
+        ahead = -1;
+        if (step < my_end && tile * KV4_TILE < hi_all) {
+            const int at = tile / tiles_per_page, page = table[at];
+            if (page >= 0 && page < p.cache.num_pages) {
+                ahead = static_cast<int64_t>(page) * p.cache.page_stride + (tile - at * tiles_per_page) * TILE;
+            } else {
+                atomicCAS(&g_kv4_attention_device_status, 0, 404);
+            }
         }
-        return page;
     };
-    auto fetch = [&](int step, int page, int stage) {
-        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+    auto fetch = [&](int k, int stage) {  // the warp's k-th step
+        if ((k & 7) == 0) look_up(k);
+        const int64_t where = __shfl_sync(0xffffffffu, ahead, (k & 7) * AT_TILES + (lane & (AT_TILES - 1)));
+        const uint32_t have = __ballot_sync(0xffffffffu, where >= 0) & ((1u << AT_TILES) - 1u);
         if (lane == 0) {
             valid[stage] = have;
             mbar_arrive_expect_tx(&bars[stage], __popc(have) * TILE);
         }
         __syncwarp();
-        if (page >= 0) {
-            bulk_load_1d(ring + stage * L::STAGE + lane * TILE,
-                         head_base + static_cast<int64_t>(page) * p.cache.page_stride + (tile_of(step) % tiles_per_page) * TILE, TILE,
-                         &bars[stage]);
-        }
+        if (lane < AT_TILES && where >= 0) bulk_load_1d(ring + stage * L::STAGE + lane * TILE, head_base + where, TILE, &bars[stage]);
     };
+    const int mine = my_end - my_begin > warp ? (my_end - my_begin - warp + AT_WARPS - 1) / AT_WARPS : 0;  // steps of this warp
 #pragma unroll
-    for (int s = 0; s < AT_STAGES; ++s) {
-        const int step = my_begin + warp + s * AT_WARPS;
-        if (step < my_end) fetch(step, page_of(step), s);
-    }
+    for (int k = 0; k < AT_STAGES; ++k)
+        if (k < mine) fetch(k, k);
 
     // the query rows as B fragments: lane (r, c) holds, of row r of each 8-row block, channels 64 g + 16 c .. + 15
     uint32_t qf[NT][G][8];
-    float qscale[NT][2], qsum[NT][2][G];  // of this lane's score columns 2 c, 2 c + 1
+    uint32_t qsum[NT];    // the sum over group c, as two f16 numbers, for the minima's product
+    float qscale[NT][2];  // of this lane's score columns 2 c, 2 c + 1
     int row_hi[NT][2], row_lo[NT][2];     // keys [lo, hi) that those rows see
     int hi_min = 0x7fffffff, lo_max = 0;  // over the rows that exist: steps inside need no mask
 #pragma unroll
@@ -184,6 +206,14 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
                 qf[nt][g][4 * u + 3] = pack_half2(w[3] * odd, w[7] * odd);
             }
         }
+        {
+            float mine_sum = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) mine_sum = c == g ? sums[g] : mine_sum;
+            mine_sum *= down * 0.0078125f;  // 64 * 2^15 at most: 2^-7 brings it into f16
+            const float high = __half2float(__float2half_rn(mine_sum));
+            qsum[nt] = pack_half2(high, mine_sum - high);
+        }
         const int i = row / p.group;
         const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
         const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
@@ -192,8 +222,6 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
         for (int e = 0; e < 2; ++e) {
             const int from = (2 * c + e) * 4;  // a lane that holds row 2 c + e
             qscale[nt][e] = __shfl_sync(0xffffffffu, up, from) * (16777216.0f * p.scale_log2);
-#pragma unroll
-            for (int g = 0; g < G; ++g) qsum[nt][e][g] = __shfl_sync(0xffffffffu, sums[g], from) * p.scale_log2;
             row_hi[nt][e] = __shfl_sync(0xffffffffu, hi, from);
             row_lo[nt][e] = __shfl_sync(0xffffffffu, lo, from);
         }
@@ -204,65 +232,53 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
         lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
     }
 
-    float acc[NT][MT][4];
-    float l[NT][2], z[NT][2][G], ref[NT][2];
-    float vscale = 1.0f, vbound = 0.0f;  // W = p * s * vscale; s up to vbound keeps it within f16
+    float acc[NT][MT][4], low[NT][4];  // O^T of the codes, and of the minima (row r: group r % G)
+    float l[NT][2], ref[NT][2];
+    bool fresh[NT][2];  // no key seen yet: any reference will do
+    float cap = 15.0f, s_cap = 1.0f;  // p <= 2^cap keeps p and p * s within f16 for s <= s_cap
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low[nt][e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[nt][e] = 0.0f;
-            ref[nt][e] = KV4_NO_REF;
-#pragma unroll
-            for (int g = 0; g < G; ++g) z[nt][e][g] = 0.0f;
-        }
+        for (int e = 0; e < 2; ++e) l[nt][e] = 0.0f, ref[nt][e] = 0.0f, fresh[nt][e] = true;
     }
 
-    uint32_t parity = 0;
-    int stage = 0;
-    bool gave_up = false;
-    int step = my_begin + warp;
-    for (; step < my_end; step += AT_WARPS) {
-        const int ahead = step + AT_STAGES * AT_WARPS;
-        const int next_page = page_of(ahead);  // asked for now, used after this step
-        if (!mbar_try_wait(&bars[stage], parity)) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&bars[stage], parity)) {
-                if (clock64() - t0 > KV4_WAIT_LIMIT) {
-                    gave_up = true;
-                    break;
-                }
-            }
-            gave_up = __any_sync(0xffffffffu, gave_up);
-            if (gave_up) break;
-        }
-        __syncwarp();
-        const uint32_t have = valid[stage];
-        const uint8_t* base = ring + stage * L::STAGE;
-        const int token0 = (step0 + step) * AT_STEP;
-        constexpr int TILES = AT_STEP / KV4_TILE;
-        const bool edge = token0 + AT_STEP > hi_min || token0 < lo_max || have != (1u << TILES) - 1u;
-
-        // scores of both tiles, in units of log2
-        float sc[TILES][NT][4];
-        float sv[TILES][2][G], mv[TILES][2][G];  // the values' scales and minima of tokens r and r + 8
-        float top[NT][2], stop = 0.0f;
+    // x = log2 p of the tiles of a step.  EDGE: some row does not see some key, or a tile is missing.
+    auto weights = [&](auto edge, const uint8_t* base, int token0, uint32_t have, float (&x)[AT_TILES][NT][4], float (&top)[NT][2], uint32_t& s_top) {
+        constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
+        for (int t = 0; t < AT_TILES; ++t) {
             const uint8_t* tile = base + t * TILE;
-            float s[G][NT][4];
+            float s[G][NT][4], m[NT][4];
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 4; ++e) {
+                    m[nt][e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[g][nt][e] = 0.0f;
+                    for (int g = 0; g < G; ++g) s[g][nt][e] = 0.0f;
+                }
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(tile + kv4_pair_offset(D, 0));
+            const uint32_t* vp = reinterpret_cast<const uint32_t*>(tile + kv4_pair_offset(D, 1));
+            {  // the minima, against the sums (zero for c >= G)
+                const int g = c < G ? c : 0;
+                const uint32_t a0 = __byte_perm(kp[r * G + g], 0u, 0x3232), a1 = __byte_perm(kp[(r + 8) * G + g], 0u, 0x3232);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_f16(m[nt], a0, a1, 0u, 0u, c < G ? qsum[nt] : 0u, 0u);
+                // every token and group lies in some lane
+                uint32_t v0 = vp[r * G + g], v1 = vp[(r + 8) * G + g];
+                if constexpr (EDGE) {
+                    const int j = token0 + t * KV4_TILE + r;
+                    if (j >= sq.len || ((have >> t) & 1u) == 0u) v0 = 0u;
+                    if (j + 8 >= sq.len || ((have >> t) & 1u) == 0u) v1 = 0u;
+                }
+                s_top = max_f16x2(s_top, max_f16x2(v0, v1));
+            }
 #pragma unroll
             for (int h = 0; h < G / W; ++h) {
                 uint32_t wa[2 * W], wb[2 * W];
@@ -278,136 +294,113 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
                     wb[0] = bb.x, wb[1] = bb.y;
                 }
 #pragma unroll
-                for (int x = 0; x < 2 * W; ++x) {
-                    const int g = h * W + x / 2, u = x % 2;
-                    const uint32_t a8 = wa[x] >> 8, b8 = wb[x] >> 8;
+                for (int y = 0; y < 2 * W; ++y) {
+                    const int g = h * W + y / 2, u = y % 2;
+                    const uint32_t a8 = wa[y] >> 8, b8 = wb[y] >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16(s[g][nt], wa[x] & 0x000f000fu, wb[x] & 0x000f000fu, wa[x] & 0x00f000f0u, wb[x] & 0x00f000f0u,
+                        mma_f16(s[g][nt], wa[y] & 0x000f000fu, wb[y] & 0x000f000fu, wa[y] & 0x00f000f0u, wb[y] & 0x00f000f0u,
                                 qf[nt][g][4 * u], qf[nt][g][4 * u + 1]);
                         mma_f16(s[g][nt], a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
                                 qf[nt][g][4 * u + 2], qf[nt][g][4 * u + 3]);
                     }
                 }
             }
-            float sk[2][G], mk[2][G];
+            float sk[2][G];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const __half2* kp = reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, 0)) + (r + 8 * e) * G;
-                const __half2* vp = reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, 1)) + (r + 8 * e) * G;
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float2 a = __half22float2(kp[g]), bb = __half22float2(vp[g]);
-                    sk[e][g] = a.x, mk[e][g] = a.y;
-                    sv[t][e][g] = bb.x, mv[t][e][g] = bb.y;
-                }
-            }
+                for (int g = 0; g < G; ++g) sk[e][g] = __low2float(*reinterpret_cast<const __half2*>(kp + (r + 8 * e) * G + g));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float dot = 0.0f, low = 0.0f;
+                    float dot = m[nt][e] * 7.62939453125e-06f;  // 2^-17: in units of 2^-24, as the codes are
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        dot = fmaf(sk[e >> 1][g], s[g][nt][e], dot);
-                        low = fmaf(mk[e >> 1][g], qsum[nt][e & 1][g], low);
-                    }
-                    sc[t][nt][e] = fmaf(dot, qscale[nt][e & 1], low);
+                    for (int g = 0; g < G; ++g) dot = fmaf(sk[e >> 1][g], s[g][nt][e], dot);
+                    x[t][nt][e] = fmaf(dot, qscale[nt][e & 1], -ref[nt][e & 1]);
                 }
-            if (edge) {
+            }
+            if constexpr (EDGE) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int j = token0 + t * KV4_TILE + r + 8 * e;
                     const bool dead = j >= sq.len || ((have >> t) & 1u) == 0u;  // nothing there, whatever the bytes say
+                    uint32_t ones = 0u;  // a value that is no number: rows that see the key become none either
 #pragma unroll
-                    for (int g = 0; g < G; ++g)
-                        if (dead) sv[t][e][g] = 0.0f, mv[t][e][g] = 0.0f;
+                    for (int g = 0; g < G; ++g) ones |= (vp[(r + 8 * e) * G + g] & 0x7c007c00u) + 0x04000400u;
+                    const bool bad = (ones & 0x80008000u) != 0u;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (dead || j >= row_hi[nt][x] || j < row_lo[nt][x]) sc[t][nt][2 * e + x] = -INFINITY;
+                        for (int y = 0; y < 2; ++y) {
+                            float& v = x[t][nt][2 * e + y];
+                            v = dead || j >= row_hi[nt][y] || j < row_lo[nt][y] ? -INFINITY : bad ? NAN : v;
+                        }
                 }
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                top[nt][0] = fmaxf(top[nt][0], fmaxf(sc[t][nt][0], sc[t][nt][2]));
-                top[nt][1] = fmaxf(top[nt][1], fmaxf(sc[t][nt][1], sc[t][nt][3]));
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int g = 0; g < G; ++g) stop = fmaxf(stop, sv[t][e][g]);
-        }
-        bool grow = stop > vbound;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) grow = grow || top[nt][0] > ref[nt][0] + SLACK || top[nt][1] > ref[nt][1] + SLACK;
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                stop = fmaxf(stop, __shfl_xor_sync(0xffffffffu, stop, o));
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
-            }
-            float vmul = 1.0f;
-            if (stop > vbound) {  // W <= 2^SLACK * s * vscale: the largest scale seen goes to [2^10, 2^11)
-                const int ex = 10 - (static_cast<int>(__float_as_uint(stop) >> 23) - 127);
-                const float to = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-                vmul = vbound > 0.0f ? to / vscale : 1.0f;
-                vscale = to;
-                vbound = 2048.0f / to;
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float fix[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float m = fmaxf(ref[nt][e], top[nt][e]);
-                    fix[e] = ex2(ref[nt][e] - m);
-                    ref[nt][e] = m;
-                    l[nt][e] *= fix[e];
-#pragma unroll
-                    for (int g = 0; g < G; ++g) z[nt][e][g] *= fix[e];
-                    fix[e] *= vmul;
-                }
-#pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    acc[nt][j][0] *= fix[0], acc[nt][j][2] *= fix[0];
-                    acc[nt][j][1] *= fix[1], acc[nt][j][3] *= fix[1];
-                }
+                top[nt][0] = fmaxf(fmaxf(top[nt][0], x[t][nt][0]), x[t][nt][2]);
+                top[nt][1] = fmaxf(fmaxf(top[nt][1], x[t][nt][1]), x[t][nt][3]);
             }
         }
+    };
+    auto values = [&](auto edge, const uint8_t* base, int token0, uint32_t have, const float (&x)[AT_TILES][NT][4]) {
+        constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const uint8_t* tile = base + t * TILE + 8 * D;
+        for (int t = 0; t < AT_TILES; ++t) {
+            const uint8_t* tile = base + t * TILE;
+            // (s, m) of the tokens 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c, as pairs of tokens
+            uint32_t sv[2][G], mv[2][G];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t v[2 * G];
+                const uint8_t* at = tile + kv4_pair_offset(D, 1) + (2 * c + 8 * e) * G * 4;
+                if constexpr (G == 1) {
+                    const uint2 y = *reinterpret_cast<const uint2*>(at);
+                    v[0] = y.x, v[1] = y.y;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < G / 2; ++q) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(at + 16 * q);
+                        v[4 * q] = y.x, v[4 * q + 1] = y.y, v[4 * q + 2] = y.z, v[4 * q + 3] = y.w;
+                    }
+                }
+                if constexpr (EDGE) {  // zeros for what is not there or no number
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t ones = 0u;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) ones |= (v[G * q + g] & 0x7c007c00u) + 0x04000400u;
+                        const bool gone = token0 + t * KV4_TILE + 2 * c + 8 * e + q >= sq.len || ((have >> t) & 1u) == 0u || (ones & 0x80008000u) != 0u;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) v[G * q + g] = gone ? 0u : v[G * q + g];
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) sv[e][g] = __byte_perm(v[g], v[G + g], 0x5410), mv[e][g] = __byte_perm(v[g], v[G + g], 0x7632);
+            }
+            uint32_t m0 = mv[0][0], m1 = mv[1][0];  // row r of the minima's product is group r % G
+#pragma unroll
+            for (int g = 1; g < G; ++g) m0 = (r & (G - 1)) == g ? mv[0][g] : m0, m1 = (r & (G - 1)) == g ? mv[1][g] : m1;
             uint32_t wf[NT][G][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float pr[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    pr[e] = ex2(sc[t][nt][e] - ref[nt][e & 1]);
+                    pr[e] = ex2(x[t][nt][e]);
                     l[nt][e & 1] += pr[e];
                 }
+                const uint32_t b0 = movmatrix_trans(pack_half2(pr[0], pr[1])), b1 = movmatrix_trans(pack_half2(pr[2], pr[3]));
+                mma_f16(low[nt], m0, 0u, m1, 0u, b0, b1);
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float sw = sv[t][e >> 1][g], mw = mv[t][e >> 1][g];
-                        if (edge && sc[t][nt][e] == -INFINITY) sw = 0.0f, mw = 0.0f;  // a key this row does not see may hold anything
-                        w[e] = pr[e] * (sw * vscale);
-                        z[nt][e & 1][g] = fmaf(pr[e], mw, z[nt][e & 1][g]);
-                    }
-                    wf[nt][g][0] = movmatrix_trans(pack_half2(w[0], w[1]));
-                    wf[nt][g][1] = movmatrix_trans(pack_half2(w[2], w[3]));
-                }
+                for (int g = 0; g < G; ++g) wf[nt][g][0] = mul_f16x2(b0, sv[0][g]), wf[nt][g][1] = mul_f16x2(b1, sv[1][g]);
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
+                const uint4 v = *reinterpret_cast<const uint4*>(tile + 8 * D + g * 512 + lane * 16);
                 const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -419,8 +412,85 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
                 }
             }
         }
+    };
+
+    uint32_t parity = 0;
+    int stage = 0, k = 0;
+    bool gave_up = false;
+    for (; k < mine; ++k) {
+        if (!mbar_try_wait(&bars[stage], parity)) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&bars[stage], parity)) {
+                if (clock64() - t0 > KV4_WAIT_LIMIT) {
+                    gave_up = true;
+                    break;
+                }
+            }
+        }
+        gave_up = __any_sync(0xffffffffu, gave_up);
+        if (gave_up) break;
+        const uint32_t have = valid[stage];
+        const uint8_t* base = ring + stage * L::STAGE;
+        const int token0 = (step0 + my_begin + warp + k * AT_WARPS) * AT_STEP;
+        const bool edge = token0 + AT_STEP > hi_min || token0 < lo_max || have != (1u << AT_TILES) - 1u;
+
+        float x[AT_TILES][NT][4], top[NT][2];
+        uint32_t s_top = 0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+        if (edge) {
+            weights(std::true_type{}, base, token0, have, x, top, s_top);
+        } else {
+            weights(std::false_type{}, base, token0, have, x, top, s_top);
+        }
+        float largest = __low2float(*reinterpret_cast<const __half2*>(&s_top));
+        bool grow = largest > s_cap;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) grow = grow || fresh[nt][0] || fresh[nt][1] || top[nt][0] > cap || top[nt][1] > cap;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], o));
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            if (largest > s_cap && largest < INFINITY) {  // the scale's power of two comes off the cap
+                const int ex = static_cast<int>(__float_as_uint(largest) >> 23) - 126;
+                cap = static_cast<float>(15 - ex);
+                s_cap = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float fix[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const bool move = top[nt][e] > cap || (fresh[nt][e] && top[nt][e] > -INFINITY);
+                    const float by = move ? top[nt][e] - (cap - SLACK) : 0.0f;
+                    fix[e] = fresh[nt][e] ? 1.0f : ex2(-by);  // nothing to rescale before the first key
+                    fresh[nt][e] = fresh[nt][e] && !move;
+                    ref[nt][e] += by;
+                    l[nt][e] *= fix[e];
+#pragma unroll
+                    for (int t = 0; t < AT_TILES; ++t) x[t][nt][e] -= by, x[t][nt][2 + e] -= by;
+                }
+                low[nt][0] *= fix[0], low[nt][1] *= fix[1];
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    acc[nt][j][0] *= fix[0], acc[nt][j][2] *= fix[0];
+                    acc[nt][j][1] *= fix[1], acc[nt][j][3] *= fix[1];
+                }
+            }
+        }
+        if (edge) {
+            values(std::true_type{}, base, token0, have, x);
+        } else {
+            values(std::false_type{}, base, token0, have, x);
+        }
         __syncwarp();
-        if (ahead < my_end) fetch(ahead, next_page, stage);
+        if (k + AT_STAGES < mine) fetch(k + AT_STAGES, stage);
         if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
     }
     if (gave_up) {
@@ -428,7 +498,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
         // copies of this warp may still be in flight into its ring: wait for them, again within a limit
         const long long t0 = clock64();
         for (int s = 0; s < AT_STAGES; ++s) {
-            if (step + s * AT_WARPS >= my_end) break;
+            if (k + s >= mine) break;
             while (!mbar_try_wait(&bars[stage], parity) && clock64() - t0 < KV4_WAIT_LIMIT) {
             }
             if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
@@ -436,32 +506,30 @@ __global__ void __launch_bounds__(AT_WARPS * 32) kv4_attention_kernel(const __gr
     }
 
     // join the lanes, then the warps
+    float z[NT][2][G];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
+            for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
 #pragma unroll
-                for (int g = 0; g < G; ++g) z[nt][e][g] += __shfl_xor_sync(0xffffffffu, z[nt][e][g], o);
-            }
+            for (int g = 0; g < G; ++g) z[nt][e][g] = __shfl_sync(0xffffffffu, low[nt][e], g * 4 + c);
         }
     __syncthreads();  // every warp has left its ring
     float* join = reinterpret_cast<float*>(smem);  // [warp][row][D], then [warp][row] (ref, l)
     float2* join_ml = reinterpret_cast<float2*>(join + AT_WARPS * ROWS * D);
-    const float unit = 16777216.0f / vscale;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float* row = join + (warp * ROWS + nt * 8 + 2 * c + e) * D;
 #pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                row[16 * j + r] = fmaf(acc[nt][j][e], unit, z[nt][e][j / 4]);
-                row[16 * j + 8 + r] = fmaf(acc[nt][j][2 + e], unit * 0.0625f, z[nt][e][j / 4]);
+            for (int j = 0; j < MT; ++j) {  // codes were 2^-24 and 2^-20
+                row[16 * j + r] = fmaf(acc[nt][j][e], 16777216.0f, z[nt][e][j / 4]);
+                row[16 * j + 8 + r] = fmaf(acc[nt][j][2 + e], 1048576.0f, z[nt][e][j / 4]);
             }
-            if (r == 0) join_ml[warp * ROWS + nt * 8 + 2 * c + e] = make_float2(ref[nt][e], l[nt][e]);
+            if (r == 0) join_ml[warp * ROWS + nt * 8 + 2 * c + e] = make_float2(fresh[nt][e] ? KV4_NO_REF : ref[nt][e], l[nt][e]);
         }
     __syncthreads();
     for (int at = threadIdx.x; at < rows * (D / 4); at += AT_WARPS * 32) {
@@ -520,19 +588,35 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     float sum = 0.0f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t slot = slot0 + static_cast<int64_t>(s) * rows_of_tile;
-        const float2 ml = p.part_ml[slot];
-        const float f = ex2(ml.x - m);
-        sum = fmaf(ml.y, f, sum);
-        const float* o = p.part_o + slot * D + lane * PER;
+    const float* from = p.part_o + slot0 * D + lane * PER;
+    const int64_t step = static_cast<int64_t>(rows_of_tile) * D;
+    for (int s0 = 0; s0 < p.splits; s0 += 32) {  // lane i weighs slice s0 + i
+        float f = 0.0f;
+        if (s0 + lane < p.splits) {
+            const float2 ml = p.part_ml[slot0 + static_cast<int64_t>(s0 + lane) * rows_of_tile];
+            f = ex2(ml.x - m);
+            sum = fmaf(ml.y, f, sum);
+        }
+        const int n = min(32, p.splits - s0);
+        for (int s1 = 0; s1 < n; s1 += 8) {  // eight slices in flight
+            float2 x[8][PER / 2];
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(o + e);
-            acc[e] = fmaf(x.x, f, acc[e]);
-            acc[e + 1] = fmaf(x.y, f, acc[e + 1]);
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int e = 0; e < PER / 2; ++e)
+                    x[s][e] = s1 + s < n ? *reinterpret_cast<const float2*>(from + (s0 + s1 + s) * step + 2 * e) : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const float w = __shfl_sync(0xffffffffu, f, (s1 + s) & 31);
+#pragma unroll
+                for (int e = 0; e < PER / 2; ++e) {
+                    if (s1 + s < n) acc[2 * e] = fmaf(x[s][e].x, w, acc[2 * e]), acc[2 * e + 1] = fmaf(x[s][e].y, w, acc[2 * e + 1]);
+                }
+            }
         }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int64_t q_row = sq.row0 + gr / p.group;
     const int head = hk * p.group + gr % p.group;
@@ -558,8 +642,8 @@ AttnShape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q
         most = max_kv / 512;
     } else {
         const int64_t steps = (max_kv + AT_STEP * AT_WARPS - 1) / (AT_STEP * AT_WARPS);  // of a CTA
-        want = (AT_ASSUMED_SMS * 8 + s.tiles - 1) / (s.tiles > 0 ? s.tiles : 1);
-        most = (steps + 1) / 2;
+        want = AT_ASSUMED_SMS * 3 * AT_WAVES / (s.tiles > 0 ? s.tiles : 1);
+        most = steps;
     }
     s.splits = static_cast<int>(want < most ? want : most);
     if (s.splits < 1) s.splits = 1;
