@@ -30,6 +30,7 @@ struct AttnParams {
     int32_t row_tiles, splits, tile_rows;  // blocks of query rows of a kv head, slices of the keys, rows of a block
     float* part_o;   // [tile][split][rows][D]
     float2* part_ml; // [tile][split][rows]
+    int2* shares;    // null, or of each block of rows: place of its first part, CTA of its last; part_o is then [CTA][2][rows][D]
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -65,7 +66,8 @@ struct AttnShape {
     int tensor;     // 1: kv4_prompt_sm100a.cu, 0: kv4_attention_sm100a.cu
     int tile_rows;  // 8 or 16; 128 or 256
     int row_tiles, splits;
-    int64_t tiles;
+    int64_t tiles, ctas;
+    bool joined;    // a second kernel adds parts of blocks
 };
 int32_t launch_kv4_prompt(AttnParams& p, const AttnShape& s, cudaStream_t stream);
 int32_t read_and_clear_kv4_prompt_device_status();

@@ -14,10 +14,12 @@
 // largest p near 2^11, weights keep full precision down to 2^-25 of it.  The reference moves only when a p would exceed 2^cap,
 // so the common step has one vote instead of a reduction.
 //
-// Work: a CTA of 4 warps takes one (sequence, kv head, block of 8 or 16 query rows, slice of the keys); each warp streams its
-// own 64-token steps through two shared-memory stages filled by bulk copies (one lane per 16-token tile issues the copy, the
-// pages of the next 32 tiles are looked up at once), so the main loop has no CTA-wide synchronisation.  Warps are joined in
-// shared memory, slices through the workspace by a second kernel (in slice order: the result does not depend on timing).
+// Work: as many CTAs of 4 warps as are resident at once share the launch's work equally, whatever the lengths of its sequences:
+// each takes a run of blocks of 8 or 16 query rows of a kv head, the first and the last perhaps in part.  Each warp streams its
+// own 64-token steps (32 where D is 256) through two shared-memory stages filled by bulk copies (one lane per 16-token tile
+// issues the copy, the pages of the next 32 tiles are looked up at once), so the main loop has no CTA-wide synchronisation.
+// Warps are joined in shared memory, parts of a block through the workspace by a second kernel (in the order of the keys: the
+// result does not depend on timing).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,16 +36,13 @@ namespace {
 
 __device__ int g_kv4_attention_device_status = 0;
 
-#ifndef AT_WAVES
-#define AT_WAVES 1
-#endif
-#ifndef AT_MINB
-#define AT_MINB 3
-#endif
 constexpr int AT_WARPS = 4;
-constexpr int AT_STAGES = 2;
-constexpr int AT_STEP = 64;  // tokens of a warp's step
-constexpr int AT_TILES = AT_STEP / KV4_TILE;
+constexpr int AT_BLOCK_UNITS = 2;  // look-ups, queries and join of a block take the time of about two units
+constexpr int AT_STAGES = 2;  // the parts of a CTA alternate between them: not another number
+#ifndef AT_MOST_ROWS
+#define AT_MOST_ROWS 64
+#define AT_MOST_ROWS_256 32
+#endif
 constexpr float SLACK = 4.0f;  // a new reference leaves this many powers of two before the next
 constexpr int AT_ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
 
@@ -69,18 +68,45 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     return r;
 }
 template <int D, int NT>
+struct AttnCfg {
+    static constexpr int TILES = D == 256 ? 2 : 4;           // of 16 tokens, of a warp's step
+    static constexpr int STEP = TILES * KV4_TILE;
+    static constexpr int RESIDENT = NT == 2 || D == 256 ? 2 : D == 128 ? 3 : 4;  // CTAs of an SM (registers, shared memory)
+};
+template <int D, int NT>
 struct AttnSmem {
+    static constexpr int AT_TILES = AttnCfg<D, NT>::TILES;
     static constexpr int STAGE = AT_TILES * kv4_tile_bytes(D);
-    static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;
+    static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;  // [stage][warp]: the join takes the place of one stage
     static constexpr int JOIN = AT_WARPS * 8 * NT * (D + 2) * 4;
-    static constexpr int BODY = RING > JOIN ? RING : JOIN;
-    static constexpr int BARS = BODY;
+    static_assert(JOIN <= AT_WARPS * STAGE, "the join fits one stage");
+    static constexpr int BARS = RING;
     static constexpr int VALID = BARS + AT_WARPS * AT_STAGES * 8;
-    static constexpr int TOTAL = VALID + AT_WARPS * AT_STAGES * 4;
+    static constexpr int SCAN = VALID + AT_WARPS * AT_STAGES * 4;  // sums of the warps, then what the scan found
+    static constexpr int TOTAL = SCAN + (AT_WARPS + 4) * 8;
 };
 
+// What a sequence asks for: blocks of rows, the warp steps from the first row's first key to the last row's last, units of a block
+// (AT_BLOCK_UNITS of them for what a block costs apart from its keys: they come first, without keys).
+struct Extent {
+    Sequence sq;
+    int blocks, step0, steps, units;
+};
+template <int STEP, int ROWS>
+__device__ __forceinline__ Extent extent_of(const AttnParams& p, int b) {
+    Extent x;
+    x.sq = sequence_of(p, b, &g_kv4_attention_device_status);
+    x.blocks = (x.sq.n * p.group + ROWS - 1) / ROWS;
+    const int first = x.sq.len - x.sq.n;
+    const int hi = max(0, p.causal ? min(x.sq.len, first + x.sq.n) : x.sq.len), lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    x.step0 = lo / STEP;
+    x.steps = max(0, (hi + STEP - 1) / STEP - x.step0);
+    x.units = AT_BLOCK_UNITS + max(1, (x.steps + AT_WARPS - 1) / AT_WARPS);  // rows without keys are to be written too
+    return x;
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB : 1) kv4_attention_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_attention_kernel(const __grid_constant__ AttnParams p) {
     using L = AttnSmem<D, NT>;
     constexpr int G = D / KV4_GROUP;
     constexpr int W = D >= 128 ? 2 : 1;       // groups of a 16-byte chunk of keys
@@ -90,30 +116,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 
-    int id = blockIdx.x;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int tile_id = id;
-    const int rt = id % p.row_tiles;
-    id /= p.row_tiles;
-    const int hk = id % p.cache.heads_kv, b = id / p.cache.heads_kv;
-    const Sequence sq = sequence_of(p, b, &g_kv4_attention_device_status);
-    const int rows = min(ROWS, sq.n * p.group - rt * ROWS);  // row = query index * group + head in group
-    if (rows <= 0) return;
-
-    // keys that any row of this block sees, and this CTA's slice of them, in steps
-    const int i_first = rt * ROWS / p.group, i_last = (rt * ROWS + rows - 1) / p.group;
-    const int past = sq.len - sq.n;  // the last key that query row i sees is past + i when causal
-    int hi_all = p.causal ? min(sq.len, past + i_last + 1) : sq.len;
-    int lo_all = p.window > 0 ? max(0, past + i_first - p.window + 1) : 0;
-    hi_all = max(hi_all, 0);
-    const int step0 = lo_all / AT_STEP, steps = max(0, (hi_all + AT_STEP - 1) / AT_STEP - step0);
-    const int per = (steps + p.splits - 1) / p.splits;
-    const int my_begin = min(split * per, steps), my_end = min(my_begin + per, steps);
+    constexpr int AT_TILES = AttnCfg<D, NT>::TILES, AT_STEP = AttnCfg<D, NT>::STEP;
 
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS) + warp * AT_STAGES;
     volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::VALID) + warp * AT_STAGES;
-    uint8_t* ring = smem + warp * AT_STAGES * L::STAGE;
+    uint8_t* ring = smem + warp * L::STAGE;  // stages AT_WARPS * STAGE apart
     if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < AT_STAGES; ++s) mbar_init(&bars[s], 1);
@@ -121,39 +128,129 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
     }
     __syncwarp();
 
-    // lane i knows where the i-th of the warp's next 32 tiles lies (-1: nowhere); lanes 0 .. 3 fetch the tiles of a step
-    const int32_t* table = p.table + static_cast<int64_t>(b) * p.ld_table;
+    // This CTA's share: of the launch's units (256 tokens of one block of rows and kv head; 128 where D is 256), numbered over
+    // sequences, kv heads, blocks of rows and tokens, an equal part in a row.  Its ends may lie inside a block: the parts of such a
+    // block are joined by the second kernel.
+    auto units_of = [&](int b_) -> int64_t {
+        if (b_ >= p.batch) return 0;
+        const Extent x = extent_of<AT_STEP, ROWS>(p, b_);
+        return static_cast<int64_t>(x.blocks) * p.cache.heads_kv * x.units;
+    };
+    int64_t* scan = reinterpret_cast<int64_t*>(smem + L::SCAN);  // [AT_WARPS] sums, then sequence and the units before it
+    const int64_t mine0 = units_of(threadIdx.x);                 // of the first 128 sequences, often all
+    int64_t total = mine0;
+    for (int x = threadIdx.x + AT_WARPS * 32; x < p.batch; x += AT_WARPS * 32) total += units_of(x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) scan[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < AT_WARPS; ++w) total += scan[w];
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);  // none without a unit: parts are counted by CTAs
+    if (blockIdx.x >= ctas) return;
+    int64_t unit = blockIdx.x * total / ctas;
+    const int64_t unit_end = (blockIdx.x + 1) * total / ctas;
+    int64_t before = 0;
+    for (int x0 = 0;; x0 += AT_WARPS * 32) {
+        int64_t sum = x0 == 0 ? mine0 : units_of(x0 + threadIdx.x);
+        const int64_t own = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = sum;
+        __syncthreads();
+        int64_t chunk = 0;
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) {
+            if (w < warp) sum += scan[w];
+            chunk += scan[w];
+        }
+        if (before + sum - own <= unit && unit < before + sum) scan[AT_WARPS] = x0 + threadIdx.x, scan[AT_WARPS + 1] = before + sum - own;
+        if (unit < before + chunk) break;
+        before += chunk;
+    }
+    __syncthreads();
+    int b = static_cast<int>(scan[AT_WARPS]);
+    before = scan[AT_WARPS + 1];
+    Extent xt = extent_of<AT_STEP, ROWS>(p, b);
+    uint32_t phases = 0;  // bit s: the phase that stage s is waited for next; every part begins with stage 0
+    bool at_start = true;
+
+    // a block of rows, or the part of one that falls to this CTA
+    struct Part {
+        int b, hk, rt, unit0, unit1, units;  // units with keys: [unit0, unit1) of `units`
+        int64_t begin;                       // number of the block's first unit
+        Sequence sq;
+        int step0, my_begin, my_end, hi_all, mine;
+    };
+    // the next part of this CTA from `unit` on that has keys (or is a block without any); false at the end
+    auto next_part = [&](Part& t) {
+        while (unit < unit_end) {
+            while (unit >= before + static_cast<int64_t>(xt.blocks) * p.cache.heads_kv * xt.units) {
+                before += static_cast<int64_t>(xt.blocks) * p.cache.heads_kv * xt.units;
+                xt = extent_of<AT_STEP, ROWS>(p, ++b);
+            }
+            const int64_t in_seq = unit - before;
+            const int block = static_cast<int>(in_seq / xt.units), at = static_cast<int>(in_seq - static_cast<int64_t>(block) * xt.units);
+            const int to = static_cast<int>(min(static_cast<int64_t>(xt.units), at + (unit_end - unit)));
+            t.begin = unit - at;
+            unit += to - at;
+            t.units = xt.units - AT_BLOCK_UNITS;
+            t.unit0 = max(0, at - AT_BLOCK_UNITS), t.unit1 = max(0, to - AT_BLOCK_UNITS);
+            if (t.unit0 == t.unit1) continue;
+            t.b = b, t.hk = block / xt.blocks, t.rt = block - t.hk * xt.blocks;
+            t.sq = xt.sq;
+            const int last_row = min(ROWS, t.sq.n * p.group - t.rt * ROWS) - 1 + t.rt * ROWS;
+            t.hi_all = max(0, p.causal ? min(t.sq.len, t.sq.len - t.sq.n + last_row / p.group + 1) : t.sq.len);
+            t.step0 = xt.step0, t.my_begin = t.unit0 * AT_WARPS, t.my_end = min(t.unit1 * AT_WARPS, xt.steps);
+            t.mine = t.my_end - t.my_begin > warp ? (t.my_end - t.my_begin - warp + AT_WARPS - 1) / AT_WARPS : 0;  // steps of this warp
+            return true;
+        }
+        return false;
+    };
+    // lane i knows where the i-th of the warp's next 32 tiles lies (-1: nowhere); the first lanes fetch the tiles of a step
     const int tiles_per_page = p.cache.page_size / KV4_TILE;
-    const uint8_t* head_base = p.cache.base + static_cast<int64_t>(hk) * tiles_per_page * TILE;
     int64_t ahead = -1;
-    auto look_up = [&](int k) {  // of this warp's steps k .. k + 7
-        const int step = my_begin + warp + (k + lane / AT_TILES) * AT_WARPS;
-        const int tile = (step0 + step) * AT_TILES + lane % AT_TILES;
+    constexpr int LOOK = 32 / AT_TILES;
+    auto look_up = [&](const Part& t, int k) {  // of this warp's steps k .. k + LOOK - 1
+        const int step = t.my_begin + warp + (k + lane / AT_TILES) * AT_WARPS;
+        const int tile = (t.step0 + step) * AT_TILES + lane % AT_TILES;
         ahead = -1;
-        if (step < my_end && tile * KV4_TILE < hi_all) {
-            const int at = tile / tiles_per_page, page = table[at];
+        if (step < t.my_end && tile * KV4_TILE < t.hi_all) {
+            const int at = tile / tiles_per_page, page = p.table[static_cast<int64_t>(t.b) * p.ld_table + at];
             if (page >= 0 && page < p.cache.num_pages) {
-                ahead = static_cast<int64_t>(page) * p.cache.page_stride + (tile - at * tiles_per_page) * TILE;
+                ahead = static_cast<int64_t>(page) * p.cache.page_stride + (static_cast<int64_t>(t.hk) * tiles_per_page + tile - at * tiles_per_page) * TILE;
             } else {
                 atomicCAS(&g_kv4_attention_device_status, 0, 404);
             }
         }
     };
-    auto fetch = [&](int k, int stage) {  // the warp's k-th step
-        if ((k & 7) == 0) look_up(k);
-        const int64_t where = __shfl_sync(0xffffffffu, ahead, (k & 7) * AT_TILES + (lane & (AT_TILES - 1)));
+    auto fetch = [&](const Part& t, int k, int to_stage) {  // the warp's k-th step
+        if (k % LOOK == 0) look_up(t, k);
+        const int64_t where = __shfl_sync(0xffffffffu, ahead, k % LOOK * AT_TILES + (lane & (AT_TILES - 1)));
         const uint32_t have = __ballot_sync(0xffffffffu, where >= 0) & ((1u << AT_TILES) - 1u);
         if (lane == 0) {
-            valid[stage] = have;
-            mbar_arrive_expect_tx(&bars[stage], __popc(have) * TILE);
+            valid[to_stage] = have;
+            mbar_arrive_expect_tx(&bars[to_stage], __popc(have) * TILE);
         }
         __syncwarp();
-        if (lane < AT_TILES && where >= 0) bulk_load_1d(ring + stage * L::STAGE + lane * TILE, head_base + where, TILE, &bars[stage]);
+        if (lane < AT_TILES && where >= 0) bulk_load_1d(ring + to_stage * (AT_WARPS * L::STAGE) + lane * TILE, p.cache.base + where, TILE, &bars[to_stage]);
     };
-    const int mine = my_end - my_begin > warp ? (my_end - my_begin - warp + AT_WARPS - 1) / AT_WARPS : 0;  // steps of this warp
-#pragma unroll
-    for (int k = 0; k < AT_STAGES; ++k)
-        if (k < mine) fetch(k, k);
+
+    Part now;
+    if (!next_part(now)) return;
+    if (now.mine > 0) fetch(now, 0, 0);
+    for (;;) {
+    const Sequence sq = now.sq;
+    const int hk = now.hk, rt = now.rt, step0 = now.step0, my_begin = now.my_begin, mine = now.mine;
+    const int rows = min(ROWS, sq.n * p.group - rt * ROWS);  // row = query index * group + head in group
+    const int past = sq.len - sq.n;                          // the last key that query row i sees is past + i when causal
+    if (mine > 1) fetch(now, 1, 1);  // the first step is on its way
+    int stage = 0;
 
     // the query rows as B fragments: lane (r, c) holds, of row r of each 8-row block, channels 64 g + 16 c .. + 15
     uint32_t qf[NT][G][8];
@@ -249,7 +346,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
     }
 
     // x = log2 p of the tiles of a step.  EDGE: some row does not see some key, or a tile is missing.
-    auto weights = [&](auto edge, const uint8_t* base, int token0, uint32_t have, float (&x)[AT_TILES][NT][4], float (&top)[NT][2], uint32_t& s_top) {
+    auto weights = [&](auto edge, const uint8_t* base, int token0, uint32_t have, auto& x, float (&top)[NT][2], uint32_t& s_top) {
         constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
         for (int t = 0; t < AT_TILES; ++t) {
@@ -346,7 +443,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
             }
         }
     };
-    auto values = [&](auto edge, const uint8_t* base, int token0, uint32_t have, const float (&x)[AT_TILES][NT][4]) {
+    auto values = [&](auto edge, const uint8_t* base, int token0, uint32_t have, const auto& x) {
         constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
         for (int t = 0; t < AT_TILES; ++t) {
@@ -414,10 +511,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
         }
     };
 
-    uint32_t parity = 0;
-    int stage = 0, k = 0;
+    int k = 0;
     bool gave_up = false;
     for (; k < mine; ++k) {
+        const uint32_t parity = (phases >> stage) & 1u;
         if (!mbar_try_wait(&bars[stage], parity)) {
             const long long t0 = clock64();
             while (!mbar_try_wait(&bars[stage], parity)) {
@@ -430,7 +527,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
         gave_up = __any_sync(0xffffffffu, gave_up);
         if (gave_up) break;
         const uint32_t have = valid[stage];
-        const uint8_t* base = ring + stage * L::STAGE;
+        const uint8_t* base = ring + stage * (AT_WARPS * L::STAGE);
         const int token0 = (step0 + my_begin + warp + k * AT_WARPS) * AT_STEP;
         const bool edge = token0 + AT_STEP > hi_min || token0 < lo_max || have != (1u << AT_TILES) - 1u;
 
@@ -490,8 +587,9 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
             values(std::false_type{}, base, token0, have, x);
         }
         __syncwarp();
-        if (k + AT_STAGES < mine) fetch(k + AT_STAGES, stage);
-        if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
+        if (k + AT_STAGES < mine) fetch(now, k + AT_STAGES, stage);
+        phases ^= 1u << stage;
+        stage ^= 1;
     }
     if (gave_up) {
         if (lane == 0) atomicCAS(&g_kv4_attention_device_status, 0, 411);
@@ -499,9 +597,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
         const long long t0 = clock64();
         for (int s = 0; s < AT_STAGES; ++s) {
             if (k + s >= mine) break;
-            while (!mbar_try_wait(&bars[stage], parity) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            while (!mbar_try_wait(&bars[stage], (phases >> stage) & 1u) && clock64() - t0 < KV4_WAIT_LIMIT) {
             }
-            if (++stage == AT_STAGES) stage = 0, parity ^= 1u;
+            phases ^= 1u << stage;
+            stage ^= 1;
         }
     }
 
@@ -516,8 +615,13 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
 #pragma unroll
             for (int g = 0; g < G; ++g) z[nt][e][g] = __shfl_sync(0xffffffffu, low[nt][e], g * 4 + c);
         }
+    // the next part's first step goes to stage 0, the join to the place of stage 1
+    Part then;
+    const bool more = next_part(then);
+    fence_proxy_async_smem();
     __syncthreads();  // every warp has left its ring
-    float* join = reinterpret_cast<float*>(smem);  // [warp][row][D], then [warp][row] (ref, l)
+    if (more && then.mine > 0 && !gave_up) fetch(then, 0, 0);
+    float* join = reinterpret_cast<float*>(smem + AT_WARPS * L::STAGE);  // [warp][row][D], then [warp][row] (ref, l)
     float2* join_ml = reinterpret_cast<float2*>(join + AT_WARPS * ROWS * D);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -532,6 +636,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
             if (r == 0) join_ml[warp * ROWS + nt * 8 + 2 * c + e] = make_float2(fresh[nt][e] ? KV4_NO_REF : ref[nt][e], l[nt][e]);
         }
     __syncthreads();
+    const bool whole = now.unit0 == 0 && now.unit1 == now.units;
     for (int at = threadIdx.x; at < rows * (D / 4); at += AT_WARPS * 32) {
         const int row = at / (D / 4), d = at % (D / 4) * 4;
         float m = KV4_NO_REF;
@@ -547,7 +652,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
             sum = fmaf(ml.y, f, sum);
             o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
         }
-        if (p.splits == 1) {
+        if (whole) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const int gr = rt * ROWS + row;
             const int64_t q_row = sq.row0 + gr / p.group;
@@ -557,17 +662,40 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D <= 128 && NT == 1 ? AT_MINB :
                 make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&bb));
             if (p.lse != nullptr && d == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
         } else {
-            const int64_t slot = (static_cast<int64_t>(tile_id) * p.splits + split) * ROWS + row;
+            const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (at_start ? 0 : 1)) * ROWS + row;
             *reinterpret_cast<float4*>(p.part_o + slot * D + d) = o;
             if (d == 0) p.part_ml[slot] = make_float2(m, sum);
         }
     }
+    // the CTA with a block's first unit says who has the others (parts of a CTA's first block are in its first place, of its last
+    // in its second)
+    if (now.unit0 == 0 && threadIdx.x == 0 && p.shares != nullptr) {
+        const int64_t tile_id = (static_cast<int64_t>(now.b) * p.cache.heads_kv + hk) * p.row_tiles + rt;
+        const int64_t last = ((now.begin + AT_BLOCK_UNITS + now.units) * ctas - 1) / total;  // the CTA of the block's last unit
+        p.shares[tile_id] = make_int2(2 * blockIdx.x + (at_start ? 0 : 1), static_cast<int>(last));
+    }
+    // a warp that gave up has no copy in flight; the others may have one, which its own barrier waits for at the end
+    if (__syncthreads_or(gave_up)) {
+        if (more && then.mine > 0 && !gave_up) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&bars[0], phases & 1u) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            }
+        }
+        return;
+    }
+    if (!more) return;
+    at_start = false;
+    now = then;
+    fence_proxy_async_smem();  // the join's place is read; copies may follow
+    __syncthreads();
+    }
 }
 
-// Adds the slices of one block of rows, in slice order.  One warp per row.
+// Adds the parts of one block of rows, in the order of the keys.  One warp per row; launched to start while the kernel before it ends.
 template <int D>
 __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_constant__ AttnParams p) {
     const int rows_of_tile = p.tile_rows;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int row = static_cast<int>(id % rows_of_tile);
@@ -579,32 +707,39 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     const Sequence sq = sequence_of(p, b, &g_kv4_attention_device_status);
     const int gr = rt * rows_of_tile + row;
     if (gr >= sq.n * p.group) return;
-    const int64_t slot0 = tile_id * p.splits * rows_of_tile + row;
+    // where the block's parts are: in slices of its own, or in the places of the CTAs that shared it
+    int parts = p.splits;
+    int64_t first = tile_id * p.splits, second = first + 1, stride = 1;
+    if (p.shares != nullptr) {
+        const int2 share = p.shares[tile_id];
+        parts = share.y - share.x / 2 + 1;
+        if (parts == 1) return;
+        first = share.x, second = share.x / 2 * 2 + 2, stride = 2;
+    }
+    auto place = [&](int s) { return (s == 0 ? first : second + (s - 1) * stride) * rows_of_tile + row; };
     float m = KV4_NO_REF;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[slot0 + static_cast<int64_t>(s) * rows_of_tile].x);
+    for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.part_ml[place(s)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     constexpr int PER = D / 32;
     float sum = 0.0f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.0f;
-    const float* from = p.part_o + slot0 * D + lane * PER;
-    const int64_t step = static_cast<int64_t>(rows_of_tile) * D;
-    for (int s0 = 0; s0 < p.splits; s0 += 32) {  // lane i weighs slice s0 + i
+    for (int s0 = 0; s0 < parts; s0 += 32) {  // lane i weighs slice s0 + i
         float f = 0.0f;
-        if (s0 + lane < p.splits) {
-            const float2 ml = p.part_ml[slot0 + static_cast<int64_t>(s0 + lane) * rows_of_tile];
+        if (s0 + lane < parts) {
+            const float2 ml = p.part_ml[place(s0 + lane)];
             f = ex2(ml.x - m);
             sum = fmaf(ml.y, f, sum);
         }
-        const int n = min(32, p.splits - s0);
+        const int n = min(32, parts - s0);
         for (int s1 = 0; s1 < n; s1 += 8) {  // eight slices in flight
             float2 x[8][PER / 2];
 #pragma unroll
             for (int s = 0; s < 8; ++s)
 #pragma unroll
                 for (int e = 0; e < PER / 2; ++e)
-                    x[s][e] = s1 + s < n ? *reinterpret_cast<const float2*>(from + (s0 + s1 + s) * step + 2 * e) : make_float2(0.0f, 0.0f);
+                    x[s][e] = s1 + s < n ? *reinterpret_cast<const float2*>(p.part_o + place(s0 + s1 + s) * D + lane * PER + 2 * e) : make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 const float w = __shfl_sync(0xffffffffu, f, (s1 + s) & 31);
@@ -626,29 +761,34 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     if (p.lse != nullptr && lane == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Which kernel and how the work is cut.  Up to 16 rows of a kv head the codes go to mma.sync as they are (8 rows where D is 256: its
-// accumulators take the registers); beyond, keys and values are brought to f16 in shared memory for tcgen05 blocks of 128 rows,
-// or two of them from 129 rows on (D <= 128).  Slices fill the SMs where there are few blocks.
+// Which kernel and how the work is cut.  Up to 16 rows of a kv head (8 where D is 256: its accumulators take the registers) the codes
+// go to mma.sync as they are, on as many CTAs as are resident at once; beyond, keys and values are brought to f16 in shared
+// memory for tcgen05 blocks of 128 rows, or two of them from 129 rows on (D <= 128), in slices where there are few blocks.
 AttnShape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
     AttnShape s;
     const int64_t rows = max_q * (heads_q / heads_kv);
-    s.tensor = rows > (head_dim <= 128 ? 16 : 8);
-    s.tile_rows = s.tensor ? (rows > 128 && head_dim <= 128 ? 256 : 128) : (rows > 8 ? 16 : 8);
+    s.tensor = rows > (head_dim <= 128 ? AT_MOST_ROWS : AT_MOST_ROWS_256);
+    s.tile_rows = s.tensor ? (rows > 128 && head_dim <= 128 ? 256 : 128) : (rows > 8 && head_dim <= 128 ? 16 : 8);
     s.row_tiles = static_cast<int>((rows + s.tile_rows - 1) / s.tile_rows);
     s.tiles = batch * heads_kv * s.row_tiles;
-    int64_t want, most;
+    s.splits = 1;
+    s.ctas = s.tiles;
     if (s.tensor) {  // one block per SM; a slice has at least 512 keys
-        want = AT_ASSUMED_SMS / (s.tiles > 0 ? s.tiles : 1);
-        most = max_kv / 512;
+        const int64_t want = AT_ASSUMED_SMS / (s.tiles > 0 ? s.tiles : 1), most = max_kv / 512;
+        s.splits = static_cast<int>(want < most ? want : most);
+        if (s.splits < 1) s.splits = 1;
+        s.ctas = s.tiles * s.splits;
+        s.joined = s.splits > 1;
     } else {
-        const int64_t steps = (max_kv + AT_STEP * AT_WARPS - 1) / (AT_STEP * AT_WARPS);  // of a CTA
-        want = AT_ASSUMED_SMS * 3 * AT_WAVES / (s.tiles > 0 ? s.tiles : 1);
-        most = steps;
+        const int resident = s.tile_rows == 16 || head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4;
+        const int64_t unit = head_dim == 256 ? 32 * AT_WARPS : 64 * AT_WARPS, units = s.tiles * (max_kv > unit ? (max_kv + unit - 1) / unit : 1);
+        s.ctas = units < AT_ASSUMED_SMS * resident ? units : AT_ASSUMED_SMS * resident;
+        s.joined = max_kv > unit;  // else no block has two parts
     }
-    s.splits = static_cast<int>(want < most ? want : most);
-    if (s.splits < 1) s.splits = 1;
     return s;
 }
+
+size_t parts_of(const AttnShape& s) { return static_cast<size_t>(s.tensor ? s.ctas : 2 * s.ctas) * s.tile_rows; }
 
 template <int D, int NT>
 int32_t launch_rows(const AttnParams& p, const AttnShape& s, cudaStream_t stream) {
@@ -658,7 +798,7 @@ int32_t launch_rows(const AttnParams& p, const AttnShape& s, cudaStream_t stream
         (void)cudaGetLastError();
         return BQ_STATUS_LAUNCH_FAILURE;
     }
-    kern<<<static_cast<unsigned>(s.tiles * s.splits), AT_WARPS * 32, L::TOTAL, stream>>>(p);
+    kern<<<static_cast<unsigned>(s.ctas), AT_WARPS * 32, L::TOTAL, stream>>>(p);
     return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
 }
 
@@ -672,9 +812,21 @@ int32_t launch_d(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
     } else {
         st = launch_rows<D, 1>(p, s, stream);
     }
-    if (st != BQ_STATUS_OK || s.splits == 1) return st;
-    kv4_attention_join_kernel<D><<<static_cast<unsigned>((s.tiles * s.tile_rows + 3) / 4), 128, 0, stream>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;
+    if (st != BQ_STATUS_OK || !s.joined) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((s.tiles * s.tile_rows + 3) / 4), 1, 1);
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kv4_attention_join_kernel<D>, p) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return BQ_STATUS_LAUNCH_FAILURE;
+    }
+    return BQ_STATUS_OK;
 }
 
 }  // namespace
@@ -682,14 +834,14 @@ int32_t launch_d(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
 bool kv4_attention_fits(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim) {
     if (batch == 0 || max_q == 0) return true;
     const AttnShape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
-    return s.tiles * s.tile_rows <= 0x7fffffff && s.tiles * s.splits <= 0x7fffffff;
+    return s.tiles * s.tile_rows <= 0x7fffffff && s.ctas <= 0x7fffffff;
 }
 
 size_t kv4_attention_workspace_bytes(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv,
                                      int32_t head_dim) {
     const AttnShape s = shape_of(batch, max_q, max_kv, heads_q, heads_kv, head_dim);
-    if (s.splits <= 1) return 0;
-    return static_cast<size_t>(s.tiles) * s.splits * s.tile_rows * (head_dim + 2) * 4;
+    if (!s.joined) return 0;
+    return parts_of(s) * (head_dim + 2) * 4 + (s.tensor ? 0 : static_cast<size_t>(s.tiles) * sizeof(int2));
 }
 
 int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
@@ -718,7 +870,8 @@ int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
     p.splits = s.splits;
     p.tile_rows = s.tile_rows;
     p.part_o = static_cast<float*>(g.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + s.tiles * s.splits * s.tile_rows * g.cache.head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + parts_of(s) * g.cache.head_dim);
+    p.shares = s.tensor || !s.joined ? nullptr : reinterpret_cast<int2*>(p.part_ml + parts_of(s));
     switch (g.cache.head_dim) {
         case 64: return launch_d<64>(p, s, stream);
         case 128: return launch_d<128>(p, s, stream);
