@@ -78,7 +78,8 @@ struct AttnSmem {
     static constexpr int AT_TILES = AttnCfg<D, NT>::TILES;
     static constexpr int STAGE = AT_TILES * kv4_tile_bytes(D);
     static constexpr int RING = AT_WARPS * AT_STAGES * STAGE;  // [stage][warp]: the join takes the place of one stage
-    static constexpr int JOIN = AT_WARPS * 8 * NT * (D + 2) * 4;
+    static constexpr int PITCH = D + 4;  // of a row in the join: a warp's stores go to all banks
+    static constexpr int JOIN = AT_WARPS * 8 * NT * (PITCH + 2) * 4;
     static_assert(JOIN <= AT_WARPS * STAGE, "the join fits one stage");
     static constexpr int BARS = RING;
     static constexpr int VALID = BARS + AT_WARPS * AT_STAGES * 8;
@@ -136,46 +137,65 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         const Extent x = extent_of<AT_STEP, ROWS>(p, b_);
         return static_cast<int64_t>(x.blocks) * p.cache.heads_kv * x.units;
     };
-    int64_t* scan = reinterpret_cast<int64_t*>(smem + L::SCAN);  // [AT_WARPS] sums, then sequence and the units before it
-    const int64_t mine0 = units_of(threadIdx.x);                 // of the first 128 sequences, often all
-    int64_t total = mine0;
-    for (int x = threadIdx.x + AT_WARPS * 32; x < p.batch; x += AT_WARPS * 32) total += units_of(x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) scan[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) total += scan[w];
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);  // none without a unit: parts are counted by CTAs
-    if (blockIdx.x >= ctas) return;
-    int64_t unit = blockIdx.x * total / ctas;
-    const int64_t unit_end = (blockIdx.x + 1) * total / ctas;
-    int64_t before = 0;
-    for (int x0 = 0;; x0 += AT_WARPS * 32) {
-        int64_t sum = x0 == 0 ? mine0 : units_of(x0 + threadIdx.x);
-        const int64_t own = sum;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may take its place early; it waits for the end
+    int64_t total = 0, before = 0;  // units of the launch; of the sequences before b
+    int b = 0;
+    if (p.batch <= 32) {  // each warp for itself
+        const int64_t own = units_of(lane);
+        int64_t sum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += y;
         }
-        __syncthreads();
-        if (lane == 31) scan[warp] = sum;
-        __syncthreads();
-        int64_t chunk = 0;
+        total = __shfl_sync(0xffffffffu, sum, 31);
+        const int64_t ctas_ = min(static_cast<int64_t>(gridDim.x), total);
+        b = __popc(__ballot_sync(0xffffffffu, sum <= blockIdx.x * total / max(ctas_, int64_t{1})));  // sequences that end at or before this CTA's first unit
+        before = __shfl_sync(0xffffffffu, sum - own, b & 31);
+    } else {
+        int64_t* scan = reinterpret_cast<int64_t*>(smem + L::SCAN);  // [AT_WARPS] sums, then sequence and the units before it
+        const int64_t mine0 = units_of(threadIdx.x);                 // of the first 128 sequences, often all
+        total = mine0;
+        for (int x = threadIdx.x + AT_WARPS * 32; x < p.batch; x += AT_WARPS * 32) total += units_of(x);
 #pragma unroll
-        for (int w = 0; w < AT_WARPS; ++w) {
-            if (w < warp) sum += scan[w];
-            chunk += scan[w];
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (lane == 0) scan[warp] = total;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; ++w) total += scan[w];
+        const int64_t first = blockIdx.x * total / max(min(static_cast<int64_t>(gridDim.x), total), int64_t{1});
+        if (first < total) {
+            for (int x0 = 0;; x0 += AT_WARPS * 32) {
+                int64_t sum = x0 == 0 ? mine0 : units_of(x0 + threadIdx.x);
+                const int64_t own = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += y;
+                }
+                __syncthreads();
+                if (lane == 31) scan[warp] = sum;
+                __syncthreads();
+                int64_t chunk = 0;
+#pragma unroll
+                for (int w = 0; w < AT_WARPS; ++w) {
+                    if (w < warp) sum += scan[w];
+                    chunk += scan[w];
+                }
+                if (before + sum - own <= first && first < before + sum) scan[AT_WARPS] = x0 + threadIdx.x, scan[AT_WARPS + 1] = before + sum - own;
+                if (first < before + chunk) break;
+                before += chunk;
+            }
+            __syncthreads();
+            b = static_cast<int>(scan[AT_WARPS]);
+            before = scan[AT_WARPS + 1];
         }
-        if (before + sum - own <= unit && unit < before + sum) scan[AT_WARPS] = x0 + threadIdx.x, scan[AT_WARPS + 1] = before + sum - own;
-        if (unit < before + chunk) break;
-        before += chunk;
     }
-    __syncthreads();
-    int b = static_cast<int>(scan[AT_WARPS]);
-    before = scan[AT_WARPS + 1];
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);  // none without a unit: parts are counted by CTAs
+    if (blockIdx.x >= ctas) return;
+    int64_t unit = blockIdx.x * total / ctas;
+    const int64_t unit_end = (blockIdx.x + 1) * total / ctas;
     Extent xt = extent_of<AT_STEP, ROWS>(p, b);
     uint32_t phases = 0;  // bit s: the phase that stage s is waited for next; every part begins with stage 0
     bool at_start = true;
@@ -621,13 +641,13 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
     fence_proxy_async_smem();
     __syncthreads();  // every warp has left its ring
     if (more && then.mine > 0 && !gave_up) fetch(then, 0, 0);
-    float* join = reinterpret_cast<float*>(smem + AT_WARPS * L::STAGE);  // [warp][row][D], then [warp][row] (ref, l)
-    float2* join_ml = reinterpret_cast<float2*>(join + AT_WARPS * ROWS * D);
+    float* join = reinterpret_cast<float*>(smem + AT_WARPS * L::STAGE);  // [warp][row][PITCH], then [warp][row] (ref, l)
+    float2* join_ml = reinterpret_cast<float2*>(join + AT_WARPS * ROWS * L::PITCH);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float* row = join + (warp * ROWS + nt * 8 + 2 * c + e) * D;
+            float* row = join + (warp * ROWS + nt * 8 + 2 * c + e) * L::PITCH;
 #pragma unroll
             for (int j = 0; j < MT; ++j) {  // codes were 2^-24 and 2^-20
                 row[16 * j + r] = fmaf(acc[nt][j][e], 16777216.0f, z[nt][e][j / 4]);
@@ -648,7 +668,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         for (int w = 0; w < AT_WARPS; ++w) {
             const float2 ml = join_ml[w * ROWS + row];
             const float f = ex2(ml.x - m);
-            const float4 x = *reinterpret_cast<const float4*>(join + (w * ROWS + row) * D + d);
+            const float4 x = *reinterpret_cast<const float4*>(join + (w * ROWS + row) * L::PITCH + d);
             sum = fmaf(ml.y, f, sum);
             o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
         }
