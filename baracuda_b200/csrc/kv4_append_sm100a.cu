@@ -477,54 +477,170 @@ int32_t launch_norm_rope_d(NormRopeParams& p, cudaStream_t stream) {
     return wide ? go(norm_rope_kernel<D, NR_IT, true>, NR_IT) : go(norm_rope_kernel<D, NR_IT, false>, NR_IT);
 }
 
-// One lane of the reader holds 8 channels of one token and head: keys 8 in a row (one word), values r = 0..7 of one nibble
-// column (8 bytes, which the neighbouring lane reads as well).
+// 8 codes as f32 pairs in the order of the nibbles: each code becomes the low byte of 2^23 + c, from which 2^23 is taken.
+__device__ __forceinline__ void codes_f32(uint32_t even, uint32_t odd, f32x2 (&out)[4]) {
+    const f32x2 back = both(-8388608.0f, -8388608.0f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        out[e] = add2(both(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + e)), __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + e))), back);
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+constexpr int RD_WARPS = 4;
+
+// A warp reads one tile of one head: the tokens of the call whose slots are that tile's, in a row, as they are for a sequence's
+// tokens.  Lanes hold what a 16-byte read gives them: of the keys 16 channels of a token (twice per group), of the values 2 channels
+// of 4 tokens per word, which 8 x 8 transposes turn into pairs of channels of one token.  Rows are put together in shared memory and
+// leave whole.  Tokens whose slots are not a tile's are read one by one, 8 channels per lane.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4ReadDesc g) {
-    constexpr int LPH = D / 8;
-    constexpr int G = D / KV4_GROUP;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int l = static_cast<int>(id % LPH);
-    const int64_t row = id / LPH;
-    const int h = static_cast<int>(row % g.cache.heads_kv);
-    const int64_t token = row / g.cache.heads_kv;
-    if (token >= g.tokens) return;
-    const int64_t slot = g.slots[token];
-    if (slot < 0) return;
-    const int64_t page = slot / g.cache.page_size;
-    if (page >= g.cache.num_pages) {
-        atomicCAS(&g_kv4_append_device_status, 0, 402);
+__global__ void __launch_bounds__(RD_WARPS * 32) kv4_read_kernel(const __grid_constant__ Kv4ReadDesc g) {
+    constexpr int G = D / KV4_GROUP, W = D >= 128 ? 2 : 1, PITCH = 2 * D + 16;  // bytes of a staged row: 4 banks on from the one before
+    __shared__ __align__(16) uint8_t staged[RD_WARPS][KV4_TILE * PITCH];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * RD_WARPS + warp;
+    const int64_t chunk = id / g.cache.heads_kv;
+    const int h = static_cast<int>(id - chunk * g.cache.heads_kv);
+    // chunks are cut where the first token's tile ends, and every 16 tokens from there
+    const int64_t slot0 = g.slots[0];
+    const int64_t token0 = chunk * KV4_TILE - (slot0 > 0 ? slot0 & (KV4_TILE - 1) : 0);
+    if (token0 >= g.tokens) return;
+    const int64_t limit = static_cast<int64_t>(g.cache.num_pages) * g.cache.page_size;
+    const int t = lane & (KV4_TILE - 1);
+    const bool asked = token0 + t >= 0 && token0 + t < g.tokens;
+    const int64_t slot = asked ? g.slots[token0 + t] : -1;
+    const uint32_t asked_mask = __ballot_sync(0xffffffffu, asked);
+    const int64_t tile_slot = __shfl_sync(0xffffffffu, slot - t, __ffs(asked_mask) - 1);
+    const bool whole = __all_sync(0xffffffffu, !asked || (slot - t == tile_slot && slot >= 0 && slot < limit && (tile_slot & (KV4_TILE - 1)) == 0));
+    auto tile_at = [&](int64_t s) {
+        const int64_t page = s >> 32 == 0 ? static_cast<uint32_t>(s) / static_cast<uint32_t>(g.cache.page_size) : s / g.cache.page_size;
+        const int off = static_cast<int>(s - page * g.cache.page_size);
+        return g.cache.base + page * g.cache.page_stride + (static_cast<int64_t>(h) * (g.cache.page_size / KV4_TILE) + off / KV4_TILE) * kv4_tile_bytes(D);
+    };
+    if (whole) {
+        const uint8_t* tile = tile_at(tile_slot);
+        uint8_t* mine = staged[warp];
+        uint32_t kw[2][2 * G], kp[2][G], vw[4 * G], vp[4][G];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if constexpr (W == 2) {
+#pragma unroll
+                for (int q = 0; q < G / 2; ++q) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(tile + q * 1024 + e * 512 + lane * 16));
+                    kw[e][4 * q] = v.x, kw[e][4 * q + 1] = v.y, kw[e][4 * q + 2] = v.z, kw[e][4 * q + 3] = v.w;
+                }
+            } else {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(tile + e * 256 + lane * 8));
+                kw[e][0] = v.x, kw[e][1] = v.y;
+            }
+#pragma unroll
+            for (int q = 0; q < G; ++q) kp[e][q] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_pair_offset(D, 0)) + (r + 8 * e) * G + q);
+        }
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(tile + 8 * D + q * 512 + lane * 16));
+            vw[4 * q] = v.x, vw[4 * q + 1] = v.y, vw[4 * q + 2] = v.z, vw[4 * q + 3] = v.w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // tokens 2 c, 8 + 2 c, 2 c + 1, 9 + 2 c, as the bytes of a word
+                vp[e][q] = __ldg(reinterpret_cast<const uint32_t*>(tile + kv4_pair_offset(D, 1)) + (2 * c + (e >> 1) + 8 * (e & 1)) * G + q);
+        }
+        auto pair = [](uint32_t v, f32x2& s, f32x2& m) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+            s = both(f.x, f.x), m = both(f.y, f.y);
+        };
+        auto leave = [&](void* base, int64_t ld) {
+            __syncwarp();
+            constexpr int CHUNKS = D / 8;  // of 16 bytes in a row
+#pragma unroll
+            for (int y = 0; y < KV4_TILE * CHUNKS / 32; ++y) {
+                const int row = (y * 32 + lane) / CHUNKS, at = lane % CHUNKS;
+                if ((asked_mask >> row) & 1u)
+                    *(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + (token0 + row) * ld + static_cast<int64_t>(h) * D) + at) =
+                        *reinterpret_cast<const uint4*>(mine + row * PITCH + at * 16);
+            }
+            __syncwarp();
+        };
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                f32x2 s, m;
+                pair(kp[e][q], s, m);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t word = W == 2 ? kw[e][q / 2 * 4 + (q & 1) * 2 + u] : kw[e][u];
+                    f32x2 x[4];
+                    codes_f32(word & 0x0f0f0f0fu, (word >> 4) & 0x0f0f0f0fu, x);  // byte b: channels 2 b and 2 b + 1
+                    uint32_t o[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) o[b] = pack2(fma2(s, x[b], m));
+                    *reinterpret_cast<uint4*>(mine + (r + 8 * e) * PITCH + 2 * (64 * q + 16 * c + 8 * u)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+        leave(g.k, g.ldk);
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
+            // pairs of tokens: (2 c, 2 c + 1) are bytes 0 and 2 of a word, (8 + 2 c, 9 + 2 c) bytes 1 and 3
+            f32x2 s[2], m[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&vp[e][q])), b = __half22float2(*reinterpret_cast<const __half2*>(&vp[2 + e][q]));
+                s[e] = both(a.x, b.x), m[e] = both(a.y, b.y);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint32_t four = (vw[4 * q + j] >> (4 * n)) & 0x0f0f0f0fu;
+                    const f32x2 back = both(-8388608.0f, -8388608.0f);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const f32x2 x = add2(both(__uint_as_float(__byte_perm(four, 0x4b000000u, 0x7440 + e)), __uint_as_float(__byte_perm(four, 0x4b000000u, 0x7442 + e))), back);
+                        const uint32_t turned = movmatrix_trans(pack2(fma2(s[e], x, m[e])));  // token 8 e + r, channels 2 c, 2 c + 1 of eight
+                        *reinterpret_cast<uint32_t*>(mine + (8 * e + r) * PITCH + 2 * (64 * q + 16 * j + 8 * n + 2 * c)) = turned;
+                    }
+                }
+        }
+        leave(g.v, g.ldv);
         return;
     }
-    const int off = static_cast<int>(slot - page * g.cache.page_size), t = off % KV4_TILE;
-    const uint8_t* tile = g.cache.base + page * g.cache.page_stride +
-                          (static_cast<int64_t>(h) * (g.cache.page_size / KV4_TILE) + off / KV4_TILE) * kv4_tile_bytes(D);
-    const int d = 8 * l;
-    auto pair_of = [&](int values) {
-        return __half22float2(*reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, values) + (t * G + (d >> 6)) * 4));
-    };
-    auto store = [&](void* base, int64_t ld, const float* x) {
-        const uint2 a = pack4(x), b = pack4(x + 4);
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + token * ld + static_cast<int64_t>(h) * D + d) =
-            make_uint4(a.x, a.y, b.x, b.y);
-    };
-    float x[8];
-    {
-        const float2 sm = pair_of(0);
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + kv4_key_byte<D>(t, d));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn(sm.x, static_cast<float>((word >> (4 * e)) & 15u)), sm.y);
-        store(g.k, g.ldk, x);
-    }
-    {
-        const float2 sm = pair_of(1);
-        const int shift = (d & 8) ? 4 : 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t byte = tile[kv4_value_byte<D>(t, (d & ~15) + e)];
-            x[e] = __fadd_rn(__fmul_rn(sm.x, static_cast<float>((byte >> shift) & 15u)), sm.y);
+    for (uint32_t left = asked_mask & 0xffffu; left != 0u; left &= left - 1u) {
+        const int row = __ffs(left) - 1;
+        const int64_t s = __shfl_sync(0xffffffffu, slot, row);
+        if (s < 0) continue;
+        if (s >= limit) {
+            atomicCAS(&g_kv4_append_device_status, 0, 402);
+            continue;
         }
-        store(g.v, g.ldv, x);
+        const uint8_t* tile = tile_at(s);
+        const int tok = static_cast<int>(s & (KV4_TILE - 1));
+        if (lane < D / 8) {
+            const int d = 8 * lane;
+            auto pair_of = [&](int values) {
+                return __half22float2(*reinterpret_cast<const __half2*>(tile + kv4_pair_offset(D, values) + (tok * G + (d >> 6)) * 4));
+            };
+            auto store = [&](void* base, int64_t ld, const float* x) {
+                const uint2 a = pack4(x), b = pack4(x + 4);
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + (token0 + row) * ld + static_cast<int64_t>(h) * D + d) = make_uint4(a.x, a.y, b.x, b.y);
+            };
+            float x[8];
+            float2 sm = pair_of(0);
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + kv4_key_byte<D>(tok, d));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn(sm.x, static_cast<float>((word >> (4 * e)) & 15u)), sm.y);
+            store(g.k, g.ldk, x);
+            sm = pair_of(1);
+            const int shift = (d & 8) ? 4 : 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t byte = tile[kv4_value_byte<D>(tok, (d & ~15) + e)];
+                x[e] = __fadd_rn(__fmul_rn(sm.x, static_cast<float>((byte >> shift) & 15u)), sm.y);
+            }
+            store(g.v, g.ldv, x);
+        }
     }
 }
 
@@ -545,13 +661,13 @@ int32_t launch_qk_norm_rope(const NormRopeDesc& g, cudaStream_t stream) {
 }
 
 int32_t launch_kv4_read(const Kv4ReadDesc& g, cudaStream_t stream) {
-    const int64_t threads = static_cast<int64_t>(g.tokens) * g.cache.heads_kv * (g.cache.head_dim / 8);
-    const int64_t blocks = (threads + 255) / 256;
+    const int64_t warps = (static_cast<int64_t>(g.tokens) + 2 * KV4_TILE - 2) / KV4_TILE * g.cache.heads_kv;  // the first tile may begin anywhere
+    const int64_t blocks = (warps + RD_WARPS - 1) / RD_WARPS;
     if (blocks > 0x7fffffff) return BQ_STATUS_UNSUPPORTED;
     switch (g.cache.head_dim) {
-        case 64: kv4_read_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g); break;
-        case 128: kv4_read_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g); break;
-        case 256: kv4_read_kernel<256><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g); break;
+        case 64: kv4_read_kernel<64><<<static_cast<unsigned>(blocks), RD_WARPS * 32, 0, stream>>>(g); break;
+        case 128: kv4_read_kernel<128><<<static_cast<unsigned>(blocks), RD_WARPS * 32, 0, stream>>>(g); break;
+        case 256: kv4_read_kernel<256><<<static_cast<unsigned>(blocks), RD_WARPS * 32, 0, stream>>>(g); break;
         default: return BQ_STATUS_UNSUPPORTED;
     }
     return cudaPeekAtLastError() == cudaSuccess ? BQ_STATUS_OK : BQ_STATUS_LAUNCH_FAILURE;

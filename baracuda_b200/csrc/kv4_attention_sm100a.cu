@@ -39,10 +39,9 @@ __device__ int g_kv4_attention_device_status = 0;
 constexpr int AT_WARPS = 4;
 constexpr int AT_BLOCK_UNITS = 2;  // look-ups, queries and join of a block take the time of about two units
 constexpr int AT_STAGES = 2;  // the parts of a CTA alternate between them: not another number
-#ifndef AT_MOST_ROWS
-#define AT_MOST_ROWS 64
-#define AT_MOST_ROWS_256 32
-#endif
+// Rows of a kv head up to which codes go to mma.sync as they are: 16 sequences x 6000 tokens take 54 us with 48 rows (tcgen05 kernel 53),
+// 42 with 32 (52) and 97 with 96 (54); with D = 256, 84 us with 32 rows (96) and 122 with 48 (96)
+constexpr int AT_MOST_ROWS = 48, AT_MOST_ROWS_256 = 32;
 constexpr float SLACK = 4.0f;  // a new reference leaves this many powers of two before the next
 constexpr int AT_ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
 
@@ -781,9 +780,9 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     if (p.lse != nullptr && lane == 0) p.lse[q_row * p.heads_q + head] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Which kernel and how the work is cut.  Up to 16 rows of a kv head (8 where D is 256: its accumulators take the registers) the codes
-// go to mma.sync as they are, on as many CTAs as are resident at once; beyond, keys and values are brought to f16 in shared
-// memory for tcgen05 blocks of 128 rows, or two of them from 129 rows on (D <= 128), in slices where there are few blocks.
+// Which kernel and how the work is cut.  A few rows of a kv head meet the codes as they are, 8 or 16 rows at a time (8 where D is 256:
+// its accumulators take the registers), on as many CTAs as are resident at once; beyond, keys and values are brought to f16 in
+// shared memory for tcgen05 blocks of 128 rows, or two of them from 129 rows on (D <= 128), in slices where there are few blocks.
 AttnShape shape_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t heads_q, int64_t heads_kv, int64_t head_dim) {
     AttnShape s;
     const int64_t rows = max_q * (heads_q / heads_kv);

@@ -565,3 +565,26 @@ def test_many_rows_without_keys(dim):
     for _ in range(30):
         again = p.run()
         assert torch.equal(again.out, first.out) and torch.equal(again.lse, first.lse)
+
+
+@pytest.mark.parametrize("dim,page,start,tokens", [(64, 16, 0, 16), (128, 32, 5, 100), (128, 64, 15, 1), (256, 48, 33, 300), (64, 128, 127, 130), (128, 16, 8, 8)])
+def test_read_of_a_sequences_tokens(dim, page, start, tokens):
+    """Slots of a sequence, beginning and ending inside tiles, its pages in no order: the values, and the rows beside them untouched."""
+    g = _gen(start + tokens)
+    heads = 3
+    pages = -(-(start + tokens) // page) + 2
+    desc, cache = _cache(pages, page, heads, dim)
+    cache.random_(0, 256, generator=g)
+    codes, s, m = ref.unpack(cache, page, heads, dim)
+    order = torch.randperm(pages, generator=g, device="cuda")
+    place = torch.arange(start, start + tokens, device="cuda")
+    slots = order[place // page] * page + place % page
+    out = torch.full((2, tokens + 2, heads * dim), 7.0, dtype=BF16, device="cuda")
+    bq.Kv4ReadPlan.select(None, bq.Kv4ReadDescriptor(tokens, desc)).run(None, None, bq.Kv4ReadArgs(cache=cache, slots=slots, k=out[0, 1:-1], v=out[1, 1:-1]))
+    torch.cuda.synchronize()
+    for which in (0, 1):
+        want = ref.values(codes[which], s[which], m[which]).float().to(BF16)[slots].flatten(1)
+        got = out[which, 1:-1]
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+        assert torch.all(out[which, 0] == 7) and torch.all(out[which, -1] == 7)
+    assert bq.device_status() == 0
