@@ -62,11 +62,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 
 // bf16 pair -> f32 pair and back
 __device__ __forceinline__ f32x2 unpack2(uint32_t raw) { return both(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u)); }

@@ -144,4 +144,10 @@ size_t kv4_attention_workspace_bytes(int32_t batch, int32_t max_q, int32_t max_k
 bool kv4_attention_fits(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
 int32_t read_and_clear_kv4_attention_device_status();
 
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 }  // namespace bq

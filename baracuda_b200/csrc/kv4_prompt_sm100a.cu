@@ -8,15 +8,22 @@
 //   v' likewise, but stored by channel with the tokens in a row, as the masks leave pairs of tokens: both products have
 //   operands whose contraction index is contiguous, in the 128-byte swizzle.
 // S = Q K'^T (f16 x f16 -> f32 in TMEM), one softmax thread per row reads S, writes P (f16) over it in TMEM, O += P V' with P as
-// the operand from TMEM.  Queries are brought to f16 by a power of two per row (exact unless 2^-38 of the row's largest).
+// the operand from TMEM; Q too lies in TMEM where that has room, which spares shared memory 128 x D x 2 bytes a step.  Queries
+// are brought to f16 by a power of two per row (exact unless 2^-38 of the row's largest).
 // Roundings to 16 bits: k', v' and P, 2^-11 each, and the output.
-// The softmax reads S twice, first for the maximum: a row's reference moves only when a score exceeds it by 2^SLACK, and O is
-// rescaled (TMEM -> registers -> TMEM) only then.
+// The softmax reads S once: a row's reference moves only when a score exceeds it by 2^SLACK, and only then S is read again and O
+// rescaled (TMEM -> registers -> TMEM).  Steps that a mask or a NaN touches read S twice, first for the maximum.
 //
 // Two row blocks (256 rows, D <= 128): while one block's softmax runs, the tensor core works on the other.  One row block
 // (128 rows; D = 256, or few rows): S is double-buffered instead, the next step's S is computed under this step's softmax.
-// Warps: 4 softmax warps per row block, 4 bring keys and 4 bring values to f16, one issues the MMAs.
+// Warps: 4 softmax warps per row block, 8 (D = 256: 16) bring keys and values to f16, one issues the MMAs.
 // Every mbarrier wait is bounded (status 412..416).
+//
+// Measured (B200): 4096 rows x 32 heads on 8, D = 128, causal: 173 us, 0.80 PFLOP/s of the products that the mask leaves.  The tensor
+// core is busy 38 % of the time: the chain S -> P -> O of a row block takes 4400 clocks a step, 2150 of them the softmax of two
+// warps per quarter of an SM, which share its issue slots with the feeding warps.  2048 rows x 16 heads on 2, D = 256, window
+// 4096: 289 us; there the steps wait for the feeding warps (issue slots 62 % busy; 16 of them: 315 -> 294 us), and the blocks of equal
+// length leave the last wave of three a third full.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -31,33 +38,35 @@ namespace {
 
 __device__ int g_kv4_prompt_device_status = 0;
 
-#ifndef PR_POLY_MASK
-#define PR_POLY_MASK 14
-#define PR_POLY_AT 2
-#endif
 constexpr float PR_SLACK = 7.0f;  // p <= 2^(SLACK + LIFT) stays within f16
+// of 8 pairs of exponentials one comes from the polynomial: prompts of 4096 tokens took 190.3 us with none, 186.2 with 1 of 8, 188.4
+// with 1 of 4, 204 with 1 of 2
+constexpr int PR_POLY_MASK = 14, PR_POLY_AT = 2;
 constexpr float PR_LIFT = 8.0f;   // f16's range below the reference: 2^-22 in full precision
 
 template <int D, int NQ>
 struct PromptCfg {
     static constexpr int KT = D == 256 ? 64 : 128;  // keys of a step
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    static constexpr int FEED_WARPS = 8;
-    static constexpr int SHARES = FEED_WARPS / (KT / KV4_TILE);  // of a tile of 16 keys: whole tiles, or halves of its channels
+    static constexpr int FEED_WARPS = D == 256 ? 16 : 8;
+    static constexpr int SHARES = FEED_WARPS / (KT / KV4_TILE);  // of a tile of 16 keys: whole tiles, or a group of its channels each
     static constexpr int MMA_WARP = SOFTMAX_WARPS + FEED_WARPS;
     static constexpr int THREADS = (MMA_WARP + 1) * 32;
-    // two row blocks: 17 warps leave 96 registers a thread at launch; the feeding warps hand a third of theirs to the softmax warps
-    static constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 128, FEED_REGS = 64;
-    static_assert(NQ == 1 || SOFTMAX_WARPS * SOFTMAX_REGS + FEED_WARPS * FEED_REGS + LAUNCH_REGS <= (MMA_WARP + 1) * LAUNCH_REGS,
+    // 17 or 21 warps leave 96 or 80 registers a thread at launch, and, the feeding warps hand some of theirs to the softmax warps
+    static constexpr bool SPLIT_REGS = NQ == 2 || D == 256;
+    static constexpr int LAUNCH_REGS = D == 256 ? 80 : 96, SOFTMAX_REGS = 128, FEED_REGS = 64;
+    static_assert(!SPLIT_REGS || SOFTMAX_WARPS * SOFTMAX_REGS + FEED_WARPS * FEED_REGS + LAUNCH_REGS <= (MMA_WARP + 1) * LAUNCH_REGS,
                   "the shares come out of what the block was launched with");
     static constexpr int Q_BYTES = NQ * 128 * D * 2;
     static constexpr int K_BYTES = KT * D * 2;  // V the same
     static constexpr int K_OFF = Q_BYTES;
     static constexpr int V_OFF = K_OFF + 2 * K_BYTES;
     static constexpr int BAR_OFF = V_OFF + 2 * K_BYTES;
-    static constexpr int FLAG_OFF = BAR_OFF + 192;           // [2][dead, nan][KT / 16] halfwords
-    static constexpr int TOTAL = FLAG_OFF + 2 * 2 * 8 * 2 + 1024;  // + alignment slack
+    static constexpr int FLAG_OFF = BAR_OFF + 192;           // [2][dead, nan][FEED_WARPS] halfwords
+    static constexpr int TOTAL = FLAG_OFF + 2 * 2 * FEED_WARPS * 2 + 1024;  // + alignment slack
     static constexpr uint32_t S_COL = NQ * D;                // TMEM columns: O of each block, then two S
+    static constexpr uint32_t Q_COL = S_COL + 2 * KT;        // then the queries, where there is room for them
+    static constexpr bool Q_TMEM = Q_COL + NQ * D / 2 <= 512;
 };
 
 struct PromptBars {
@@ -111,6 +120,12 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 16 bytes to shared memory, zeros where there are none.
+__device__ __forceinline__ void cp_async16(void* to, const void* from, bool have) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t bits) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));  // (a & mask) | bits
@@ -121,8 +136,7 @@ __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<
 
 // 2^x of a pair on the FMA units, x at most 16: n = rint(x), 2^(x - n) by the polynomial of degree 4 that is nearest in relative
 // error on [-1/2, 1/2] (Remez exchange; 2.7e-6 with its f32 roundings), n added to the exponent.  Below 2^-125 the result is no more
-// than that.  The special function unit gives 2 results per clock and quarter of an SM, 16 clocks for a warp, and would bound the
-// kernel at 4096 clocks for 256 rows x 128 keys; half of the exponentials are computed here.
+// than that.  The special function unit takes 8 clocks for a warp's results, 2048 for 256 rows x 128 keys, so some are computed here.
 __device__ __forceinline__ float2 ex2_pair(float2 x) {
     const f32x2 magic = both(12582912.0f, 12582912.0f), back = both(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
     const f32x2 v = both(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
@@ -161,6 +175,15 @@ __device__ __forceinline__ uint32_t seen_keys(int key, int lo, int hi) {
     return (to == 32 ? 0xffffffffu : (1u << to) - 1u) & (0xffffffffu << from);
 }
 
+// What a feeding warp's lane holds of a step: codes and (s, m) pairs of the keys r and r + 8, of the values of 2 c, 2 c + 1,
+// 8 + 2 c, 9 + 2 c (GW groups of channels).
+template <int GW>
+struct FeedRegs {
+    uint32_t key[2][2 * GW] = {}, key_pair[2][GW] = {};
+    uint32_t value[4 * GW] = {}, value_pair[4][GW] = {};
+    bool have = false;  // the values' tile
+};
+
 template <int D, int NQ>
 __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kernel(const __grid_constant__ AttnParams p) {
     using C = PromptCfg<D, NQ>;
@@ -173,7 +196,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     uint8_t* smem = pr_smem_raw + ((1024u - (smem_u32(pr_smem_raw) & 1023u)) & 1023u);
     PromptBars* bar = reinterpret_cast<PromptBars*>(smem + C::BAR_OFF);
     volatile uint32_t* abort_word = &bar->abort_word;
-    constexpr int FLAGS = 16;
+    constexpr int FLAGS = 2 * C::FEED_WARPS;
     uint16_t* flags = reinterpret_cast<uint16_t*>(smem + C::FLAG_OFF);  // [stage][dead, nan][feeding warp], a bit per key
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -225,7 +248,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     const uint32_t tmem = bar->tmem_slot;
 
     if (warp < C::SOFTMAX_WARPS) {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         // ---------------------------------------------------------------- softmax: one thread per row
         const int t = warp >> 2;                         // row block
         const int in_block = threadIdx.x & 127;
@@ -235,50 +258,57 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const int i = row / p.group;
         const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
         const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
-        // this warp's 32 query rows to f16 in shared memory, each by a power of two of its own: D / 8 lanes read a row, and the
-        // thread of the row keeps its exponent
+        // this warp's 32 query rows: D / 8 lanes copy one to shared memory, all copies in flight; then each thread brings its row
+        // to f16 by a power of two, to TMEM or back to its place
         const int64_t q_row = sq.row0 + (there ? i : 0);
         const int head = hk * p.group + (there ? row % p.group : 0);
-        constexpr int LPR = D / 8, RPI = 32 / LPR, BATCH = 8;  // lanes of a row, rows of a load, loads in flight
+        constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows of a copy
         uint8_t* q_smem = smem + t * 128 * D * 2;
-        const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-        int ex = 0;
+        auto chunk = [&](int at, int w) { return q_smem + (w >> 3) * (128 * 128) + at * 128 + (((w & 7) ^ (at & 7)) << 4); };
+#pragma unroll 8
+        for (int y = 0; y < LPR; ++y) {
+            const int from = y * RPI + lane / LPR;  // of the warp's 32
+            const int rr = __shfl_sync(0xffffffffu, static_cast<int>(q_row), from), hh = __shfl_sync(0xffffffffu, head, from);
+            const bool have = __shfl_sync(0xffffffffu, static_cast<int>(there), from) != 0;
+            cp_async16(chunk((warp & 3) * 32 + from, lane % LPR), have ? p.q + rr * p.ldq + static_cast<int64_t>(hh) * D + lane % LPR * 8 : p.q, have);
+        }
+        cp_async_wait_all();
+        __syncwarp();
+        uint32_t top2 = 0u;  // of |x|, the even and the odd channels
+#pragma unroll 8
+        for (int w = 0; w < LPR; ++w) {
+            const uint4 v = *reinterpret_cast<const uint4*>(chunk(in_block, w));
+            top2 = max_bf16x2(top2, max_bf16x2(max_bf16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), max_bf16x2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        }
+        const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+        const int ex = top == 0u || top >= 0x7f80u ? 0 : max(-100, min(100, static_cast<int>(top >> 7) - 127 - 14));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
 #pragma unroll 1
-        for (int b0 = 0; b0 < LPR; b0 += BATCH) {
-            uint4 raw[BATCH];
+        for (int x = 0; x < D / 64; ++x) {
+            uint32_t h[32];
 #pragma unroll
-            for (int y = 0; y < BATCH; ++y) {
-                const int from = (b0 + y) * RPI + lane / LPR;  // of the warp's 32
-                const int rr = __shfl_sync(0xffffffffu, static_cast<int>(q_row), from), hh = __shfl_sync(0xffffffffu, head, from);
-                const bool have = __shfl_sync(0xffffffffu, static_cast<int>(there), from) != 0;
-                raw[y] = make_uint4(0u, 0u, 0u, 0u);
-                if (have) raw[y] = __ldg(reinterpret_cast<const uint4*>(p.q + rr * p.ldq + static_cast<int64_t>(hh) * D) + lane % LPR);
-            }
-#pragma unroll
-            for (int y = 0; y < BATCH; ++y) {
-                const uint32_t v[4] = {raw[y].x, raw[y].y, raw[y].z, raw[y].w};
-                uint32_t top = 0u;  // the bits of |x| order as the numbers do
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, max((v[e] << 16) & 0x7fffffffu, v[e] & 0x7fff0000u));
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                int x = static_cast<int>(top >> 23) - 127 - 14;
-                x = top == 0u || top >= 0x7f800000u ? 0 : max(-100, min(100, x));
-                const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23) * sign;
+            for (int w = 0; w < 8; ++w) {
+                const uint4 u = *reinterpret_cast<const uint4*>(chunk(in_block, 8 * x + w));
+                const uint32_t v[4] = {u.x, u.y, u.z, u.w};
                 float f[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[2 * e] = __uint_as_float(v[e] << 16) * down, f[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u) * down;
-                const int w = lane % LPR, at = (warp & 3) * 32 + (b0 + y) * RPI + lane / LPR;
-                *reinterpret_cast<uint4*>(q_smem + (w >> 3) * (128 * 128) + at * 128 + (((w & 7) ^ (at & 7)) << 4)) =
-                    make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
-                const int mine = __shfl_sync(0xffffffffu, x, (lane % RPI) * LPR);
-                if (lane / RPI == b0 + y) ex = mine;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[4 * w + e] = pack_half2(f[e], f[e + 4]);
+                if constexpr (!C::Q_TMEM)
+                    *reinterpret_cast<uint4*>(chunk(in_block, 8 * x + w)) = make_uint4(h[4 * w], h[4 * w + 1], h[4 * w + 2], h[4 * w + 3]);
             }
+            if constexpr (C::Q_TMEM) tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + t * (D / 2) + 32 * x, h);
         }
-        const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f);
-        fence_proxy_async_smem();
+        if constexpr (C::Q_TMEM) {
+            tmem_st_wait();
+            tc_fence_before_sync();
+        } else {
+            fence_proxy_async_smem();
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->qfull);
+        const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f);
 
         // rows of this block that exist see at least [lo_max, hi_min)
         const int last_there = min(all_rows, rt * ROWS + t * 128 + 128) - 1;  // may lie before the block's first row
@@ -306,10 +336,18 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             const uint32_t* nans = gone + FLAGS / 4;
             uint32_t any = 0u;
 #pragma unroll
-            for (int x = 0; x < C::FEED_WARPS / 2; ++x) any |= gone[x] | nans[x];
+            for (int x = 0; x < FLAGS / 8; ++x) {
+                const uint4 f = reinterpret_cast<const uint4*>(gone)[x];
+                any |= f.x | f.y | f.z | f.w;
+            }
             auto bits_of = [](const uint32_t* w, int x) {  // of keys 32 x .. 32 x + 31
-                if constexpr (C::SHARES == 1) return w[x];
-                return ((w[2 * x] | (w[2 * x] >> 16)) & 0xffffu) | ((w[2 * x + 1] | (w[2 * x + 1] << 16)) & 0xffff0000u);
+                if constexpr (C::SHARES == 1) {
+                    return w[x];
+                } else {
+                    static_assert(C::SHARES == 4, "two words a tile");
+                    const uint32_t a = w[4 * x] | w[4 * x + 1], b = w[4 * x + 2] | w[4 * x + 3];
+                    return ((a | (a >> 16)) & 0xffffu) | ((b | (b << 16)) & 0xffff0000u);
+                }
             };
             const bool edge = key0 + KT > hi_min || key0 < lo_max || any != 0u;
             const f32x2 factor2 = both(factor, factor);
@@ -322,19 +360,24 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 f32x2 sum[2] = {0ull, 0ull};
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 uint32_t pk[KT / 32][16];
+                constexpr int CH = D == 256 ? 32 : 64;
 #pragma unroll
-                for (int x = 0; x < KT / 64; ++x) {
-                    uint32_t v[64];
-                    tmem_ld_32x32b_x64(s_tmem + 64 * x, v);
+                for (int x = 0; x < KT / CH; ++x) {
+                    uint32_t v[CH];
+                    if constexpr (CH == 64) {
+                        tmem_ld_32x32b_x64(s_tmem + CH * x, v);
+                    } else {
+                        tmem_ld_32x32b_x32(s_tmem + CH * x, v);
+                    }
                     tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
+                    for (int e = 0; e < CH; e += 2) {
                         const float s0 = __uint_as_float(v[e]), s1 = __uint_as_float(v[e + 1]);
                         m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], s0), s1);
                         const float2 w = each(fma2(both(s0, s1), factor2, base2));
                         const float2 pr = (e & PR_POLY_MASK) == PR_POLY_AT ? ex2_pair(w) : make_float2(ex2(w.x), ex2(w.y));
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(pr.x, pr.y));
-                        pk[2 * x + (e >> 5)][(e & 31) / 2] = pack_half2(pr.x, pr.y);
+                        pk[CH / 32 * x + (e >> 5)][(e & 31) / 2] = pack_half2(pr.x, pr.y);
                     }
                 }
                 mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * factor;
@@ -483,7 +526,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             }
         }
     } else if (warp < C::MMA_WARP) {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEED_REGS));
+        if constexpr (C::SPLIT_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEED_REGS));
         // ---------------------------------------------------------------- keys and values to f16
         // a warp's share of a step: one tile of 16 keys, or half of its channels (groups g0 .. g0 + GW - 1)
         constexpr int STEP_TILES = KT / KV4_TILE, GW = G / C::SHARES;
@@ -506,10 +549,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 }
             }
         };
-        // a step's codes and (s, m) pairs of this lane: of the keys r and r + 8, of the values of 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
-        uint32_t key[2][2 * GW] = {}, key_pair[2][GW] = {};
-        uint32_t value[4 * GW] = {}, value_pair[4][GW] = {};
-        bool have = false;  // the values' tile
+        FeedRegs<GW> h;
         auto place_of = [&](int j) -> const uint8_t* {
             const int64_t where = __shfl_sync(0xffffffffu, ahead, j & 31);
             return where < 0 ? nullptr : head_base + where;
@@ -520,38 +560,42 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             if (at == nullptr) return;  // whatever is in the registers: these keys are masked
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if constexpr (W == 2) {
+                if constexpr (W == 2 && GW == 1) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + (g0 >> 1) * 1024 + e * 512 + lane * 16 + (g0 & 1) * 8);
+                    h.key[e][0] = v.x, h.key[e][1] = v.y;
+                    h.key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g0) * 4);
+                } else if constexpr (W == 2) {
 #pragma unroll
-                    for (int h = 0; h < GW / 2; ++h) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(at + (g0 / 2 + h) * 1024 + e * 512 + lane * 16);
-                        key[e][4 * h] = v.x, key[e][4 * h + 1] = v.y, key[e][4 * h + 2] = v.z, key[e][4 * h + 3] = v.w;
+                    for (int x = 0; x < GW / 2; ++x) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(at + (g0 / 2 + x) * 1024 + e * 512 + lane * 16);
+                        h.key[e][4 * x] = v.x, h.key[e][4 * x + 1] = v.y, h.key[e][4 * x + 2] = v.z, h.key[e][4 * x + 3] = v.w;
                     }
                     const uint2 v = *reinterpret_cast<const uint2*>(at + kv4_pair_offset(D, 0) + ((r + 8 * e) * G + g0) * 4);
-                    key_pair[e][0] = v.x, key_pair[e][1] = v.y;
+                    h.key_pair[e][0] = v.x, h.key_pair[e][1] = v.y;
                 } else {
                     const uint2 v = *reinterpret_cast<const uint2*>(at + e * 256 + lane * 8);
-                    key[e][0] = v.x, key[e][1] = v.y;
-                    key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + (r + 8 * e) * 4);
+                    h.key[e][0] = v.x, h.key[e][1] = v.y;
+                    h.key_pair[e][0] = *reinterpret_cast<const uint32_t*>(at + kv4_pair_offset(D, 0) + (r + 8 * e) * 4);
                 }
             }
         };
         auto load_values = [&](int j) {
             const uint8_t* at = place_of(j);
-            have = at != nullptr;
-            if (!have) return;  // as above: zeroed below
+            h.have = at != nullptr;
+            if (!h.have) return;  // as above: zeroed below
 #pragma unroll
             for (int g = 0; g < GW; ++g) {
                 const uint4 v = *reinterpret_cast<const uint4*>(at + 8 * D + (g0 + g) * 512 + lane * 16);
-                value[4 * g] = v.x, value[4 * g + 1] = v.y, value[4 * g + 2] = v.z, value[4 * g + 3] = v.w;
+                h.value[4 * g] = v.x, h.value[4 * g + 1] = v.y, h.value[4 * g + 2] = v.z, h.value[4 * g + 3] = v.w;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint8_t* pair = at + kv4_pair_offset(D, 1) + ((2 * c + (e & 1) + 8 * (e >> 1)) * G + g0) * 4;
-                if constexpr (W == 2) {
+                if constexpr (GW == 2) {
                     const uint2 v = *reinterpret_cast<const uint2*>(pair);
-                    value_pair[e][0] = v.x, value_pair[e][1] = v.y;
+                    h.value_pair[e][0] = v.x, h.value_pair[e][1] = v.y;
                 } else {
-                    value_pair[e][0] = *reinterpret_cast<const uint32_t*>(pair);
+                    h.value_pair[e][0] = *reinterpret_cast<const uint32_t*>(pair);
                 }
             }
         };
@@ -561,11 +605,11 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 uint8_t* row = k_smem + (in_step * KV4_TILE + r + 8 * e) * 128;
 #pragma unroll
                 for (int g = 0; g < GW; ++g) {
-                    const __half2 sm = as_h2(key_pair[e][g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
+                    const __half2 sm = as_h2(h.key_pair[e][g]), s2 = __low2half2(sm), m2 = __high2half2(sm);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         uint32_t o[4];
-                        expand(key[e][2 * g + u], s2, m2, s2, m2, o);
+                        expand(h.key[e][2 * g + u], s2, m2, s2, m2, o);
                         *reinterpret_cast<uint4*>(row + (g0 + g) * (KT * 128) + (((2 * c + u) ^ r) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 }
@@ -578,19 +622,19 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int g = 0; g < GW; ++g) top |= (value_pair[e][g] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
+                for (int g = 0; g < GW; ++g) top |= (h.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;  // sign bits: an exponent of ones
             uint32_t nan_bits = 0u;
-            if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len || !have)) {
+            if (__any_sync(0xffffffffu, (top & 0x80008000u) != 0u || key0 + KV4_TILE > sq.len || !h.have)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int tok = 2 * c + (e & 1) + 8 * (e >> 1);
                     uint32_t ones = 0u;
 #pragma unroll
-                    for (int g = 0; g < GW; ++g) ones |= (value_pair[e][g] & 0x7c007c00u) + 0x04000400u;
-                    const bool beyond = key0 + tok >= sq.len || !have, nan = (ones & 0x80008000u) != 0u;
+                    for (int g = 0; g < GW; ++g) ones |= (h.value_pair[e][g] & 0x7c007c00u) + 0x04000400u;
+                    const bool beyond = key0 + tok >= sq.len || !h.have, nan = (ones & 0x80008000u) != 0u;
                     if (beyond || nan) {
 #pragma unroll
-                        for (int g = 0; g < GW; ++g) value_pair[e][g] = 0u;
+                        for (int g = 0; g < GW; ++g) h.value_pair[e][g] = 0u;
                     }
                     if (nan && !beyond) nan_bits |= 1u << tok;
                 }
@@ -598,19 +642,19 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 nan_bits |= __shfl_xor_sync(0xffffffffu, nan_bits, 2);
             }
             if (lane == 0) {
-                flags[stage * FLAGS + feeder] = have || key0 >= hi_all ? 0u : 0xffffu;
-                flags[stage * FLAGS + 8 + feeder] = static_cast<uint16_t>(nan_bits);
+                flags[stage * FLAGS + feeder] = h.have || key0 >= hi_all ? 0u : 0xffffu;
+                flags[stage * FLAGS + C::FEED_WARPS + feeder] = static_cast<uint16_t>(nan_bits);
             }
             uint8_t* row = v_smem + (in_step >> 2) * (D * 128) + r * 128 + 4 * c;
             const int at0 = ((2 * (in_step & 3)) ^ r) << 4, at1 = ((2 * (in_step & 3) + 1) ^ r) << 4;
 #pragma unroll
             for (int g = 0; g < GW; ++g) {
-                const __half2 t0 = as_h2(value_pair[0][g]), t1 = as_h2(value_pair[1][g]), t2 = as_h2(value_pair[2][g]), t3 = as_h2(value_pair[3][g]);
+                const __half2 t0 = as_h2(h.value_pair[0][g]), t1 = as_h2(h.value_pair[1][g]), t2 = as_h2(h.value_pair[2][g]), t3 = as_h2(h.value_pair[3][g]);
                 const __half2 s_lo = __lows2half2(t0, t1), m_lo = __highs2half2(t0, t1), s_hi = __lows2half2(t2, t3), m_hi = __highs2half2(t2, t3);
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     uint32_t o[4];  // (channel r, tokens 2 c ..), (r + 8, 2 c ..), (r, 8 + 2 c ..), (r + 8, 8 + 2 c ..)
-                    expand(value[4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
+                    expand(h.value[4 * g + jj], s_lo, m_lo, s_hi, m_hi, o);
                     uint8_t* to = row + (64 * (g0 + g) + 16 * jj) * 128;
                     *reinterpret_cast<uint32_t*>(to + at0) = o[0];
                     *reinterpret_cast<uint32_t*>(to + 8 * 128 + at0) = o[1];
@@ -619,38 +663,42 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 }
             }
         };
-        // the next step's keys are on their way under this step's values, and the other way round
-        if (n > 0) load_keys(0), load_values(0);
-        bool ok = true;
-        for (int j = 0; j < n; ++j) {
+        // the next step's keys are on their way under this step's values, and the other way round; a step further ahead, in
+        // registers, was slower (16 warps of D = 256 with two steps each: 294 -> 310 us)
+        auto step = [&](int j) -> bool {
             const int stage = j & 1;
+            bool ok = true;
             if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
                 give_up(abort_word, 415);
                 ok = false;
             }
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!__all_sync(0xffffffffu, ok)) return false;
             convert_keys(smem + C::K_OFF + stage * C::K_BYTES);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->kfull[stage]);
-            // the look-up of the next 32 steps must not replace what this step's values still go by: they are loaded already
+            // the look-up of the next 32 steps must not replace what earlier steps' values still go by: they are loaded already
             if (j + 1 < n) load_keys(j + 1);
             if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
                 give_up(abort_word, 415);
                 ok = false;
             }
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!__all_sync(0xffffffffu, ok)) return false;
             convert_values(smem + C::V_OFF + stage * C::K_BYTES, j, stage);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->vfull[stage]);
             if (j + 1 < n) load_values(j + 1);
+            return true;
+        };
+        if (n > 0) load_keys(0), load_values(0);
+        for (int j = 0; j < n && step(j); ++j) {
         }
     } else {
         // ---------------------------------------------------------------- MMA issue: the warp walks the steps, one lane issues
         constexpr uint32_t IDESC_S = idesc_f16(128, KT), IDESC_O = idesc_f16(128, D);
         const bool leader = elect_one() != 0u;
-        const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(smem));
+        [[maybe_unused]] const uint64_t q_desc = umma_desc_kmajor_sw128(smem_u32(smem));
         const uint64_t k_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::K_OFF), v_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::V_OFF);
         bool ok = true;
         auto wait = [&](uint64_t* what, uint32_t parity) {
@@ -663,12 +711,18 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         };
         // descriptors count addresses in 16 bytes: a 16-deep slice is 32 bytes on within a 128-byte block of 64
         auto scores = [&](int t, int j, int slot) {
-            const uint64_t q = q_desc + t * (128 * D * 2 / 16), k = k_desc + (j & 1) * (C::K_BYTES / 16);
+            const uint64_t k = k_desc + (j & 1) * (C::K_BYTES / 16);
             const uint32_t to = tmem + C::S_COL + slot * KT;
             if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    umma_f16_ss(to, q + ((ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2), k + ((ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2), IDESC_S, ks > 0);
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint64_t keys = k + ((ks >> 2) * (KT * 128 / 16) + (ks & 3) * 2);
+                    if constexpr (C::Q_TMEM) {
+                        umma_f16_ts(to, tmem + C::Q_COL + t * (D / 2) + ks * 8, keys, IDESC_S, ks > 0);
+                    } else {
+                        umma_f16_ss(to, q_desc + (t * (128 * D * 2 / 16) + (ks >> 2) * (128 * 128 / 16) + (ks & 3) * 2), keys, IDESC_S, ks > 0);
+                    }
+                }
                 umma_commit(&bar->sfull[slot]);
             }
             __syncwarp();
@@ -736,7 +790,7 @@ int32_t launch_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stre
     auto kern = kv4_prompt_kernel<D, NQ>;
     constexpr int bytes = PromptCfg<D, NQ>::TOTAL;
     static_assert(bytes <= 232448, "shared memory of an SM");
-    if constexpr (NQ == 2) {
+    if constexpr (PromptCfg<D, NQ>::SPLIT_REGS) {
         // the warps' shares of the registers are sums over what a launch gets: never start a build that gets another number
         static const bool as_assumed = [kern] {
             cudaFuncAttributes a;
