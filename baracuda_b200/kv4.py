@@ -220,7 +220,7 @@ class QkNormRopePlan:
             shape = args.cos_sin.shape
             if len(shape) != 2 or shape[1] != self._rot:
                 raise InvalidProblem(f"cos_sin: expected [max_pos, {self._rot}]")
-            max_pos = shape[0]
+            max_pos = min(shape[0], 2**31 - 1)  # positions are int32
             positions = _vector(args.positions, torch.int32, 1, "positions", dev)
             shape = args.positions.shape
             pos_stride = shape[-1] if shape else 0
@@ -380,10 +380,12 @@ class Kv4AttentionPlan:
     def run(self, stream, workspace: Optional[torch.Tensor], args: Kv4AttentionArgs) -> None:
         d = self.desc
         c = d.cache
-        total = args.q.shape[0]
-        if d.batch == 0 or d.max_q == 0 or total == 0:
+        if d.batch == 0 or d.max_q == 0:
             return
         dev, cols = _device_of(args.q, "q"), d.heads_q * c.head_dim
+        total = args.q.shape[0] if args.q.dim() else 0
+        if total == 0:
+            return
         q, ldq = _matrix(args.q, total, cols, "q", dev)
         out, ldo = _matrix(args.out, total, cols, "out", dev)
         lse = None if args.lse is None else _vector(args.lse, torch.float32, total * d.heads_q, "lse", dev)

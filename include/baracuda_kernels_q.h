@@ -570,8 +570,8 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
  * on the pages page_table[b][0 ..] (int32, row pitch ld_table >= ceil(max_kv / page_size)).  Row i of n sees key j when
  *   j < kv_lens[b], with causal != 0 also j <= kv_lens[b] - n + i, with window > 0 also j > kv_lens[b] - n + i - window.
  * out = sum_j softmax_j(scale * q . k[j]) v[j], rounded once; a row that sees no key gets zeros.  lse, float
- * [total_q][heads_q] or NULL, gets log sum_j exp(scale * q . k[j]), minus infinity for such a row.  Rows outside every sequence
- * are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
+ * [total_q][heads_q] or NULL, gets log sum_j exp(scale * q . k[j]), minus infinity for such a row.  A NaN key makes the rows that
+ * see it NaN, a NaN value at least the channels of its group in them.  Rows outside every sequence are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
  * by them, and the workspace (16-byte aligned) needs no initialisation; two launches that may overlap need one each.
  * Lengths beyond max_q, max_kv or total_q are cut and reported as device status 403; a page number outside [0, num_pages)
  * where a key is seen leaves its keys out and is reported as 404.
@@ -815,7 +815,7 @@ int32_t baracuda_q_nccl_all_gather_bytes(void* comm, int32_t world, const void* 
  * of its bounded barrier waits ran out (0 = none; the code names the kernel and
  * the waiting role: 101..104 1-CTA GEMM, 111..115 CTA-pair GEMM, 121..123 cluster split-K GEMM, 201..207 streaming GEMVs, 299 the self-test, 301 the peer barrier, 401 / 402 a position / a slot out of
  * range in the norm, rotation, append and read kernels, 403 / 404 a length / a page number out of range in the attention over
- * the 4-bit cache, 411 its bounded waits).  Call it after synchronising the stream.
+ * the 4-bit cache, 411..416 its bounded waits).  Call it after synchronising the stream.
  * set_tuning: forces a kernel choice for the CALLING THREAD only (thread-local; other threads' launches are not
  * affected, nothing process-wide is kept), so tests can run every kernel on the same shapes:
  *   key 0  GEMM tile: 0 automatic; 64, 128, 256 = 1-CTA kernel with that N-tile; 512 = the CTA-pair kernel;

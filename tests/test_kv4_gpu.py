@@ -588,3 +588,87 @@ def test_read_of_a_sequences_tokens(dim, page, start, tokens):
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
         assert torch.all(out[which, 0] == 7) and torch.all(out[which, -1] == 7)
     assert bq.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ large batches, holes, two at once
+@pytest.mark.parametrize("batch,dim,heads_q,heads_kv,most_rows", [(33, 128, 4, 1, 1), (128, 64, 2, 2, 3), (129, 256, 2, 1, 2), (300, 128, 16, 2, 2), (1000, 64, 1, 1, 1)])
+def test_many_sequences(batch, dim, heads_q, heads_kv, most_rows):
+    """More sequences than a warp, and than a block, looks at in one go, of very different lengths; some without rows, some without keys."""
+    g = torch.Generator().manual_seed(batch)
+    rows = torch.randint(0, most_rows + 1, (batch,), generator=g).tolist()
+    lens = (torch.rand(batch, generator=g) ** 4 * 900).int().tolist()
+    rows[0] = rows[-1] = most_rows
+    p = Problem(list(zip(rows, lens)), heads_q, heads_kv, dim, 16, seed=batch)
+    p.check(p.run())
+
+
+def test_many_prompts():
+    p = Problem([(40 + 37 * i % 100, 30 + 91 * i % 400) for i in range(40)], 4, 2, 64, 16, seed=40)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (1, 128), (3, 256), (20, 128), (100, 128), (200, 128), (160, 64), (20, 64), (140, 256)])
+def test_pages_that_are_missing_inside_leave_their_keys_out(rows, dim):
+    """Of 400 keys the pages of 48..79 and 320..335 have no number: what is seen is the rest."""
+    page, heads_q, heads_kv = 16, 4, 2
+    p = Problem([(rows, 400)], heads_q, heads_kv, dim, page, seed=rows)
+    keys = [j for j in range(400) if j // page not in (3, 4, 20)]
+    values = ref.values(*(x[:, p.table[0].long()[torch.tensor(keys, device="cuda") // page] * page + torch.tensor(keys, device="cuda") % page]
+                          for x in ref.unpack(p.cache, page, heads_kv, dim))).double()
+    table = p.table.clone()
+    p.table[0, 3], p.table[0, 4], p.table[0, 20] = -1, p.desc.num_pages, 2 ** 31 - 1
+    got = p.run()
+    torch.cuda.synchronize()
+    assert bq.device_status() == 404 and bq.device_status() == 0
+    k, v = (x.repeat_interleave(heads_q // heads_kv, 1) for x in values)
+    q = p.q[:rows].double().reshape(rows, heads_q, dim)
+    score = torch.einsum("ihd,jhd->hij", q, k) * p.scale
+    seen = torch.tensor(keys, device="cuda")[None, :] <= 400 - rows + torch.arange(rows, device="cuda")[:, None]
+    weight = torch.softmax(score.masked_fill(~seen, -math.inf), -1)
+    want = torch.einsum("hij,jhd->ihd", weight, v)
+    # all roundings together: bf16 of the output, f16 of keys, values and weights
+    err = (got.out[:rows].double().reshape(want.shape) - want).norm() / want.norm()
+    assert float(err) <= 2.0 ** -8 / math.sqrt(3.0) + 4 * 2.0 ** -11
+    p.table.copy_(table)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (1, 128), (3, 256), (20, 128), (200, 128), (160, 64), (140, 256)])
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_a_nan_reaches_the_rows_that_see_it_and_no_other(rows, dim, what):
+    page, at = 16, 400 - rows + rows // 2
+    p = Problem([(rows, 400), (rows, 30)], 2, 1, dim, page, seed=rows + dim)
+    clean = p.run()
+    codes, s, m = ref.unpack(p.cache, page, 1, dim)
+    slot = p.table[0].long()[at // page] * page + at % page
+    k, v = (ref.values(codes[i], s[i], m[i])[slot].reshape(1, 1, dim).to(BF16) for i in (0, 1))
+    (k if what == "key" else v)[0, 0, 5] = math.nan
+    ref.fill(p.cache, page, 1, dim, slot.reshape(1), k, v)
+    got = p.run()
+    torch.cuda.synchronize()
+    sees = 400 - rows + torch.arange(rows, device="cuda") >= at
+    out, before = (x.out[:rows].reshape(rows, 2, dim) for x in (got, clean))
+    assert out[sees][:, :, :64].isnan().all()
+    assert what == "value" or out[sees].isnan().all()
+    assert torch.equal(out[~sees], before[~sees])
+    assert torch.equal(got.out[rows:], clean.out[rows:])
+    assert bq.device_status() == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with a workspace of its own, leave what they leave one after the other."""
+    problems = [Problem([(1, 5000), (2, 3000)], 8, 2, 128, 32, seed=1), Problem([(150, 2000)], 8, 2, 128, 32, seed=2)]
+    alone = [p.run() for p in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    plans = [p.plan() for p in problems]
+    spaces = [torch.empty(max(1, plan.workspace_size()), dtype=torch.uint8, device="cuda") for plan in plans]
+    outs = [[torch.zeros_like(a.out) for _ in range(10)] for a in alone]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for p, plan, stream, space, out in zip(problems, plans, streams, spaces, outs):
+            plan.run(stream, space, bq.Kv4AttentionArgs(q=p.q, cu_q=p.cu_q, kv_lens=p.kv_lens, page_table=p.table, cache=p.cache, out=out[i]))
+    torch.cuda.synchronize()
+    for p, a, out in zip(problems, alone, outs):
+        assert all(torch.equal(o[: p.rows], a.out[: p.rows]) for o in out)
+    assert bq.device_status() == 0

@@ -136,3 +136,12 @@ def test_plans_refuse_before_they_call(qlib):
     with pytest.raises(bq.InvalidProblem):
         plan.run(None, None, bq.Kv4AppendArgs(k=x, v=x, cache=buf, slots=slots))  # host buffers
     bq.Kv4AppendPlan.select(None, bq.Kv4AppendDescriptor(0, cache)).run(None, None, bq.Kv4AppendArgs(k=x, v=x, cache=buf, slots=slots))
+
+
+def test_attention_plan_refuses_missing_and_host_queries(qlib):
+    cache = bq.Kv4CacheDescriptor(4, 16, 2, 128)
+    plan = bq.Kv4AttentionPlan.select(None, bq.Kv4AttentionDescriptor(1, 1, 10, 8, cache))
+    some = torch.zeros(1, dtype=torch.int32)
+    for q in (None, torch.zeros(1, 1024, dtype=torch.bfloat16), torch.zeros((), dtype=torch.bfloat16)):
+        with pytest.raises(bq.InvalidProblem):
+            plan.run(None, None, bq.Kv4AttentionArgs(q=q, cu_q=some, kv_lens=some, page_table=some, cache=some, out=q))
