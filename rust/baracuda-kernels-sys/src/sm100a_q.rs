@@ -435,6 +435,73 @@ extern "C" {
         out: *mut c_void, out_pitch: i64, stream: *mut c_void,
     ) -> i32;
 
+    /// Attention step over a paged 4-bit cache.  Bytes of a page (0 where not served).
+    pub fn baracuda_kernels_kv4_page_bytes(page_size: i32, heads_kv: i32, head_dim: i32) -> usize;
+    /// RMS norm of every query and key head and the rotation by position; `axis_of_pair` is a host array.
+    pub fn baracuda_kernels_qk_norm_rope_bf16_sm100a_run(
+        tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32,
+        q: *const c_void, ldq: i64, k: *const c_void, ldk: i64,
+        q_weight: *const c_void, k_weight: *const c_void, eps: f32,
+        cos_sin: *const c_void, rot_dim: i32, max_pos: i32, interleaved: i32,
+        positions: *const c_void, pos_stride: i64, axes: i32, axis_of_pair: *const u8,
+        q_out: *mut c_void, ldqo: i64, k_out: *mut c_void, ldko: i64,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+    pub fn baracuda_kernels_qk_norm_rope_bf16_sm100a_can_implement(
+        tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32, rot_dim: i32, axes: i32,
+    ) -> i32;
+    pub fn baracuda_kernels_qk_norm_rope_bf16_sm100a_workspace_size(tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32) -> usize;
+    /// The same with keys and values into the cache at `slots`.
+    pub fn baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_run(
+        tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32,
+        q: *const c_void, ldq: i64, k: *const c_void, ldk: i64, v: *const c_void, ldv: i64,
+        q_weight: *const c_void, k_weight: *const c_void, eps: f32,
+        cos_sin: *const c_void, rot_dim: i32, max_pos: i32, interleaved: i32,
+        positions: *const c_void, pos_stride: i64, axes: i32, axis_of_pair: *const u8,
+        q_out: *mut c_void, ldqo: i64,
+        cache: *mut c_void, page_stride: i64, num_pages: i32, page_size: i32, slots: *const c_void,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+    pub fn baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_can_implement(
+        tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32, rot_dim: i32, axes: i32, page_size: i32,
+    ) -> i32;
+    pub fn baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_workspace_size(tokens: i32, heads_q: i32, heads_kv: i32, head_dim: i32) -> usize;
+    /// Keys and values into the cache as they are.
+    pub fn baracuda_kernels_kv4_append_bf16_sm100a_run(
+        tokens: i32, heads_kv: i32, head_dim: i32,
+        k: *const c_void, ldk: i64, v: *const c_void, ldv: i64,
+        cache: *mut c_void, page_stride: i64, num_pages: i32, page_size: i32, slots: *const c_void,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+    pub fn baracuda_kernels_kv4_append_bf16_sm100a_can_implement(tokens: i32, heads_kv: i32, head_dim: i32, page_size: i32) -> i32;
+    pub fn baracuda_kernels_kv4_append_bf16_sm100a_workspace_size(tokens: i32, heads_kv: i32, head_dim: i32) -> usize;
+    /// The tokens at `slots` as bf16 keys and values.
+    pub fn baracuda_kernels_kv4_read_bf16_sm100a_run(
+        tokens: i32, heads_kv: i32, head_dim: i32,
+        cache: *const c_void, page_stride: i64, num_pages: i32, page_size: i32, slots: *const c_void,
+        k: *mut c_void, ldk: i64, v: *mut c_void, ldv: i64,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+    pub fn baracuda_kernels_kv4_read_bf16_sm100a_can_implement(tokens: i32, heads_kv: i32, head_dim: i32, page_size: i32) -> i32;
+    pub fn baracuda_kernels_kv4_read_bf16_sm100a_workspace_size(tokens: i32, heads_kv: i32, head_dim: i32) -> usize;
+    /// Attention of ragged query rows over the cache: decode steps, drafted tokens, prompts.
+    pub fn baracuda_kernels_attention_kv4_bf16_sm100a_run(
+        batch: i32, total_q: i32, max_q: i32, max_kv: i32,
+        heads_q: i32, heads_kv: i32, head_dim: i32,
+        q: *const c_void, ldq: i64, cu_q: *const c_void,
+        cache: *const c_void, page_stride: i64, num_pages: i32, page_size: i32,
+        page_table: *const c_void, ld_table: i64, kv_lens: *const c_void,
+        scale: f32, causal: i32, window: i32,
+        out: *mut c_void, ldo: i64, lse: *mut c_void,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+    pub fn baracuda_kernels_attention_kv4_bf16_sm100a_can_implement(
+        batch: i32, max_q: i32, max_kv: i32, heads_q: i32, heads_kv: i32, head_dim: i32, page_size: i32,
+    ) -> i32;
+    pub fn baracuda_kernels_attention_kv4_bf16_sm100a_workspace_size(
+        batch: i32, max_q: i32, max_kv: i32, heads_q: i32, heads_kv: i32, head_dim: i32,
+    ) -> usize;
+
     /// Communicator helpers over the run-time-loaded NCCL (`Communicator::{new_with_id, all_gather}` of baracuda-nccl).
     pub fn baracuda_q_nccl_version() -> i32;
     pub fn baracuda_q_nccl_unique_id(id_out_128_bytes: *mut c_void) -> i32;

@@ -1,10 +1,15 @@
 """Refusals of the attention step over the 4-bit cache: everything that is decided before a launch, without a GPU; and the
 storage formulas against one another."""
+import re
+import subprocess
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
 
 import baracuda_b200 as bq
+from baracuda_b200 import _lib
 import kv4_reference as ref
 
 P = 16  # any pointer that is aligned; nothing here launches
@@ -145,3 +150,27 @@ def test_attention_plan_refuses_missing_and_host_queries(qlib):
     for q in (None, torch.zeros(1, 1024, dtype=torch.bfloat16), torch.zeros((), dtype=torch.bfloat16)):
         with pytest.raises(bq.InvalidProblem):
             plan.run(None, None, bq.Kv4AttentionArgs(q=q, cu_q=some, kv_lens=some, page_table=some, cache=some, out=q))
+
+
+def test_cpp_plans(qlib, tmp_path):
+    """Compiles and runs the host-only checks of include/baracuda_kernels_kv4_plan.hpp against the library."""
+    root = Path(__file__).resolve().parents[1]
+    exe, lib = tmp_path / "kv4_plan_host_test", _lib.LIB_PATH.parent
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", str(root / "include"), str(root / "tests" / "cpp" / "kv4_plan_host_test.cpp"),
+                    "-o", str(exe), "-L", str(lib), "-lbaracuda_kernels_q", f"-Wl,-rpath,{lib}"], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0 and "kv4_plan_host_test ok" in res.stdout, res.stdout + res.stderr
+
+
+def test_rust_declarations_name_the_headers_symbols():
+    """The -sys declarations have the header's symbols with as many parameters."""
+    root = Path(__file__).resolve().parents[1]
+    strip = lambda text: re.sub(r"/\*.*?\*/|//[^\n]*", "", text, flags=re.S)  # noqa: E731
+    header = strip((root / "include" / "baracuda_kernels_q.h").read_text())
+    rust = strip((root / "rust" / "baracuda-kernels-sys" / "src" / "sm100a_q.rs").read_text())
+    names = re.findall(r"\b(baracuda_kernels_(?:qk_norm_rope|kv4|attention_kv4)\w*)\(([^)]*)\)", header)
+    assert len(names) == 16
+    for name, params in names:
+        found = re.search(rf"fn {name}\(([^)]*)\)", rust)
+        assert found, name
+        assert len([x for x in found.group(1).split(",") if x.strip()]) == len(params.split(",")), name
