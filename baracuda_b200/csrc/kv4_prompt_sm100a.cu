@@ -316,6 +316,11 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const int hi_min = p.causal ? min(sq.len, past + first_i + 1) : sq.len;
         const int lo_max = p.window > 0 ? max(0, past + last_i - p.window + 1) : 0;
         const uint32_t o_tmem = tmem + lanes + t * D;
+        // The product of step j with the values completes a phase of its score slot's barrier.  A warp of the block may be a whole step
+        // ahead of another (one row block: S(j + 1) is there before P(j) is), never two: S(j) is issued after the product of step j
+        // less the number of slots, so a slot's barrier is at most in the phase that is waited for, and its parity tells.
+        auto pv_slot = [&](int j) { return NQ == 2 ? t : j & 1; };
+        auto pv_parity = [](int j) { return static_cast<uint32_t>(NQ == 2 ? j : j >> 1) & 1u; };
         float ref = KV4_NO_REF, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < n; ++j) {
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     ref = to;
                     l *= fix;
                     if (j > 0) {
-                        if (!mbar_wait_bounded(&bar->pvdone[t], (j - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+                        if (!mbar_wait_bounded(&bar->pvdone[pv_slot(j - 1)], pv_parity(j - 1), abort_word, KV4_WAIT_LIMIT)) {
                             give_up(abort_word, 413);
                             ok = false;
                         }
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         }
         // ---------------------------------------------------------------- output
         if (n > 0 && ok && *abort_word == 0u) {
-            if (!mbar_wait_bounded(&bar->pvdone[t], (n - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+            if (!mbar_wait_bounded(&bar->pvdone[pv_slot(n - 1)], pv_parity(n - 1), abort_word, KV4_WAIT_LIMIT)) {
                 give_up(abort_word, 414);
                 ok = false;
             }
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
 #pragma unroll
                 for (int ks = 0; ks < KT / 16; ++ks)
                     umma_f16_ts(to, from + ks * 8, v + ((ks >> 2) * (D * 128 / 16) + (ks & 3) * 2), IDESC_O, ks > 0 ? 1u : more);
-                umma_commit(&bar->pvdone[t]);
+                umma_commit(&bar->pvdone[slot]);
                 if (t == NQ - 1) umma_commit(&bar->vfree[j & 1]);
             }
             __syncwarp();
