@@ -10,6 +10,12 @@
 // Bound: bytes (each element read and written once), once the instructions per head are few: a head is D / 16 lanes of 16
 // channels, which contain whole rotation pairs, so nothing is exchanged between lanes but the sums and the groups' extrema; a
 // warp takes twice 512 / D heads of one token, whose sums share their exchanges, division and square root.
+//
+// Measured (B200): 4097 tokens of 28 + 4 heads of 128, three axes, dense output: 25.8 us (2.7 TB/s; a plain copy takes 12, this
+// structure without norm and rotation 15); 8191 tokens of 64 + 8 + 8 heads into the cache: 99 us, and 11 to read them back; 5 tokens:
+// 2.8 us.  Reading 65537 tokens of 8 heads: 57 us, 6.0 TB/s.  Half of the issue slots are used: what is left is the chain position
+// -> angles -> product within a warp and the ramp at both ends.  With 8 heads a warp in fragment order, sums of squares from
+// mma.sync and a loop over blocks of heads, the same cases took 29.6 and 131 us: its angles and weights need twice the registers.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -20,6 +20,11 @@
 // issues the copy, the pages of the next 32 tiles are looked up at once), so the main loop has no CTA-wide synchronisation.
 // Warps are joined in shared memory, parts of a block through the workspace by a second kernel (in the order of the keys: the
 // result does not depend on timing).
+//
+// Measured (B200), 32 query and 8 kv heads of 128 unless said: one sequence of 129 tokens 6.2 us; 64 ragged ones up to 4001 tokens
+// (179 MB) 48.8 us, 7 TB/s inside the loop; 2 x 131071 tokens with 64 query heads 64.4 us, 4.7 TB/s over all; 16 x 5 drafted tokens
+// over up to 6001 with 40 heads 49.7 us: 25 rows of a kv head are two blocks of 16, whose products and softmax are the bound.  Blocks of
+// 24 rows spilled and took 41 us against 41 (24 rows, 16 x 6000) and 60 against 54 (48 rows).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
