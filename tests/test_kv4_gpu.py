@@ -687,3 +687,74 @@ def test_blocks_whose_warps_run_apart_agree_every_time(lens, heads_q, heads_kv, 
     for _ in range(25):
         again = p.run()
         assert torch.equal(again.out, first.out) and torch.equal(again.lse, first.lse)
+
+
+@pytest.mark.parametrize("dim,rot,interleaved", [(64, 64, False), (128, 128, True), (256, 64, False)])
+@pytest.mark.parametrize("tokens", [1, 37, 1500])
+@pytest.mark.parametrize("weights", ["q", "k"])
+def test_norm_of_one_side_keys_alone_and_rows_on_eight_bytes(tokens, dim, rot, interleaved, weights):
+    """Only queries or only keys are normed; no queries at all; matrices that begin and step by 8 bytes."""
+    hq, hkv = 9, 3
+    qkv, (wq, wk), positions, _, angles = _norm_inputs(tokens, hq, hkv, dim, rot, None, tokens + dim)
+    wide = torch.full((tokens, qkv.shape[1] + 12), 3.0, dtype=BF16, device="cuda")
+    wide[:, 4:-8] = qkv
+    q, k = wide[:, 4 : 4 + hq * dim], wide[:, 4 + hq * dim : 4 + (hq + hkv) * dim]
+    wq, wk = (wq, None) if weights == "q" else (None, wk)
+    out = torch.full((tokens, (hq + hkv) * dim + 4), 7.0, dtype=BF16, device="cuda")
+    args = bq.QkNormRopeArgs(q=q, k=k, q_out=out[:, 4 : 4 + hq * dim], k_out=out[:, 4 + hq * dim :], q_weight=wq, k_weight=wk, cos_sin=angles, positions=positions)
+    bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(tokens, hq, hkv, dim, rot_dim=rot, interleaved=interleaved)).run(None, None, args)
+    alone = torch.empty(tokens, hkv * dim, dtype=BF16, device="cuda")
+    bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(tokens, 0, hkv, dim, rot_dim=rot, interleaved=interleaved)).run(
+        None, None, bq.QkNormRopeArgs(q=None, k=k, k_out=alone, k_weight=wk, cos_sin=angles, positions=positions))
+    torch.cuda.synchronize()
+    assert bq.device_status() == 0
+    for x, got, heads, w in ((q, args.q_out, hq, wq), (k, args.k_out, hkv, wk), (k, alone, hkv, wk)):
+        want, tol = ref.norm_rope(x, heads, dim, w, 1e-6, angles, positions, None, rot, interleaved)
+        assert torch.all((got.double().reshape(want.shape) - want).abs() <= tol)
+    assert torch.equal(alone, args.k_out) and torch.all(out[:, :4] == 7) and torch.all(wide[:, :4] == 3) and torch.all(wide[:, -8:] == 3)
+
+
+def test_a_captured_step_with_a_padded_batch():
+    """Norm, rotation and append, then attention, captured once; replayed with other tokens, positions, slots and lengths, and rows of
+    padding: they write nothing to the cache and get zeros."""
+    hq, hkv, dim, page, batch = 8, 2, 128, 16, 6
+    desc, cache = _cache(40, page, hkv, dim)
+    qkv, (wq, wk), positions, _, angles = _norm_inputs(batch, hq, hkv, dim, dim, None, 8)
+    q, k, v = qkv[:, : hq * dim], qkv[:, hq * dim : (hq + hkv) * dim], qkv[:, (hq + hkv) * dim :]
+    slots, lens = torch.full((batch,), -1, device="cuda"), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    table = torch.arange(36, dtype=torch.int32, device="cuda").reshape(batch, 6)
+    q_out, out = torch.empty(batch, hq * dim, dtype=BF16, device="cuda"), torch.empty(batch, hq * dim, dtype=BF16, device="cuda")
+    rope = bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(batch, hq, hkv, dim, cache=desc))
+    attend = bq.Kv4AttentionPlan.select(None, bq.Kv4AttentionDescriptor(batch, 1, 6 * page, hq, desc))
+    space = torch.empty(attend.workspace_size(), dtype=torch.uint8, device="cuda")
+    rope_args = bq.QkNormRopeArgs(q=q, k=k, v=v, q_out=q_out, q_weight=wq, k_weight=wk, cos_sin=angles, positions=positions, cache=cache, slots=slots)
+    attend_args = bq.Kv4AttentionArgs(q=q_out, cu_q=torch.arange(batch + 1, dtype=torch.int32, device="cuda"), kv_lens=lens, page_table=table,
+                                      cache=cache, out=out)
+
+    def step():
+        rope.run(None, None, rope_args)
+        attend.run(None, space, attend_args)
+
+    step()
+    torch.cuda.synchronize()
+    empty = cache.clone()
+    assert torch.all(cache == 255) and not out.any()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = _gen(77)
+    held = torch.zeros(batch, dtype=torch.long)
+    for i in range(20):
+        live = torch.tensor([(i + b) % 3 != 0 and b != 4 for b in range(batch)])  # sequence 4 is padding throughout
+        qkv.copy_(_randn(g, *qkv.shape).to(BF16))
+        slots.copy_(torch.where(live, table[:, 0].cpu().long() * page + held, -1))
+        held += live
+        positions[0].copy_(held.to(torch.int32))
+        lens.copy_(torch.where(live, held, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bq.device_status() == 0
+        want, _, tol, _ = ref.attention(q_out, attend_args.cu_q, lens, table, cache, page, hkv, dim, dim ** -0.5, True, 0)
+        assert torch.all((out.double().reshape(want.shape) - want).abs() <= tol)
+        assert not out[~live.cuda()].any()
+    assert torch.equal(cache[24:30], empty[24:30]) and torch.equal(cache[36:], empty[36:])
