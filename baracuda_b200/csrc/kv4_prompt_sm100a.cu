@@ -135,8 +135,9 @@ __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<con
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 
 // 2^x of a pair on the FMA units, x at most 16: n = rint(x), 2^(x - n) by the polynomial of degree 4 that is nearest in relative
-// error on [-1/2, 1/2] (Remez exchange; 2.7e-6 with its f32 roundings), n added to the exponent.  Below 2^-125 the result is no more
-// than that.  The special function unit takes 8 clocks for a warp's results, 2048 for 256 rows x 128 keys, so some are computed here.
+// error on [-1/2, 1/2] (Remez exchange; 2.7e-6 with its f32 roundings), n added to the exponent.  Below 2^-125, and of a NaN, the
+// result is no more than that.  The special function unit takes 8 clocks for a warp's results, 2048 for 256 rows x 128 keys, so some
+// are computed here.
 __device__ __forceinline__ float2 ex2_pair(float2 x) {
     const f32x2 magic = both(12582912.0f, 12582912.0f), back = both(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
     const f32x2 v = both(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 // the common step in one reading: P with the reference as it is, and the maximum that tells whether it holds; P goes
                 // over S only then
                 const f32x2 base2 = both(PR_LIFT - ref, PR_LIFT - ref);
-                f32x2 sum[2] = {0ull, 0ull};
+                f32x2 sum[2] = {0ull, 0ull}, nan2 = 0ull;  // nan2: 0, or NaN for a NaN among the polynomial's scores; the row's sum takes it over
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 uint32_t pk[KT / 32][16];
                 constexpr int CH = D == 256 ? 32 : 64;
@@ -382,6 +383,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                         const float2 w = each(fma2(both(s0, s1), factor2, base2));
                         const float2 pr = (e & PR_POLY_MASK) == PR_POLY_AT ? ex2_pair(w) : make_float2(ex2(w.x), ex2(w.y));
                         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], both(pr.x, pr.y));
+                        if ((e & PR_POLY_MASK) == PR_POLY_AT) nan2 = fma2(both(s0, s1), 0ull, nan2);  // the polynomial makes a number of a NaN
                         pk[CH / 32 * x + (e >> 5)][(e & 31) / 2] = pack_half2(pr.x, pr.y);
                     }
                 }
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     done = true;
 #pragma unroll
                     for (int x = 0; x < KT / 32; ++x) tmem_st_32x32b_x16(s_tmem + 16 * x, pk[x]);
-                    const float2 total = each(add2(sum[0], sum[1]));
+                    const float2 total = each(add2(add2(sum[0], sum[1]), nan2));
                     l += total.x + total.y;
                 }
             } else {

@@ -758,3 +758,24 @@ def test_a_captured_step_with_a_padded_batch():
         assert torch.all((out.double().reshape(want.shape) - want).abs() <= tol)
         assert not out[~live.cuda()].any()
     assert torch.equal(cache[24:30], empty[24:30]) and torch.equal(cache[36:], empty[36:])
+
+
+# ------------------------------------------------------------------------------------------------ far ends of the ranges
+@pytest.mark.parametrize("rows,dim", [(60, 64), (160, 64), (60, 128), (200, 128), (140, 256)])
+def test_a_nan_key_reaches_every_row_wherever_it_lies_in_its_tile(rows, dim):
+    """Each of the 16 places, in a step that all rows see in full and that comes when the softmax's reference has settled; the values are numbers."""
+    page, first = 16, 256
+    p = Problem([(rows, 700)], 2, 1, dim, page, seed=rows + dim)
+    p.check(p.run())
+    clean = p.cache.clone()
+    codes, s, m = ref.unpack(p.cache, page, 1, dim)
+    for place in range(16):
+        slot = p.table[0].long()[first // page] * page + place
+        k, v = (ref.values(codes[i], s[i], m[i])[slot].reshape(1, 1, dim).to(BF16) for i in (0, 1))
+        k[0, 0, 7] = math.nan
+        p.cache.copy_(clean)
+        ref.fill(p.cache, page, 1, dim, slot.reshape(1), k, v)
+        got = p.run()
+        torch.cuda.synchronize()
+        assert got.out[:rows].isnan().all() and got.lse[:rows].isnan().all(), place
+    assert bq.device_status() == 0
