@@ -895,6 +895,8 @@ int32_t baracuda_kernels_q_selftest_bounded_wait(int64_t limit_cycles, void* str
     return bq::launch_bounded_wait_selftest(static_cast<long long>(limit_cycles), static_cast<cudaStream_t>(stream));
 }
 
+int32_t baracuda_kernels_q_selftest_kv4_waits(int64_t limit_cycles) { return bq::set_kv4_wait_selftest(limit_cycles); }
+
 int32_t baracuda_kernels_q_set_tuning(int32_t key, int32_t value) {
     switch (key) {
         case 0:

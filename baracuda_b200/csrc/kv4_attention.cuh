@@ -28,10 +28,20 @@ struct AttnParams {
     int32_t causal, window;
     int32_t batch, total_q, max_q, max_kv, heads_q, group;
     int32_t row_tiles, splits, tile_rows;  // blocks of query rows of a kv head, slices of the keys, rows of a block
+    int32_t ctas;                          // of the launch
     float* part_o;   // [tile][split][rows][D]
     float2* part_ml; // [tile][split][rows]
     int2* shares;    // null, or of each block of rows: place of its first part, CTA of its last; part_o is then [CTA][2][rows][D]
+    int32_t stall;         // 1: barriers that nothing completes (the self-test of the waits)
+    long long wait_limit;  // of every wait, in cycles
 };
+
+// How many parts a block of rows has by its entry in `shares`; 0 for an entry that no CTA of the launch can have written: one that
+// gave up a wait leaves those of its later blocks as they were, and the workspace may hold anything.
+__device__ __forceinline__ int parts_of_share(int2 share, int ctas) {
+    if (share.x < 0 || share.x >= 2 * ctas || share.y < share.x / 2 || share.y >= ctas) return 0;
+    return share.y - share.x / 2 + 1;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -69,7 +79,7 @@ struct AttnShape {
     int64_t tiles, ctas;
     bool joined;    // a second kernel adds parts of blocks
 };
-int32_t launch_kv4_prompt(AttnParams& p, const AttnShape& s, cudaStream_t stream);
+int32_t launch_kv4_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stream);
 int32_t read_and_clear_kv4_prompt_device_status();
 
 }  // namespace bq

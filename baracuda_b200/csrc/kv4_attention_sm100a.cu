@@ -49,6 +49,7 @@ constexpr int AT_STAGES = 2;  // the parts of a CTA alternate between them: not 
 constexpr int AT_MOST_ROWS = 48, AT_MOST_ROWS_256 = 32;
 constexpr float SLACK = 4.0f;  // a new reference leaves this many powers of two before the next
 constexpr int AT_ASSUMED_SMS = 148;  // the workspace's size must not depend on the device that asks
+thread_local long long t_wait_selftest = 0;  // 0, or the limit of waits whose barriers are not to be completed
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
     uint8_t* ring = smem + warp * L::STAGE;  // stages AT_WARPS * STAGE apart
     if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < AT_STAGES; ++s) mbar_init(&bars[s], 1);
+        for (int s = 0; s < AT_STAGES; ++s) mbar_init(&bars[s], 1 + p.stall);
         fence_barrier_init();
     }
     __syncwarp();
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         if (!mbar_try_wait(&bars[stage], parity)) {
             const long long t0 = clock64();
             while (!mbar_try_wait(&bars[stage], parity)) {
-                if (clock64() - t0 > KV4_WAIT_LIMIT) {
+                if (clock64() - t0 > p.wait_limit) {
                     gave_up = true;
                     break;
                 }
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         const long long t0 = clock64();
         for (int s = 0; s < AT_STAGES; ++s) {
             if (k + s >= mine) break;
-            while (!mbar_try_wait(&bars[stage], (phases >> stage) & 1u) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            while (!mbar_try_wait(&bars[stage], (phases >> stage) & 1u) && clock64() - t0 < p.wait_limit) {
             }
             phases ^= 1u << stage;
             stage ^= 1;
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
     if (__syncthreads_or(gave_up)) {
         if (more && then.mine > 0 && !gave_up) {
             const long long t0 = clock64();
-            while (!mbar_try_wait(&bars[0], phases & 1u) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            while (!mbar_try_wait(&bars[0], phases & 1u) && clock64() - t0 < p.wait_limit) {
             }
         }
         return;
@@ -736,8 +737,9 @@ __global__ void __launch_bounds__(128) kv4_attention_join_kernel(const __grid_co
     int64_t first = tile_id * p.splits, second = first + 1, stride = 1;
     if (p.shares != nullptr) {
         const int2 share = p.shares[tile_id];
-        parts = share.y - share.x / 2 + 1;
-        if (parts == 1) return;
+        parts = parts_of_share(share, p.ctas);
+        if (parts == 0) atomicCAS(&g_kv4_attention_device_status, 0, 411);
+        if (parts <= 1) return;
         first = share.x, second = share.x / 2 * 2 + 2, stride = 2;
     }
     auto place = [&](int s) { return (s == 0 ? first : second + (s - 1) * stride) * rows_of_tile + row; };
@@ -827,7 +829,7 @@ int32_t launch_rows(const AttnParams& p, const AttnShape& s, cudaStream_t stream
 }
 
 template <int D>
-int32_t launch_d(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
+int32_t launch_d(const AttnParams& p, const AttnShape& s, cudaStream_t stream) {
     int32_t st;
     if (s.tensor) {
         st = launch_kv4_prompt(p, s, stream);
@@ -893,6 +895,9 @@ int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
     p.row_tiles = s.row_tiles;
     p.splits = s.splits;
     p.tile_rows = s.tile_rows;
+    p.ctas = static_cast<int32_t>(s.ctas);
+    p.stall = t_wait_selftest != 0;
+    p.wait_limit = p.stall ? t_wait_selftest : KV4_WAIT_LIMIT;
     p.part_o = static_cast<float*>(g.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + parts_of(s) * g.cache.head_dim);
     p.shares = s.tensor || !s.joined ? nullptr : reinterpret_cast<int2*>(p.part_ml + parts_of(s));
@@ -902,6 +907,13 @@ int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
         case 256: return launch_d<256>(p, s, stream);
         default: return BQ_STATUS_UNSUPPORTED;
     }
+}
+
+int32_t set_kv4_wait_selftest(int64_t limit_cycles) {
+    // long enough for every copy in flight to arrive meanwhile, a sixth of a second at most
+    if (limit_cycles != 0 && (limit_cycles < (1LL << 20) || limit_cycles > (1LL << 28))) return BQ_STATUS_INVALID_PROBLEM;
+    t_wait_selftest = limit_cycles;
+    return BQ_STATUS_OK;
 }
 
 int32_t read_and_clear_kv4_attention_device_status() {

@@ -143,6 +143,7 @@ size_t kv4_attention_workspace_bytes(int32_t batch, int32_t max_q, int32_t max_k
 // Whether the launch's block count fits a grid.
 bool kv4_attention_fits(int32_t batch, int32_t max_q, int32_t max_kv, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
 int32_t read_and_clear_kv4_attention_device_status();
+int32_t set_kv4_wait_selftest(int64_t limit_cycles);
 
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;

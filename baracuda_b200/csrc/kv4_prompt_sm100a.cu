@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
             mbar_init(&bar->kfull[s], C::FEED_WARPS);
-            mbar_init(&bar->vfull[s], C::FEED_WARPS);
+            mbar_init(&bar->vfull[s], C::FEED_WARPS + p.stall);
             mbar_init(&bar->kfree[s], 1);
             mbar_init(&bar->vfree[s], 1);
             mbar_init(&bar->sfull[s], 1);
@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             const int slot = NQ == 2 ? t : j & 1;
             const uint32_t slot_parity = (NQ == 2 ? j : j >> 1) & 1;
             const uint32_t s_tmem = tmem + lanes + C::S_COL + slot * KT;
-            if (!mbar_wait_bounded(&bar->vfull[j & 1], (j >> 1) & 1, abort_word, KV4_WAIT_LIMIT) ||
-                !mbar_wait_bounded(&bar->sfull[slot], slot_parity, abort_word, KV4_WAIT_LIMIT)) {
+            if (!mbar_wait_bounded(&bar->vfull[j & 1], (j >> 1) & 1, abort_word, p.wait_limit) ||
+                !mbar_wait_bounded(&bar->sfull[slot], slot_parity, abort_word, p.wait_limit)) {
                 give_up(abort_word, 412);
                 ok = false;
             }
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     ref = to;
                     l *= fix;
                     if (j > 0) {
-                        if (!mbar_wait_bounded(&bar->pvdone[pv_slot(j - 1)], pv_parity(j - 1), abort_word, KV4_WAIT_LIMIT)) {
+                        if (!mbar_wait_bounded(&bar->pvdone[pv_slot(j - 1)], pv_parity(j - 1), abort_word, p.wait_limit)) {
                             give_up(abort_word, 413);
                             ok = false;
                         }
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         }
         // ---------------------------------------------------------------- output
         if (n > 0 && ok && *abort_word == 0u) {
-            if (!mbar_wait_bounded(&bar->pvdone[pv_slot(n - 1)], pv_parity(n - 1), abort_word, KV4_WAIT_LIMIT)) {
+            if (!mbar_wait_bounded(&bar->pvdone[pv_slot(n - 1)], pv_parity(n - 1), abort_word, p.wait_limit)) {
                 give_up(abort_word, 414);
                 ok = false;
             }
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         auto step = [&](int j) -> bool {
             const int stage = j & 1;
             bool ok = true;
-            if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+            if (j >= 2 && !mbar_wait_bounded(&bar->kfree[stage], ((j >> 1) - 1) & 1, abort_word, p.wait_limit)) {
                 give_up(abort_word, 415);
                 ok = false;
             }
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             if (lane == 0) mbar_arrive(&bar->kfull[stage]);
             // the look-up of the next 32 steps must not replace what earlier steps' values still go by: they are loaded already
             if (j + 1 < n) load_keys(j + 1);
-            if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, KV4_WAIT_LIMIT)) {
+            if (j >= 2 && !mbar_wait_bounded(&bar->vfree[stage], ((j >> 1) - 1) & 1, abort_word, p.wait_limit)) {
                 give_up(abort_word, 415);
                 ok = false;
             }
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const uint64_t k_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::K_OFF), v_desc = umma_desc_kmajor_sw128(smem_u32(smem) + C::V_OFF);
         bool ok = true;
         auto wait = [&](uint64_t* what, uint32_t parity) {
-            if (ok && !mbar_wait_bounded(what, parity, abort_word, KV4_WAIT_LIMIT)) {
+            if (ok && !mbar_wait_bounded(what, parity, abort_word, p.wait_limit)) {
                 give_up(abort_word, 416);
                 ok = false;
             }
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             // nothing of this thread's may be in flight when the TMEM is given back
             commit(&bar->done);
             const long long t0 = clock64();
-            while (!mbar_try_wait(&bar->done, 0u) && clock64() - t0 < KV4_WAIT_LIMIT) {
+            while (!mbar_try_wait(&bar->done, 0u) && clock64() - t0 < p.wait_limit) {
             }
         }
     }
@@ -815,7 +815,7 @@ int32_t launch_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stre
 
 }  // namespace
 
-int32_t launch_kv4_prompt(AttnParams& p, const AttnShape& s, cudaStream_t stream) {
+int32_t launch_kv4_prompt(const AttnParams& p, const AttnShape& s, cudaStream_t stream) {
     switch (p.cache.head_dim) {
         case 64: return s.tile_rows == 256 ? launch_prompt<64, 2>(p, s, stream) : launch_prompt<64, 1>(p, s, stream);
         case 128: return s.tile_rows == 256 ? launch_prompt<128, 2>(p, s, stream) : launch_prompt<128, 1>(p, s, stream);

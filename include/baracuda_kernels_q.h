@@ -831,9 +831,13 @@ int32_t baracuda_q_nccl_all_gather_bytes(void* comm, int32_t world, const void* 
  * selftest_bounded_wait: launches one thread that waits, for at most limit_cycles SM clock cycles
  * (1 .. 2^28), on a barrier that nothing completes -- the time-out path of every kernel here.  After the
  * stream is synchronised device_status() returns 299 once and the context is as usable as before.
+ * selftest_kv4_waits: the CALLING THREAD's launches of the attention over the 4-bit cache wait, from here on, on barriers that
+ * nothing completes and give up after limit_cycles (2^20 .. 2^28; 0 = as they are): the outputs of the sequences' rows are then
+ * unspecified, nothing else is written, device_status() returns one of 411..416, and the context is as usable as before.
  * ------------------------------------------------------------------------- */
 int32_t baracuda_kernels_q_device_status(void);
 int32_t baracuda_kernels_q_selftest_bounded_wait(int64_t limit_cycles, void* stream);
+int32_t baracuda_kernels_q_selftest_kv4_waits(int64_t limit_cycles);
 int32_t baracuda_kernels_q_set_tuning(int32_t key, int32_t value);
 
 #ifdef __cplusplus

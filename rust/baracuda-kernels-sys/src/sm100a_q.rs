@@ -516,6 +516,7 @@ extern "C" {
     /// whose only thread waits `limit_cycles` on a barrier nothing completes (status 299 afterwards).
     pub fn baracuda_kernels_q_set_tuning(key: i32, value: i32) -> i32;
     pub fn baracuda_kernels_q_selftest_bounded_wait(limit_cycles: i64, stream: *mut c_void) -> i32;
+    pub fn baracuda_kernels_q_selftest_kv4_waits(limit_cycles: i64) -> i32;
 
     /// Read-and-clear of the word a kernel sets when one of its bounded waits ran out (0 = none).
     pub fn baracuda_kernels_q_device_status() -> i32;

@@ -779,3 +779,33 @@ def test_a_nan_key_reaches_every_row_wherever_it_lies_in_its_tile(rows, dim):
         torch.cuda.synchronize()
         assert got.out[:rows].isnan().all() and got.lse[:rows].isnan().all(), place
     assert bq.device_status() == 0
+
+
+@pytest.mark.parametrize("lens,heads_q,heads_kv,dim,statuses", [([(1, 600)] * 300, 4, 2, 128, (411,)), ([(3, 400 + 31 * i) for i in range(40)], 4, 4, 64, (411,)),
+                                                                ([(2, 20000)], 2, 1, 256, (411,)), ([(200, 900), (150, 400)], 4, 2, 128, range(412, 417)),
+                                                                ([(60, 2000)], 2, 1, 64, range(412, 417)), ([(140, 700), (40, 300)], 2, 1, 256, range(412, 417))])
+def test_waits_that_run_out_are_reported(qlib, lens, heads_q, heads_kv, dim, statuses):
+    """Barriers that nothing completes: the call ends with a status, whatever the workspace held, writes to its sequences' rows alone, and
+    the next call is as good as any."""
+    p = Problem(lens, heads_q, heads_kv, dim, 16, seed=len(lens))
+    good = p.run()
+    p.check(good)
+    plan = p.plan()
+    g = _gen(2)
+    for fill in (0, 0x7F, 0x80, 0xFF, None):
+        space = torch.full((max(1, plan.workspace_size()),), fill or 0, dtype=torch.uint8, device="cuda")
+        if fill is None:
+            space.random_(0, 256, generator=g)
+        out, lse = torch.full_like(good.out._base, 7.0), torch.full_like(good.lse, 7.0)
+        args = bq.Kv4AttentionArgs(q=p.q, cu_q=p.cu_q, kv_lens=p.kv_lens, page_table=p.table, cache=p.cache, out=out[:, : heads_q * dim], lse=lse)
+        assert qlib.baracuda_kernels_q_selftest_kv4_waits(1 << 21) == 0  # about a millisecond
+        try:
+            plan.run(None, space, args)
+        finally:
+            assert qlib.baracuda_kernels_q_selftest_kv4_waits(0) == 0
+        torch.cuda.synchronize()
+        assert bq.device_status() in statuses and bq.device_status() == 0
+        assert torch.all(out[p.rows :] == 7) and torch.all(lse[p.rows :] == 7) and torch.all(out[:, heads_q * dim :] == 7)
+    again = p.run()
+    p.check(again)
+    assert torch.equal(again.out, good.out) and torch.equal(again.lse, good.lse)

@@ -174,3 +174,11 @@ def test_rust_declarations_name_the_headers_symbols():
         found = re.search(rf"fn {name}\(([^)]*)\)", rust)
         assert found, name
         assert len([x for x in found.group(1).split(",") if x.strip()]) == len(params.split(",")), name
+
+
+def test_the_self_test_of_the_waits_takes_limits_that_let_copies_arrive(qlib):
+    f = qlib.baracuda_kernels_q_selftest_kv4_waits
+    for limit in (-1, 1, (1 << 20) - 1, (1 << 28) + 1, 1 << 40):
+        assert f(limit) == 2
+    for limit in (1 << 20, 1 << 28, 0):
+        assert f(limit) == 0
