@@ -71,6 +71,9 @@ __device__ __forceinline__ Sequence sequence_of(const AttnParams& p, int b, int*
     return s;
 }
 
+// The first key that a row sees whose last one is `last` (negative: before the first).  Nothing here leaves 32 bits, whatever the window.
+__device__ __forceinline__ int first_seen(const AttnParams& p, int last) { return p.window > 0 && last >= p.window ? last - p.window + 1 : 0; }
+
 // Shape of a launch: which kernel, its blocks and slices.
 struct AttnShape {
     int tensor;     // 1: kv4_prompt_sm100a.cu, 0: kv4_attention_sm100a.cu

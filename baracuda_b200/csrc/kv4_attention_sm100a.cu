@@ -104,7 +104,7 @@ __device__ __forceinline__ Extent extent_of(const AttnParams& p, int b) {
     x.sq = sequence_of(p, b, &g_kv4_attention_device_status);
     x.blocks = (x.sq.n * p.group + ROWS - 1) / ROWS;
     const int first = x.sq.len - x.sq.n;
-    const int hi = max(0, p.causal ? min(x.sq.len, first + x.sq.n) : x.sq.len), lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    const int hi = max(0, p.causal ? min(x.sq.len, first + x.sq.n) : x.sq.len), lo = first_seen(p, first);
     x.step0 = lo / STEP;
     x.steps = max(0, (hi + STEP - 1) / STEP - x.step0);
     x.units = AT_BLOCK_UNITS + max(1, (x.steps + AT_WARPS - 1) / AT_WARPS);  // rows without keys are to be written too
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         }
         const int i = row / p.group;
         const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
-        const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
+        const int lo = first_seen(p, past + i);
         if (there) hi_min = min(hi_min, hi), lo_max = max(lo_max, lo);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
     const int past = sq.len - sq.n;
     const int i_first = rt * ROWS / p.group, i_last = (rt * ROWS + rows - 1) / p.group;
     const int hi_all = max(0, p.causal ? min(sq.len, past + i_last + 1) : sq.len);
-    const int lo_all = p.window > 0 ? max(0, past + i_first - p.window + 1) : 0;
+    const int lo_all = first_seen(p, past + i_first);
     const int step0 = lo_all / KT, steps = max(0, (hi_all + KT - 1) / KT - step0);
     const int per = (steps + p.splits - 1) / p.splits;
     const int begin = step0 + min(split * per, steps);
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 TMEM lanes
         const int i = row / p.group;
         const int hi = !there ? 0 : p.causal ? max(0, min(sq.len, past + i + 1)) : sq.len;
-        const int lo = p.window > 0 ? max(0, past + i - p.window + 1) : 0;
+        const int lo = first_seen(p, past + i);
         // this warp's 32 query rows: D / 8 lanes copy one to shared memory, all copies in flight; then each thread brings its row
         // to f16 by a power of two, to TMEM or back to its place
         const int64_t q_row = sq.row0 + (there ? i : 0);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         const int last_there = min(all_rows, rt * ROWS + t * 128 + 128) - 1;  // may lie before the block's first row
         const int first_i = (rt * ROWS + t * 128) / p.group, last_i = last_there / p.group;
         const int hi_min = p.causal ? min(sq.len, past + first_i + 1) : sq.len;
-        const int lo_max = p.window > 0 ? max(0, past + last_i - p.window + 1) : 0;
+        const int lo_max = first_seen(p, past + last_i);
         const uint32_t o_tmem = tmem + lanes + t * D;
         // The product of step j with the values completes a phase of its score slot's barrier.  A warp of the block may be a whole step
         // ahead of another (one row block: S(j + 1) is there before P(j) is), never two: S(j) is issued after the product of step j

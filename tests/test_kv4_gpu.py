@@ -809,3 +809,18 @@ def test_waits_that_run_out_are_reported(qlib, lens, heads_q, heads_kv, dim, sta
     again = p.run()
     p.check(again)
     assert torch.equal(again.out, good.out) and torch.equal(again.lse, good.lse)
+
+
+@pytest.mark.parametrize("lens,heads_q,dim", [([(9, 4), (1, 30)], 2, 128), ([(6, 1), (7, 70)], 3, 64), ([(5, 0), (8, 2)], 2, 256),
+                                              ([(100, 60), (30, 90)], 4, 128), ([(90, 7), (140, 300)], 2, 256)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_window_of_any_size_and_fewer_keys_than_rows(lens, heads_q, dim, causal):
+    """Windows up to the largest number limit nothing, also where the first rows come before the first key."""
+    p = Problem(lens, heads_q, 1, dim, 16, seed=dim, causal=causal)
+    free = p.run()
+    p.check(free)
+    for window in (300, 2 ** 31 - 9, 2 ** 31 - 1):
+        p.window = window
+        got = p.run()
+        p.check(got)
+        assert torch.equal(got.out, free.out) and torch.equal(got.lse, free.lse)
