@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
         const int step = t.my_begin + warp + (k + lane / AT_TILES) * AT_WARPS;
         const int tile = (t.step0 + step) * AT_TILES + lane % AT_TILES;
         ahead = -1;
-        if (step < t.my_end && tile * KV4_TILE < t.hi_all) {
+        // a step's first tiles may lie before the first key that the sequence's rows see: they need not be anywhere
+        if (step < t.my_end && tile * KV4_TILE < t.hi_all && (tile + 1) * KV4_TILE > first_seen(p, t.sq.len - t.sq.n)) {
             const int at = tile / tiles_per_page, page = p.table[static_cast<int64_t>(t.b) * p.ld_table + at];
             if (page >= 0 && page < p.cache.num_pages) {
                 ahead = static_cast<int64_t>(page) * p.cache.page_stride + (static_cast<int64_t>(t.hk) * tiles_per_page + tile - at * tiles_per_page) * TILE;

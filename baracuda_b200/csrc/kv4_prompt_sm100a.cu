@@ -547,7 +547,8 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         auto look_up = [&](int j) {
             const int tile = (begin + j + lane) * STEP_TILES + in_step;
             ahead = -1;
-            if (j + lane < n && tile * KV4_TILE < hi_all) {
+            // a step's first tiles may lie before the first key that a row sees: they need not be anywhere
+            if (j + lane < n && tile * KV4_TILE < hi_all && (tile + 1) * KV4_TILE > lo_all) {
                 const int at = tile / tiles_per_page, page = table[at];
                 if (page >= 0 && page < p.cache.num_pages) {
                     ahead = static_cast<int64_t>(page) * p.cache.page_stride + (tile - at * tiles_per_page) * TILE;

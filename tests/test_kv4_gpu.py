@@ -824,3 +824,23 @@ def test_a_window_of_any_size_and_fewer_keys_than_rows(lens, heads_q, dim, causa
         got = p.run()
         p.check(got)
         assert torch.equal(got.out, free.out) and torch.equal(got.lse, free.lse)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (1, 128), (3, 256), (20, 128), (160, 64), (200, 128), (140, 256)])
+def test_pages_before_every_rows_window_need_not_exist(rows, dim):
+    """A sequence gives up the pages that no row sees any more: neither their keys nor their numbers are looked at."""
+    page, length, window = 16, 730, 100
+    p = Problem([(rows, length), (1, 50)], 4, 2, dim, page, seed=rows, window=window)
+    clean = p.run()
+    p.check(clean)
+    gone = (length - rows - window + 1) // page
+    for number in (-1, p.desc.num_pages, 2 ** 31 - 1):
+        p.table[0, :gone] = number
+        got = p.run()
+        torch.cuda.synchronize()
+        assert bq.device_status() == 0
+        assert torch.equal(got.out, clean.out) and torch.equal(got.lse, clean.lse)
+    p.table[0, gone] = -1  # the first of which something is seen
+    p.run()
+    torch.cuda.synchronize()
+    assert bq.device_status() == 404
