@@ -176,7 +176,9 @@ __device__ __forceinline__ void inverse_rms(const Lane16 (&x)[IT], float eps, in
     }
     float inv;
     if constexpr (EXACT) {
-        inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fadd_rn(s[0], e[0]) * (1.0f / (16 * LPH)), eps)));
+        // a sum beyond f32 is infinite, and what the two-sums make of it is no number
+        const float sum = __fadd_rn(s[0], s[0] < INFINITY ? e[0] : 0.0f);
+        inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(sum * (1.0f / (16 * LPH)), eps)));
     } else {
         inv = rsqrtf(fmaf(s[0], 1.0f / (16 * LPH), eps));
     }

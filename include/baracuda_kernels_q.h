@@ -544,7 +544,8 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
  * NORM AND ROTATION.  q is bf16 [tokens][heads_q * head_dim], k (and v) bf16 [tokens][heads_kv * head_dim], each with its own
  * row pitch (elements), so all three may be columns of one qkv projection.  Per head:
  *   y = (x * (1 / sqrt(mean(x^2) + eps))) * weight      (f32; skipped where weight is NULL; a key's mean square is summed to
- *                                                        about 44 bits and rounded once, so its order does not matter)
+ *                                                        about 44 bits and rounded once, so its order does not matter;
+ *                                                        a sum of squares beyond f32 is infinite and its root's inverse 0)
  *   pair (a, b) -> (a * cos - b * sin, b * cos + a * sin)   over the first rot_dim channels (a multiple of 8, 0 = none): pair i
  *       is channels (i, i + rot_dim / 2), or (2 i, 2 i + 1) with interleaved != 0
  *   out = bf16(y)

@@ -844,3 +844,44 @@ def test_pages_before_every_rows_window_need_not_exist(rows, dim):
     p.run()
     torch.cuda.synchronize()
     assert bq.device_status() == 404
+
+
+@pytest.mark.parametrize("dim,interleaved", [(64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("tokens", [7, 1500])
+def test_norm_of_heads_beyond_the_range(tokens, dim, interleaved):
+    """A sum of squares beyond f32 is infinite: the head's numbers become 0, an infinite channel and its partner in the rotation NaN; a NaN
+    takes the whole head.  Queries and keys alike, and nothing of it reaches another head."""
+    heads = 12
+    g = _gen(dim)
+    x = _randn(g, tokens, 2 * heads, dim).to(BF16)
+    for at in (0, heads):  # some heads of a token among ordinary ones
+        x[3, at] = 3e38
+        x[3, at + 2, 5] = math.inf
+        x[3, at + 4, dim - 1] = -math.inf
+        x[3, at + 5] = 1e19
+        x[3, at + 7, 9] = 2e19
+        x[3, at + 8, 11] = math.nan
+    x = x.flatten(1)
+    q, k = x[:, : heads * dim], x[:, heads * dim :]
+    w = 1 + 0.3 * _randn(g, dim)
+    angles = _angles(1000, dim)
+    positions = torch.randint(0, 1000, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(tokens, heads, heads, dim, interleaved=interleaved)).run(
+        None, None, bq.QkNormRopeArgs(q=q, k=k, q_out=q_out, k_out=k_out, q_weight=w, k_weight=w, cos_sin=angles, positions=positions))
+    torch.cuda.synchronize()
+    for given, got in ((q, q_out), (k, k_out)):
+        y = given.reshape(tokens, heads, dim).float()
+        y = y * (1.0 / torch.sqrt(y.square().sum(-1, keepdim=True) / dim + 1e-6)) * w
+        c, s = angles[positions.long()][:, None].chunk(2, -1)
+        a, b = (y[..., 0::2], y[..., 1::2]) if interleaved else y.chunk(2, -1)
+        one, two = a * c - b * s, b * c + a * s
+        want = torch.stack([one, two], -1).flatten(-2) if interleaved else torch.cat([one, two], -1)
+        got = got.reshape(want.shape).float()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert not got[3, 0].any() and not got[3, 5].any() and not got[3, 7].any() and got[3, 8].isnan().all()
+        assert int(got[3, 2].isnan().sum()) == 2 and int(got[3, 4].isnan().sum()) == 2
+        # the ordinary heads: 8 roundings of f32 and one of bf16 over two terms, as in the tests above
+        live = torch.tensor([h for h in range(heads) if h not in (0, 2, 4, 5, 7, 8)], device="cuda")
+        true, tol = ref.norm_rope(given.reshape(tokens, heads, dim)[:, live].flatten(1), len(live), dim, w, 1e-6, angles, positions, None, dim, interleaved)
+        assert torch.all((got[:, live].double() - true).abs() <= tol)
