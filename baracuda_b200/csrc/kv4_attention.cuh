@@ -10,7 +10,8 @@
 
 namespace bq {
 
-constexpr float KV4_NO_REF = -1.0e30f;                    // the softmax's reference before the first key
+constexpr float KV4_NO_REF = -3.0e38f;                    // the softmax's reference before the first key: below every score
+constexpr float KV4_FAR = 1048576.0f;                     // scores (log2) up to here have steps of 2^-3 at most
 constexpr long long KV4_WAIT_LIMIT = 2000000000LL;        // cycles: about a second
 
 struct AttnParams {

@@ -591,7 +591,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const bool move = top[nt][e] > cap || (fresh[nt][e] && top[nt][e] > -INFINITY);
-                    const float by = move ? top[nt][e] - (cap - SLACK) : 0.0f;
+                    // where a step of f32 is no small number of powers of two, the largest itself is the reference
+                    const float by = !move ? 0.0f : fabsf(ref[nt][e] + top[nt][e]) > KV4_FAR ? top[nt][e] : top[nt][e] - (cap - SLACK);
                     fix[e] = fresh[nt][e] ? 1.0f : ex2(-by);  // nothing to rescale before the first key
                     fresh[nt][e] = fresh[nt][e] && !move;
                     ref[nt][e] += by;

@@ -63,7 +63,8 @@ struct PromptCfg {
     static constexpr int V_OFF = K_OFF + 2 * K_BYTES;
     static constexpr int BAR_OFF = V_OFF + 2 * K_BYTES;
     static constexpr int FLAG_OFF = BAR_OFF + 192;           // [2][dead, nan][FEED_WARPS] halfwords
-    static constexpr int TOTAL = FLAG_OFF + 2 * 2 * FEED_WARPS * 2 + 1024;  // + alignment slack
+    static constexpr int FAR_OFF = FLAG_OFF + 2 * 2 * FEED_WARPS * 2;       // [row] f32
+    static constexpr int TOTAL = FAR_OFF + NQ * 128 * 4 + 1024;             // + alignment slack
     static constexpr uint32_t S_COL = NQ * D;                // TMEM columns: O of each block, then two S
     static constexpr uint32_t Q_COL = S_COL + 2 * KT;        // then the queries, where there is room for them
     static constexpr bool Q_TMEM = Q_COL + NQ * D / 2 <= 512;
@@ -322,6 +323,11 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         // less the number of slots, so a slot's barrier is at most in the phase that is waited for, and its parity tells.
         auto pv_slot = [&](int j) { return NQ == 2 ? t : j & 1; };
         auto pv_parity = [](int j) { return static_cast<uint32_t>(NQ == 2 ? j : j >> 1) & 1u; };
+        // A reference beyond KV4_FAR lies in shared memory, with KV4_NO_REF in its place: such a row takes the path that reads S twice in
+        // every step, where its scores are brought down to that size, so that one operation is exact enough for them (the keys that this
+        // brings near the first are those whose scores the roundings of their operands could have exchanged).
+        float* far_ref = reinterpret_cast<float*>(smem + C::FAR_OFF) + t * 128 + in_block;
+        *far_ref = KV4_NO_REF;
         float ref = KV4_NO_REF, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < n; ++j) {
@@ -408,10 +414,17 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 mx *= factor;
             }
             if (!done) {
+                float shrink = 1.0f, slow_ref = ref;
                 if (__any_sync(0xffffffffu, mx > ref + PR_SLACK)) {
-                    const float to = mx > ref + PR_SLACK ? mx : ref;
-                    const float fix = ex2(ref - to);
-                    ref = to;
+                    float fix = 1.0f;
+                    if (mx > ref + PR_SLACK) {
+                        const float from = ref > KV4_NO_REF ? ref : *far_ref, to = fmaxf(from, mx);
+                        const bool far = fabsf(to) > KV4_FAR;
+                        if (far) *far_ref = to, shrink = KV4_FAR / fabsf(to);
+                        ref = far ? KV4_NO_REF : to;
+                        slow_ref = to * shrink;
+                        fix = ex2((from - to) * shrink);
+                    }
                     l *= fix;
                     if (j > 0) {
                         if (!mbar_wait_bounded(&bar->pvdone[pv_slot(j - 1)], pv_parity(j - 1), abort_word, p.wait_limit)) {
@@ -432,7 +445,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                         tmem_st_wait();
                     }
                 }
-                const f32x2 base2 = both(PR_LIFT - ref, PR_LIFT - ref);
+                const f32x2 slow2 = both(factor * shrink, factor * shrink), base2 = both(PR_LIFT - slow_ref, PR_LIFT - slow_ref);
                 f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll 1
                 for (int x = 0; x < KT / 32; ++x) {
@@ -443,7 +456,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float2 v = each(fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), factor2, base2));
+                        float2 v = each(fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), slow2, base2));
                         v.x = ((seen >> e) & 1u) == 0u ? -INFINITY : ((bad >> e) & 1u) ? NAN : v.x;
                         v.y = ((seen >> (e + 1)) & 1u) == 0u ? -INFINITY : ((bad >> (e + 1)) & 1u) ? NAN : v.y;
                         const float p0 = ex2(v.x), p1 = ex2(v.y);
@@ -524,7 +537,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
                 __syncwarp();
             }
             if (there) {
-                const float m = l == 0.0f ? KV4_NO_REF : ref - PR_LIFT;
+                const float m = l == 0.0f ? KV4_NO_REF : (ref > KV4_NO_REF ? ref : *far_ref) - PR_LIFT;
                 if (p.splits > 1) {
                     p.part_ml[part] = make_float2(m, l);
                 } else if (p.lse != nullptr) {

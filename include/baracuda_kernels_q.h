@@ -572,7 +572,8 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
  *   j < kv_lens[b], with causal != 0 also j <= kv_lens[b] - n + i, with window > 0 also j > kv_lens[b] - n + i - window.
  * out = sum_j softmax_j(scale * q . k[j]) v[j], rounded once; a row that sees no key gets zeros.  lse, float
  * [total_q][heads_q] or NULL, gets log sum_j exp(scale * q . k[j]), minus infinity for such a row.  A NaN key makes the rows that
- * see it NaN, a NaN value at least the channels of its group in them.  Rows outside every sequence are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
+ * see it NaN, a NaN value at least the channels of its group in them.  Scores may have any size that f32 holds; beyond 2^20, keys
+ * whose scores differ by less than their roundings may weigh alike.  Rows outside every sequence are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
  * by them, and the workspace (16-byte aligned) needs no initialisation; two launches that may overlap need one each.
  * Lengths beyond max_q, max_kv or total_q are cut and reported as device status 403; a page number outside [0, num_pages)
  * where a key is seen leaves its keys out and is reported as 404.

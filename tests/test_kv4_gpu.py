@@ -885,3 +885,31 @@ def test_norm_of_heads_beyond_the_range(tokens, dim, interleaved):
         live = torch.tensor([h for h in range(heads) if h not in (0, 2, 4, 5, 7, 8)], device="cuda")
         true, tol = ref.norm_rope(given.reshape(tokens, heads, dim)[:, live].flatten(1), len(live), dim, w, 1e-6, angles, positions, None, dim, interleaved)
         assert torch.all((got[:, live].double() - true).abs() <= tol)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (1, 128), (2, 256), (60, 128), (150, 64), (150, 128), (140, 256)])
+@pytest.mark.parametrize("gain", [1e5, 1e8, 1e12, 1e33])
+@pytest.mark.parametrize("length", [1, 400])
+def test_attention_of_far_scores_takes_one_key(rows, dim, gain, length):
+    """Scores far beyond what f32 holds to a unit, of either sign: where one is ahead its value comes out; of a single key, always."""
+    p = Problem([(rows, length)], 2, 1, dim, 16, seed=dim, q_gain=1.0, causal=False)
+    p.q.copy_(p.q.float() * gain)
+    got = p.run()
+    codes, s, m = ref.unpack(p.cache, 16, 1, dim)
+    place = torch.arange(length, device="cuda")
+    slots = p.table[0].long()[place // 16] * 16 + place % 16
+    k, v = (ref.values(codes[i, slots, 0], s[i, slots, 0], m[i, slots, 0]) for i in (0, 1))
+    x, mag = p.q[:rows].double().reshape(rows, 2, dim), ref.values(codes[0, slots, 0], s[0, slots, 0], m[0, slots, 0].abs())
+    top, best = torch.nn.functional.pad(x @ k.T, (0, 1), value=-math.inf).topk(2, -1)
+    # ahead by more than the roundings of two scores (as the reference counts them) and 40 nats
+    off = (x.abs() @ mag.T).amax(-1) * ((dim + 8) * 2.0 ** -23 + 2 * ref.HALF_F16)
+    sure = (top[..., 0] - top[..., 1] - 2 * off) * p.scale > 40.0
+    assert sure.any()
+    torch.cuda.synchronize()
+    want = v[best[..., 0]]
+    # one weight of 1: codes, scale and minimum in f16 products and f32 sums, one rounding to f16 at most, then bf16
+    err = (got.out[:rows].double().reshape(want.shape) - want).abs()
+    assert torch.isfinite(got.out[:rows]).all() and torch.all(err[sure] <= (2.0 ** -8 * want.abs() + 2.0 ** -10 * v.abs().amax())[sure])
+    lse = top[..., 0] * p.scale
+    assert torch.all((got.lse[:rows].double() - lse).abs()[sure] <= (off * p.scale + 2.0 ** -20 * lse.abs())[sure])
+    assert bq.device_status() == 0
