@@ -29,6 +29,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 
 #include <type_traits>
 
@@ -300,23 +301,23 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
                 raw[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 8);
             }
             const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(raw);
-            sums[g] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[g][2 * e] = __low2float(h[e]);
                 x[g][2 * e + 1] = __high2float(h[e]);
                 top = fmaxf(top, fmaxf(fabsf(x[g][2 * e]), fabsf(x[g][2 * e + 1])));
-                sums[g] += x[g][2 * e] + x[g][2 * e + 1];
             }
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;  // 2^-ex brings the largest into [2^14, 2^15)
-        ex = max(-100, min(100, ex));
-        if (top == 0.0f || top > 3.0e38f) ex = 0;
+        ex = top == 0.0f || top == INFINITY ? 0 : max(-100, ex);  // at most 113
         const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            sums[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sums[g] += fmaf(x[g][2 * e], down, x[g][2 * e + 1] * down);
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
             sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
 #pragma unroll
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
             float mine_sum = 0.0f;
 #pragma unroll
             for (int g = 0; g < G; ++g) mine_sum = c == g ? sums[g] : mine_sum;
-            mine_sum *= down * 0.0078125f;  // 64 * 2^15 at most: 2^-7 brings it into f16
+            mine_sum *= 0.0078125f;  // 64 * 2^15 at most: 2^-7 brings it into f16
             const float high = __half2float(__float2half_rn(mine_sum));
             qsum[nt] = pack_half2(high, mine_sum - high);
         }
@@ -344,7 +345,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, AttnCfg<D, NT>::RESIDENT) kv4_a
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int from = (2 * c + e) * 4;  // a lane that holds row 2 c + e
-            qscale[nt][e] = __shfl_sync(0xffffffffu, up, from) * (16777216.0f * p.scale_log2);
+            // finite for queries of any size: a score is then too, if it fits f32
+            qscale[nt][e] = fmaxf(fminf(__shfl_sync(0xffffffffu, up, from) * (16777216.0f * p.scale_log2), FLT_MAX), -FLT_MAX);
             row_hi[nt][e] = __shfl_sync(0xffffffffu, hi, from);
             row_lo[nt][e] = __shfl_sync(0xffffffffu, lo, from);
         }

@@ -28,6 +28,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 
 #include "../../include/baracuda_kernels_q.h"
 #include "kv4_attention.cuh"
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
             top2 = max_bf16x2(top2, max_bf16x2(max_bf16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), max_bf16x2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
         }
         const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
-        const int ex = top == 0u || top >= 0x7f80u ? 0 : max(-100, min(100, static_cast<int>(top >> 7) - 127 - 14));
+        const int ex = top == 0u || top >= 0x7f80u ? 0 : max(-100, static_cast<int>(top >> 7) - 127 - 14);  // at most 113
         const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
 #pragma unroll 1
         for (int x = 0; x < D / 64; ++x) {
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(PromptCfg<D, NQ>::THREADS, 1) kv4_prompt_kerne
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->qfull);
-        const float factor = fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f);
+        const float factor = fminf(fmaxf(__uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * fabsf(p.scale_log2), 1.0e-37f), FLT_MAX);
 
         // rows of this block that exist see at least [lo_max, hi_min)
         const int last_there = min(all_rows, rt * ROWS + t * 128 + 128) - 1;  // may lie before the block's first row

@@ -913,3 +913,28 @@ def test_attention_of_far_scores_takes_one_key(rows, dim, gain, length):
     lse = top[..., 0] * p.scale
     assert torch.all((got.lse[:rows].double() - lse).abs()[sure] <= (off * p.scale + 2.0 ** -20 * lse.abs())[sure])
     assert bq.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (2, 128), (3, 256), (150, 64), (150, 128), (140, 256)])
+@pytest.mark.parametrize("gain,scale", [(1e36, 1e-37), (5e37, 2e-38), (2e34, 1e-35)])
+def test_attention_of_the_largest_queries(rows, dim, gain, scale):
+    """Queries up to the largest bf16 numbers, under a scale that makes ordinary scores of them."""
+    p = Problem([(rows, 300)], 4, 2, dim, 16, seed=rows, q_gain=1.0, scale=scale)
+    p.q.copy_((p.q.float() * gain).clamp(-3.3e38, 3.3e38))
+    p.q[0, :5] = 3.3e38 if gain == 5e37 else p.q[0, :5]
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (1, 128), (2, 256), (150, 64), (150, 128), (140, 256)])
+def test_the_largest_queries_over_a_single_key(rows, dim):
+    """Queries of 1e36 under the usual scale, scores of either sign: of one key the value comes out."""
+    p = Problem([(rows, 1)], 2, 1, dim, 16, seed=dim, q_gain=1.0, causal=False)
+    p.q.copy_(p.q.float() * 1e36)
+    got = p.run(lse=False)
+    codes, s, m = ref.unpack(p.cache, 16, 1, dim)
+    slot = p.table[0, 0].long() * 16
+    want = ref.values(codes[1, slot, 0], s[1, slot, 0], m[1, slot, 0])
+    torch.cuda.synchronize()
+    err = (got.out[:rows].double().reshape(rows, 2, dim) - want).abs()
+    assert torch.all(err <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * want.abs().amax())
+    assert bq.device_status() == 0
