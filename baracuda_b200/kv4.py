@@ -92,6 +92,8 @@ class Kv4CacheDescriptor:
 
     @property
     def page_bytes(self) -> int:
+        if max(self.page_size, self.heads_kv, self.head_dim) >= 2**31:
+            return 0  # not served
         return int(_lib.load().baracuda_kernels_kv4_page_bytes(self.page_size, self.heads_kv, self.head_dim))
 
 
@@ -185,6 +187,7 @@ class QkNormRopePlan:
             table = (C.c_uint8 * max(1, len(given)))(*given)
         lib = _lib.load()
         if desc.cache is not None:
+            _check_dims(desc.cache.page_size)
             if (desc.cache.heads_kv, desc.cache.head_dim) != (desc.heads_kv, desc.head_dim):
                 raise InvalidProblem("the cache has other heads")
             status_to_result(lib.baracuda_kernels_qk_norm_rope_kv4_append_bf16_sm100a_can_implement(
@@ -364,11 +367,11 @@ class Kv4AttentionPlan:
         _check_backend(pref)
         c = desc.cache
         _check_dims(desc.batch, desc.max_q, desc.max_kv, desc.heads_q, c.heads_kv, c.head_dim, c.page_size, desc.window)
-        scale = c.head_dim ** -0.5 if desc.scale is None else float(desc.scale)
-        if not (abs(scale) < float("inf")):
-            raise InvalidProblem("scale must be finite")
         status_to_result(getattr(_lib.load(), cls._base + "_can_implement")(
             desc.batch, desc.max_q, desc.max_kv, desc.heads_q, c.heads_kv, c.head_dim, c.page_size), cls.__name__)
+        scale = c.head_dim ** -0.5 if desc.scale is None else float(desc.scale)
+        if not abs(scale) <= torch.finfo(torch.float32).max:
+            raise InvalidProblem("scale must be finite, in 32 bits too")
         plan = cls(desc, scale, _check_cache(c))
         if plan.workspace_size() > pref.max_workspace_bytes:
             raise Unsupported("workspace budget too small for this shape")

@@ -182,3 +182,23 @@ def test_the_self_test_of_the_waits_takes_limits_that_let_copies_arrive(qlib):
         assert f(limit) == 2
     for limit in (1 << 20, 1 << 28, 0):
         assert f(limit) == 0
+
+
+def test_plans_refuse_numbers_that_leave_their_types(qlib):
+    """Sizes beyond int32 are not taken modulo 2^32, a head size of zero is refused as such, a scale has to fit f32."""
+    wrap = 1 << 32
+    for cache in (bq.Kv4CacheDescriptor(4, wrap + 16, 2, 128), bq.Kv4CacheDescriptor(wrap, 16, 2, 128)):
+        with pytest.raises(bq.InvalidProblem):
+            bq.QkNormRopePlan.select(None, bq.QkNormRopeDescriptor(1, 8, 2, 128, cache=cache))
+        with pytest.raises(bq.InvalidProblem):
+            bq.Kv4AppendPlan.select(None, bq.Kv4AppendDescriptor(1, cache))
+        with pytest.raises(bq.InvalidProblem):
+            bq.Kv4AttentionPlan.select(None, bq.Kv4AttentionDescriptor(1, 1, 10, 8, cache))
+    for sizes in ((4, wrap + 16, 2, 128), (4, 16, wrap + 2, 128), (4, 16, 2, wrap + 128)):
+        assert bq.Kv4CacheDescriptor(*sizes).page_bytes == 0
+    for head_dim in (0, -64):
+        with pytest.raises(bq.InvalidProblem):
+            bq.Kv4AttentionPlan.select(None, bq.Kv4AttentionDescriptor(1, 1, 10, 8, bq.Kv4CacheDescriptor(4, 16, 2, head_dim)))
+    for scale in (1e39, -1e39, float("inf")):
+        with pytest.raises(bq.InvalidProblem):
+            bq.Kv4AttentionPlan.select(None, bq.Kv4AttentionDescriptor(1, 1, 10, 8, bq.Kv4CacheDescriptor(4, 16, 2, 128), scale=scale))
