@@ -4,9 +4,10 @@
 //   out = bf16(...)                                                 (one rounding, queries and dense keys)
 //   s = f16((max - min) / 15), m = f16(min), c = clamp(rint((x - m) / s), 0, 15)    (per 64 channels of the bf16 keys and values;
 //   max and min cut to +-32768)
-// Every step is one IEEE rounding in f32, in this order.  The mean square of a key is summed as pairs of f32 numbers (about 44
-// bits) and rounded once, so its bits do not depend on the order of the sum and a key next to the border of two codes gets the
-// same code from this kernel, from the two-call sequence and from any other evaluation; of a query it is an f32 sum.
+// Of keys and values every step is one IEEE rounding in f32, in this order, and the mean square of a key is summed as pairs of f32
+// numbers (about 44 bits) and rounded once: its bits do not depend on the order of the sum, and a key next to the border of two
+// codes gets the same code from this kernel, from the two-call sequence and from any other evaluation.  Queries meet no such border:
+// their mean square is an f32 sum, its root's inverse comes at once, and the rotation's products and sums are fused.
 // Bound: bytes (each element read and written once), once the instructions per head are few: a head is D / 16 lanes of 16
 // channels, which contain whole rotation pairs, so nothing is exchanged between lanes but the sums and the groups' extrema; a
 // warp takes twice 512 / D heads of one token, whose sums share their exchanges, division and square root.
@@ -141,11 +142,12 @@ __device__ __forceinline__ float squares(const Lane16& x, float& err) {
     }
 }
 
-// 1 / rms of IT heads per lane group.  The lanes trade heads first: with four, each lane goes on with one after two exchanges, so
-// the other exchanges and the root serve four.  EXACT (keys): division and square root rounded, as the definition says; queries
+// 1 / rms of IT heads per lane group, one or two.  With two the lanes trade halves first: each goes on with one head, so the other
+// exchanges and the root serve both.  EXACT (keys): division and square root rounded, as the definition says; queries
 // take the reciprocal root at once.
 template <int LPH, int IT, bool EXACT>
 __device__ __forceinline__ void inverse_rms(const Lane16 (&x)[IT], float eps, int l, float (&r)[IT]) {
+    static_assert(IT == 1 || IT == 2, "heads trade one exchange");
     float s[IT], e[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) e[i] = 0.0f, s[i] = squares<EXACT>(x[i], e[i]);
@@ -184,8 +186,7 @@ __device__ __forceinline__ void inverse_rms(const Lane16 (&x)[IT], float eps, in
     }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-        const int from = IT == 4 ? (i >> 1) * (LPH / 2) + (i & 1) * (LPH / 4) : IT == 2 ? i * (LPH / 2) : 0;
-        r[i] = IT == 1 ? inv : __shfl_sync(0xffffffffu, inv, from, LPH);
+        r[i] = IT == 1 ? inv : __shfl_sync(0xffffffffu, inv, i * (LPH / 2), LPH);
     }
 }
 
