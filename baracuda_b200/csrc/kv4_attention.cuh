@@ -26,7 +26,7 @@ struct AttnParams {
     int64_t ldo;
     float* lse;
     float scale_log2;  // scale * log2(e)
-    int32_t causal, window;
+    int32_t causal, back;  // keys that a row sees before its last one: the window less 1, 2^31 - 2 without a window
     int32_t batch, total_q, max_q, max_kv, heads_q, group;
     int32_t row_tiles, splits, tile_rows;  // blocks of query rows of a kv head, slices of the keys, rows of a block
     int32_t ctas;                          // of the launch
@@ -73,7 +73,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttnParams& p, int b, int*
 }
 
 // The first key that a row sees whose last one is `last` (negative: before the first).  Nothing here leaves 32 bits, whatever the window.
-__device__ __forceinline__ int first_seen(const AttnParams& p, int last) { return p.window > 0 && last >= p.window ? last - p.window + 1 : 0; }
+__device__ __forceinline__ int first_seen(const AttnParams& p, int last) { return max(last, p.back) - p.back; }
 
 // Shape of a launch: which kernel, its blocks and slices.
 struct AttnShape {

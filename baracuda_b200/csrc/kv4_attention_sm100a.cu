@@ -889,7 +889,7 @@ int32_t launch_kv4_attention(const Kv4AttentionDesc& g, cudaStream_t stream) {
     p.lse = g.lse;
     p.scale_log2 = static_cast<float>(static_cast<double>(g.scale) * 1.4426950408889634);
     p.causal = g.causal;
-    p.window = g.window;
+    p.back = (g.window > 0 ? g.window : 0x7fffffff) - 1;
     p.batch = g.batch;
     p.total_q = g.total_q;
     p.max_q = g.max_q;
