@@ -14,9 +14,13 @@
 //
 // Measured (B200): 4097 tokens of 28 + 4 heads of 128, three axes, dense output: 25.8 us (2.7 TB/s; a plain copy takes 12, this
 // structure without norm and rotation 15); 8191 tokens of 64 + 8 + 8 heads into the cache: 99 us, and 11 to read them back; 5 tokens:
-// 2.8 us.  Reading 65537 tokens of 8 heads: 57 us, 6.0 TB/s.  Half of the issue slots are used: what is left is the chain position
-// -> angles -> product within a warp and the ramp at both ends.  With 8 heads a warp in fragment order, sums of squares from
-// mma.sync and a loop over blocks of heads, the same cases took 29.6 and 131 us: its angles and weights need twice the registers.
+// 2.9 us; 8191 tokens of 8 + 8 heads into the cache as they are: 26.8 us (1.6 TB/s, the values leave by single bytes).  Half of the
+// issue slots are used: what is left is the chain position -> angles -> product within a warp, the ramp at both ends, and spills: the
+// two-head form is held to 64 registers for four resident blocks and loads 210 to 470 bytes a thread back (88 registers, none
+// spilled, for one head).  With 8 heads a warp in fragment order, sums of squares from mma.sync and a loop over blocks of heads, the
+// same cases took 29.6 and 131 us: its angles and weights need twice the registers.
+// Reading 65536 tokens of 8 heads: 56 us, 6.0 TB/s, of one sequence or of several that begin at the same place of a tile; of eight
+// that do not: 138 us, since all but the first are read token by token.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

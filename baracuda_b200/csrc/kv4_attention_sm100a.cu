@@ -21,10 +21,12 @@
 // Warps are joined in shared memory, parts of a block through the workspace by a second kernel (in the order of the keys: the
 // result does not depend on timing).
 //
-// Measured (B200), 32 query and 8 kv heads of 128 unless said: one sequence of 129 tokens 6.2 us; 64 ragged ones up to 4001 tokens
-// (179 MB) 48.8 us, 7 TB/s inside the loop; 2 x 131071 tokens with 64 query heads 64.4 us, 4.7 TB/s over all; 16 x 5 drafted tokens
-// over up to 6001 with 40 heads 49.7 us: 25 rows of a kv head are two blocks of 16, whose products and softmax are the bound.  Blocks of
-// 24 rows spilled and took 41 us against 41 (24 rows, 16 x 6000) and 60 against 54 (48 rows).
+// Measured (B200), 32 query and 8 kv heads of 128 unless said: one sequence of 129 tokens 7 us; 64 ragged ones up to 4001 tokens
+// (179 MB) 49.9 us; 2 x 131071 tokens with 64 query heads 65.7 us, 4.6 TB/s over all; from 64 x 2048 to 64 x 8192 tokens a call grows
+// by 6.4 TB/s, from 2 x 131071 to 2 x 262143 by 6.5, and about 20 us do not depend on the number of keys; 16 x 5 drafted tokens over up
+// to 6001 with 40 heads 50.4 us: 25 rows of a kv head are two blocks of 16, whose products and softmax are the bound.  Blocks of 24 rows
+// spilled more and took 41 us against 41 (24 rows, 16 x 6000) and 60 against 54 (48 rows); D = 128 spills 60 (8 rows, 168 registers) and
+// 80 bytes (16 rows, 255) of loads as it is.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -19,11 +19,12 @@
 // Warps: 4 softmax warps per row block, 8 (D = 256: 16) bring keys and values to f16, one issues the MMAs.
 // Every mbarrier wait is bounded (status 412..416).
 //
-// Measured (B200): 4096 rows x 32 heads on 8, D = 128, causal: 173 us, 0.80 PFLOP/s of the products that the mask leaves.  The tensor
+// Measured (B200): 4096 rows x 32 heads on 8, D = 128, causal: 175 us, 0.78 PFLOP/s of the products that the mask leaves.  The tensor
 // core is busy 38 % of the time: the chain S -> P -> O of a row block takes 4400 clocks a step, 2150 of them the softmax of two
 // warps per quarter of an SM, which share its issue slots with the feeding warps.  2048 rows x 16 heads on 2, D = 256, window
-// 4096: 289 us; there the steps wait for the feeding warps (issue slots 62 % busy; 16 of them: 315 -> 294 us), and the blocks of equal
-// length leave the last wave of three a third full.
+// 4096: 293 us; there the steps wait for the feeding warps (issue slots 62 % busy; 16 of them: 315 -> 294 us), and the blocks of equal
+// length leave the last wave of three a third full.  A sequence of one row among prompts is walked by one CTA per kv head, 18 ns a key:
+// the launcher goes by the longest sequence's rows.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -324,8 +324,9 @@ class Kv4ReadPlan(Kv4AppendPlan):
 # --------------------------------------------------------------------------- attention
 @dataclass(frozen=True)
 class Kv4AttentionDescriptor:
-    """`max_q` and `max_kv` bound the rows and cached tokens of any sequence (what a captured graph may meet); `window` > 0 lets
-    a row see that many keys back, its own included; `scale` defaults to head_dim ** -0.5."""
+    """`max_q` and `max_kv` bound the rows and cached tokens of any sequence (what a captured graph may meet), and the launch is cut
+    for them: prompts and single tokens are better served by a call each.  `window` > 0 lets a row see that many keys back, its own
+    included; `scale` defaults to head_dim ** -0.5."""
     batch: int
     max_q: int
     max_kv: int

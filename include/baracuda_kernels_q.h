@@ -570,10 +570,13 @@ int32_t baracuda_kernels_quantize_per_token_sym_bf16_e4m3_sm100a_run(
  * [batch + 1], any number from 0 to max_q) and kv_lens[b] tokens (int32, 0 to max_kv) in the cache, its own rows' included,
  * on the pages page_table[b][0 ..] (int32, row pitch ld_table >= ceil(max_kv / page_size)).  Row i of n sees key j when
  *   j < kv_lens[b], with causal != 0 also j <= kv_lens[b] - n + i, with window > 0 also j > kv_lens[b] - n + i - window.
- * out = sum_j softmax_j(scale * q . k[j]) v[j], rounded once; a row that sees no key gets zeros.  lse, float
+ * out = sum_j softmax_j(scale * q . k[j]) v[j]; a row that sees no key gets zeros.  Sums and the softmax's statistics are f32.  Rounded
+ * to f16 on the way, 2^-11 each: the weights and, with up to 48 rows of a kv head (32 for head_dim 256) in max_q, their products with
+ * the values' scales; with more rows the cache's keys and values instead; the output to bf16.  lse, float
  * [total_q][heads_q] or NULL, gets log sum_j exp(scale * q . k[j]), minus infinity for such a row.  A NaN key makes the rows that
  * see it NaN, a NaN value at least the channels of its group in them.  Scores may have any size that f32 holds; beyond 2^20, keys
- * whose scores differ by less than their roundings may weigh alike.  Rows outside every sequence are left as they are.  Any max_q and max_kv that hold are right (a captured graph passes its bounds); *_workspace_size goes
+ * whose scores differ by less than their roundings may weigh alike.  Rows outside every sequence are left as they are.
+ * Any max_q and max_kv that hold are right (a captured graph passes its bounds), but the launch is cut for them; *_workspace_size goes
  * by them, and the workspace (16-byte aligned) needs no initialisation; two launches that may overlap need one each.
  * Lengths beyond max_q, max_kv or total_q are cut and reported as device status 403; a page number outside [0, num_pages)
  * where a key is seen leaves its keys out and is reported as 404.
